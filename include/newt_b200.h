@@ -40,7 +40,8 @@ enum nb200_error {
 enum nb200_dtype {
   NB200_F32 = 0,
   NB200_F16 = 1,
-  NB200_BF16 = 2
+  NB200_BF16 = 2,
+  NB200_E4M3 = 3 /* 8-bit floating point, 4 exponent bits; outputs and caches only */
 };
 
 /* Library / ABI identification.  No reference counterpart. */
@@ -289,6 +290,109 @@ int nb200_attention_fwd(const void* q, const void* k, const void* v, void* o,
                         int64_t v_head_stride, int64_t v_row_stride,
                         int64_t o_head_stride, int64_t o_row_stride,
                         float scale, int causal, int dtype, void* stream);
+
+/* ---- root-mean-square norm of rows ------------------------------------------
+ *   h = x + residual (fp32; `residual` null: h = x)
+ *   y = h * rsqrt(mean(h^2) + eps) * w
+ * `out`: y in `dtype` (out_dtype == dtype), or in e4m3 (out_dtype == NB200_E4M3) as y / s with
+ * s = max|y| / 448 over the row (`group` 0) or over each `group` consecutive columns (32, 64 or
+ * 128; the last group of a row may be shorter); s = 1 where that quotient is zero or below the
+ * normal range.  `scales` is [rows, ceil(n / group)], row stride `stride_scales`; null for
+ * 16/32-bit outputs.  `residual_out` (null: not wanted): h in `dtype`.  One rounding per output.
+ * `out` and `residual_out` may be the very tensors x and residual (same base and strides); no
+ * other overlap.  Rows of up to 32768 elements, any alignment (16-byte aligned rows of whole vectors
+ * are faster).  Beside nb200_layernorm; the reference has no
+ * counterpart with a residual or an 8-bit output. */
+int nb200_rmsnorm(const void* x, const void* residual, const void* w, void* out, void* residual_out,
+                  float* scales, int64_t rows, int64_t n, int64_t stride_x, int64_t stride_residual,
+                  int64_t stride_out, int64_t stride_residual_out, int64_t stride_scales,
+                  int64_t group, float eps, int dtype, int out_dtype, void* stream);
+
+/* ---- paged key / value cache in 8 bits ----------------------------------------
+ * Keys and values are e4m3, a page holds `page_size` (16, 32, 64 or 128) consecutive tokens of one
+ * sequence for every head; `head_dim` is 64 or 128 with unit stride.  A value is its e4m3 number
+ * times its page's and head's scale: fp32, [pages, heads], positive, between 2^-60 and 2^60, row
+ * stride `*_scale_stride`, unit stride over heads.  Byte strides of k and v are multiples of 16, their
+ * bases 16-byte aligned; any order of page, head and token will do. */
+typedef struct nb200_kv_cache {
+  void* k;
+  void* v;
+  float* k_scales;
+  float* v_scales;
+  int64_t pages, heads, page_size, head_dim;
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+  int64_t k_scale_stride, v_scale_stride;
+} nb200_kv_cache;
+
+/* Writes new tokens: k, v are [tokens, heads, head_dim] in `dtype` (fp16 or bf16), unit stride over
+ * head_dim.  Sequence b brings rows offsets[b] .. offsets[b + 1) (int32, [batch + 1]) and had
+ * starts[b] (int32) tokens before; token t of a sequence lives in page
+ * page_table[b][t / page_size] (int32, row stride `table_stride`), row t % page_size.
+ * Scales the call writes are powers of two: the smallest one s, 2^-60 <= s <= 2^60, with
+ * max|x| <= 448 s over the new tokens of the page and head; a page that holds older tokens keeps
+ * the larger of that and its old scale, and where the scale grows its older tokens are rewritten
+ * to it.  Values beyond 448 * 2^60 and infinities become the largest value, NaN stays NaN.
+ * `max_new`: at least the largest number of new tokens of one sequence.  Rows behind offsets[batch]
+ * and page rows behind a sequence's last token are left alone; tokens whose page is missing from
+ * the table (beyond max_pages, or not a page of the cache) are not written.  The sequences of one
+ * call must write to different pages.  The call is repeatable: again with the same inputs it
+ * leaves the same cache. */
+int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const void* v, int64_t tokens,
+                    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                    int64_t v_head_stride, const int32_t* page_table, int64_t table_stride,
+                    int64_t max_pages, const int32_t* starts, const int32_t* offsets, int64_t batch,
+                    int64_t max_new, int dtype, void* stream);
+
+/* Attention of the newest `queries` tokens of each sequence over the cache:
+ * q and out are [batch, queries, heads, head_dim] in `dtype` (fp16 or bf16), unit stride over
+ * head_dim; `heads` is a multiple of the cache's heads, neighbouring query heads share one.
+ * lengths[b] (int32) counts the tokens of sequence b in the cache, the new ones among them; query i
+ * stands at position lengths[b] - queries + i and sees the tokens j up to its own position with
+ * j > position - window (`window` 0: all) or j < sinks.  A query that sees nothing (a sequence
+ * shorter than `queries`, an empty one) gives zeros.  Tokens whose page is missing from the table
+ * are not seen.  What lies in page rows that no query of the call sees has no effect, NaN included.
+ * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 14 (fp16)
+ * significant bits.
+ * `workspace`: 16-byte aligned device memory of at least nb200_kv_attention_workspace_bytes(...)
+ * bytes, the caller's; nothing in it needs clearing, and it must not be shared by launches that can
+ * overlap on the GPU.  The lengths stay on the device, so a captured call replays with new ones.
+ * Beside nb200_attention_fwd; the reference has no cache. */
+int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cache, int64_t batch,
+                                           int64_t queries, int64_t heads, int dtype);
+int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, void* out, int64_t batch,
+                       int64_t queries, int64_t heads, int64_t q_batch_stride,
+                       int64_t q_token_stride, int64_t q_head_stride, int64_t o_batch_stride,
+                       int64_t o_token_stride, int64_t o_head_stride, const int32_t* page_table,
+                       int64_t table_stride, int64_t max_pages, const int32_t* lengths, float scale,
+                       int64_t window, int64_t sinks, int dtype, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* ---- log probabilities of given tokens ----------------------------------------
+ * Over rows of `vocab` logits (row stride `stride`, unit stride along the row, any alignment) with
+ * z = logits * inv_temperature:  lse = log sum exp z,  logprob = z[token] - lse,
+ * entropy = lse - sum p z,  and the `top` (0 to 32) largest: top_index (descending by value, ties
+ * to the lower index, NaN lowest) and top_logprob, both [rows, top].  All results are fp32, the
+ * indices int64.  A negative token stands for none: logprob 0; one beyond the vocabulary gives
+ * NaN.  A row of nothing but -inf: logprobs and lse -inf, entropy 0.  A row with NaN or +inf gives NaN.
+ * tokens / logprob, entropy and lse may be null where they are not wanted.  One pass over the row;
+ * results do not depend on the launch's other rows. */
+int nb200_token_logprobs(const void* logits, const int64_t* tokens, float* logprob, float* entropy,
+                         float* lse, float* top_logprob, int64_t* top_index, int64_t rows,
+                         int64_t vocab, int64_t stride, int64_t top, float inv_temperature,
+                         int dtype, void* stream);
+
+/* Its gradient, from the forward pass's lse and entropy:
+ *   grad_logits = inv_temperature * (g ([j = token] - p) - gH p (log p + entropy))
+ * with g = grad_logprob and gH = grad_entropy (either may be null: 0).  A row whose token is
+ * negative or beyond the vocabulary has no part from g; a row masked as a whole (lse below -1e30)
+ * has gradient 0.
+ * grad_logits has the logits' type, one rounding; it may be the logits themselves. */
+int nb200_token_logprobs_bwd(const void* logits, const int64_t* tokens, const float* lse,
+                             const float* entropy, const float* grad_logprob,
+                             const float* grad_entropy, void* grad_logits, int64_t rows,
+                             int64_t vocab, int64_t stride, int64_t stride_out,
+                             float inv_temperature, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

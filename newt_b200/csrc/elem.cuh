@@ -1,0 +1,143 @@
+// Element types as fp32 arithmetic sees them, and 16-byte vectors of them with an element-wise
+// form for rows that are not aligned.  Used by the norm, cache and log-probability kernels.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace nb200 {
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int kPerVec = 4;
+  __device__ static float to_f32(float v) { return v; }
+  __device__ static float from_f32(float v) { return v; }
+};
+template <>
+struct Elem<__half> {
+  static constexpr int kPerVec = 8;
+  __device__ static float to_f32(__half v) { return __half2float(v); }
+  __device__ static __half from_f32(float v) { return __float2half_rn(v); }
+  __device__ static uint32_t pack2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr int kPerVec = 8;
+  __device__ static float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+  __device__ static __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+  __device__ static uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// One 16-byte vector of T, addressable both ways.
+template <typename T>
+union alignas(16) Vec {
+  uint4 raw;
+  T e[Elem<T>::kPerVec];
+};
+
+// Read once: no place in L1.  Not the read-only path, so that a kernel may write its result over
+// the tensor it read it from.
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void st_once(void* p, uint4 v) {
+  asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x),
+               "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+__host__ __device__ __forceinline__ bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The vector of columns [col, col + kPerVec) of a row of n; columns past n give 0.
+// FAST: the row is 16-byte aligned and n a multiple of the vector.
+template <typename T, bool FAST, bool ONCE>
+__device__ __forceinline__ Vec<T> load_row_vec(const T* row, int col, int n) {
+  constexpr int E = Elem<T>::kPerVec;
+  Vec<T> v;
+  if ((FAST || at16(row)) && col + E <= n) {
+    v.raw = ONCE ? ld_once(row + col) : __ldg(reinterpret_cast<const uint4*>(row + col));
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) v.e[j] = (!FAST && col + j < n) ? row[col + j] : Elem<T>::from_f32(0.0f);
+  }
+  return v;
+}
+template <typename T, bool FAST>
+__device__ __forceinline__ Vec<T> load_elems(const T* row, int col, int n) {
+  return load_row_vec<T, FAST, true>(row, col, n);
+}
+template <typename T, bool FAST>
+__device__ __forceinline__ Vec<T> load_cached(const T* row, int col, int n) {
+  return load_row_vec<T, FAST, false>(row, col, n);
+}
+
+// kPerVec fp32 values as one vector of T, each rounded once.
+template <typename T>
+__device__ __forceinline__ Vec<T> round_elems(const float* v) {
+  constexpr int E = Elem<T>::kPerVec;
+  Vec<T> o;
+  if constexpr (sizeof(T) == 2) {
+    uint32_t* words = reinterpret_cast<uint32_t*>(&o.raw);   // two values per conversion
+#pragma unroll
+    for (int j = 0; j < E; j += 2) words[j / 2] = Elem<T>::pack2(v[j], v[j + 1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) o.e[j] = v[j];
+  }
+  return o;
+}
+
+template <typename T, bool FAST>
+__device__ __forceinline__ void store_elems(T* row, int col, int n, const float* v) {
+  constexpr int E = Elem<T>::kPerVec;
+  const Vec<T> o = round_elems<T>(v);
+  if ((FAST || at16(row)) && col + E <= n) {
+    st_once(row + col, o.raw);
+  } else if constexpr (!FAST) {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (col + j < n) row[col + j] = o.e[j];
+  }
+}
+
+// Two fp32 values as e4m3, `lo` in the low byte; beyond +-448 they become +-448, NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+}
+
+// E values times `inv` as e4m3, at columns [col, col + E) of a row of n.
+template <int E, bool FAST>
+__device__ __forceinline__ void store_e4m3(uint8_t* row, int col, int n, const float* v, float inv) {
+  uint32_t words[E / 4];
+#pragma unroll
+  for (int j = 0; j < E; j += 4)
+    words[j / 4] = e4m3x4(v[j] * inv, v[j + 1] * inv, v[j + 2] * inv, v[j + 3] * inv);
+  if ((FAST || reinterpret_cast<uintptr_t>(row) % E == 0) && col + E <= n) {
+    if constexpr (E == 8)
+      *reinterpret_cast<uint2*>(row + col) = make_uint2(words[0], words[1]);
+    else
+      *reinterpret_cast<uint32_t*>(row + col) = words[0];
+  } else if constexpr (!FAST) {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (col + j < n) row[col + j] = (uint8_t)(words[j / 4] >> (8 * (j % 4)));
+  }
+}
+
+}  // namespace nb200

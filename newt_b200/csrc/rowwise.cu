@@ -17,47 +17,12 @@
 // All of this is HBM-bound streaming work; nothing here uses tensor cores.
 
 #include "common.cuh"
+#include "elem.cuh"
 
 namespace nb200 {
 namespace {
 
 constexpr int kWarp = 32;
-
-template <typename T>
-struct Elem;
-template <>
-struct Elem<float> {
-  static constexpr int kPerVec = 4;
-  __device__ static float to_f32(float v) { return v; }
-  __device__ static float from_f32(float v) { return v; }
-};
-template <>
-struct Elem<__half> {
-  static constexpr int kPerVec = 8;
-  __device__ static float to_f32(__half v) { return __half2float(v); }
-  __device__ static __half from_f32(float v) { return __float2half_rn(v); }
-  __device__ static uint32_t pack2(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-};
-template <>
-struct Elem<__nv_bfloat16> {
-  static constexpr int kPerVec = 8;
-  __device__ static float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-  __device__ static __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-  __device__ static uint32_t pack2(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-};
-
-// One 16-byte vector of T, addressable both ways.
-template <typename T>
-union alignas(16) Vec {
-  uint4 raw;
-  T e[Elem<T>::kPerVec];
-};
 
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 r;

@@ -8,12 +8,13 @@ The reference binds libcuda/libnvrtc the same bare-ctypes way
 
 import ctypes
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "libnewt_b200.so")
 
 OK, E_INVALID, E_UNSUPPORTED, E_CUDA, E_DEVICE = range(5)
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 
 
 class KernelLibraryError(RuntimeError):
@@ -45,6 +46,9 @@ class GemmLaunch(ctypes.Structure):
                 ("pair", "block_n", "stages", "ksub", "grid", "block", "cluster", "smem_bytes",
                  "nothing", "only_clear")] + [("reserved", ctypes.c_int32 * 6)]
 
+
+# nb200_kv_cache as bytes: four pointers, then twelve extents and strides
+KV_CACHE = struct.Struct("=4Q12q")
 
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
@@ -86,6 +90,19 @@ SIGNATURES = {
                                         ctypes.c_int, ctypes.POINTER(GemmConfig)]),
     "nb200_attention_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp] + [_i64] * 12 +
                             [ctypes.c_float, ctypes.c_int, ctypes.c_int, _vp]),
+    "nb200_rmsnorm": (ctypes.c_int, [_vp] * 6 + [_i64] * 8 +
+                      [ctypes.c_float, ctypes.c_int, ctypes.c_int, _vp]),
+    "nb200_kv_append": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp] + [_i64] * 5 +
+                        [_vp, _i64, _i64, _vp, _vp, _i64, _i64, ctypes.c_int, _vp]),
+    "nb200_kv_attention_workspace_bytes": (ctypes.c_int64, [ctypes.c_char_p, _i64, _i64, _i64,
+                                                            ctypes.c_int]),
+    "nb200_kv_attention": (ctypes.c_int, [_vp, ctypes.c_char_p, _vp] + [_i64] * 9 +
+                           [_vp, _i64, _i64, _vp, ctypes.c_float, _i64, _i64, ctypes.c_int, _vp,
+                            _i64, _vp]),
+    "nb200_token_logprobs": (ctypes.c_int, [_vp] * 7 + [_i64] * 4 +
+                             [ctypes.c_float, ctypes.c_int, _vp]),
+    "nb200_token_logprobs_bwd": (ctypes.c_int, [_vp] * 7 + [_i64] * 4 +
+                                 [ctypes.c_float, ctypes.c_int, _vp]),
 }
 
 _lib = None
