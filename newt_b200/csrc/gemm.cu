@@ -463,10 +463,14 @@ int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, int ra
   }
   for (int i = 0; i + 1 < rank; ++i) gstr[i] = strides_bytes[i];
   // the payload is moved as raw bits; the element type only sets the size
-  CUresult r = encode(out, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
-                      (cuuint32_t)rank,
-                      const_cast<void*>(base), gdim, gstr, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUtensorMapDataType type = elem_bytes == 4   ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                   : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  CUresult r = encode(out, type, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr, bx, es,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      atom32                       ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
+                      : box[0] * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)

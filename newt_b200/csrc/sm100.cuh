@@ -178,6 +178,15 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                            int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      :
+      : "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
 
 // ---- tcgen05 -----------------------------------------------------------------
 
@@ -218,6 +227,17 @@ __device__ __forceinline__ void mma_tf32_ss(uint32_t d_tmem, uint64_t a_desc, ui
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// The same for 8-bit floating-point operands (32 K-elements per instruction).
+__device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
       :
       : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
@@ -315,6 +335,18 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
 }
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// The same, and the registers the loads were to fill pass through it: whatever is computed from
+// them cannot be moved in front of the wait.
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
+  static_assert(N % 8 == 0, "eight registers at a time");
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+    asm volatile(""
+                 : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]),
+                   "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -463,6 +495,18 @@ __host__ __device__ constexpr uint64_t smem_desc_sw128_atom32(uint32_t lbo_bytes
   return (uint64_t((lbo_bytes >> 4) & 0x3fff) << 16) | (uint64_t((sbo_bytes >> 4) & 0x3fff) << 32) |
          (uint64_t(1) << 46) | (uint64_t(1) << 61);
 }
+// 64-byte swizzle (layout 4): rows of 64 bytes, groups of eight rows SBO = 512 apart; K-major rows
+// are 64 bytes of K, MN-major rows 64 bytes along MN with successive slabs LBO bytes apart.
+__host__ __device__ constexpr uint64_t smem_desc_sw64(uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return (uint64_t((lbo_bytes >> 4) & 0x3fff) << 16) | (uint64_t((sbo_bytes >> 4) & 0x3fff) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(4) << 61);
+}
+// No swizzle, MN-major 8-bit operand: 16 elements along MN by eight of K are 128 contiguous bytes;
+// the next eight of K are LBO bytes on, the next 16 along MN SBO bytes.
+__host__ __device__ constexpr uint64_t smem_desc_plain(uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return (uint64_t((lbo_bytes >> 4) & 0x3fff) << 16) | (uint64_t((sbo_bytes >> 4) & 0x3fff) << 32) |
+         (uint64_t(1) << 46);
+}
 __device__ __forceinline__ uint64_t with_address(uint64_t desc, uint32_t smem_addr) {
   return desc | uint64_t((smem_addr >> 4) & 0x3fff);
 }
@@ -480,6 +524,19 @@ __host__ __device__ constexpr uint32_t instr_desc_f16(int m, int n, bool bf16, b
 __host__ __device__ constexpr uint32_t instr_desc_tf32(int m, int n, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | (2u << 7) | (2u << 10) | ((a_mn_major ? 1u : 0u) << 15) |
          ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+// The same for kind::f8f6f4 with e4m3 operands (A and B format 0).
+__host__ __device__ constexpr uint32_t instr_desc_e4m3(int m, int n, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+// Largest of the warp's 32 values (NaN is passed over), in every lane.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 // three-input maximum and packed two-wide fp32 arithmetic (one issue slot for two values)
@@ -548,8 +605,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
 #ifndef __CUDACC_RTC__
 // ---- host: tensor maps ---------------------------------------------------------
 
-// Encodes a tiled tensor map of 16- or 32-bit elements with 128-byte swizzle and zero fill
-// (`atom32`: the swizzle's 32-byte-atom form, for MN-major tf32 operands).
+// Encodes a tiled tensor map of 8-, 16- or 32-bit elements with 128-byte swizzle (64-byte where the
+// box is 64 bytes wide) and zero fill (`atom32`: the 128-byte swizzle's 32-byte-atom form, for
+// MN-major tf32 operands).
 // dims/strides are given innermost first; `strides_bytes` has rank-1 entries.
 // Returns 0 or an NB200_E_* code (message recorded).
 int encode_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, int rank,
