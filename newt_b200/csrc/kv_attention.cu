@@ -46,11 +46,15 @@ constexpr int kTile = 128;               // tokens
 constexpr int kThreads = 192;            // producer, issuer, four softmax warps
 constexpr int kSoftmaxWarp = 2;
 constexpr int kJoinThreads = 512;
+constexpr int kMinShare = 2;             // tiles
+constexpr int kWholeItems = 4;           // tiles
+constexpr int kMaxShares = kJoinThreads;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeastScale = 8.67361738e-19f;   // 2^-60
 constexpr float kProbScale = 256.0f;     // probabilities of a tile are at most 1
 
 enum : unsigned int {
-  ST_KV_Q = 32, ST_KV_K, ST_KV_V, ST_KV_EMPTY, ST_KV_S, ST_KV_P, ST_KV_O, ST_KV_ZERO
+  ST_KV_Q = 32, ST_KV_K, ST_KV_V, ST_KV_EMPTY, ST_KV_SCALES, ST_KV_S, ST_KV_P, ST_KV_O, ST_KV_ZERO
 };
 
 struct KvAttnParams {
@@ -65,8 +69,8 @@ struct KvAttnParams {
   int64_t table_stride, k_scale_stride, v_scale_stride;
   int batch, nq, kv_heads, group;        // group: query heads per key head
   int rows, row_tiles;                   // nq * group, and how many pieces of RP rows
-  int pages, page, max_pages, window, sinks;
-  int shares, min_share, q_aligned;
+  int pages, page, page_shift, max_pages, window, sinks;
+  int shares, q_aligned;
   float scale;
   unsigned long long wait_limit_ns;
   unsigned int* status;
@@ -82,7 +86,7 @@ __device__ __forceinline__ Seq make_seq(const KvAttnParams& p, int len) {
   Seq s;
   len = max(len, 0);
   s.len = len;
-  s.limit = max(min(len, p.max_pages * p.page), 0);
+  s.limit = min(len, p.max_pages << p.page_shift);
   s.low = p.window ? max(max(len, p.nq) - p.nq + 1 - p.window, 0) : 0;   // of the first query there is
   s.sink_end = min(p.sinks, s.limit);
   const int tiles = (s.limit + kTile - 1) / kTile;
@@ -107,88 +111,111 @@ __device__ __forceinline__ bool seen_by_any(const Seq& s, int token) {
   return token < s.limit && (token >= s.low || token < s.sink_end);
 }
 
-// Running totals of the sequences' tiles, by stretches of sequences: thread i sums one stretch.
-// Leaves the totals before each stretch in `before` [threads + 1]; everyone gets the sum.
-// `warp_sum`: one number per warp.
-__device__ __forceinline__ long long scan_sequences(const KvAttnParams& p, long long* before,
-                                                    long long* warp_sum, int threads) {
-  const int stretch = (p.batch + threads - 1) / threads;
-  const int tid = threadIdx.x, lane = tid & 31;
-  long long sum = 0;
-  for (int i = 0; i < stretch; ++i) {
-    const int b = tid * stretch + i;
-    if (b < p.batch) sum += make_seq(p, p.lengths[b]).count;
-  }
-  long long run = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long other = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += other;
-  }
-  if (lane == 31) warp_sum[tid >> 5] = run;
-  __syncthreads();
-  for (int w = 0; w < (tid >> 5); ++w) run += warp_sum[w];
-  before[tid + 1] = run;
-  if (tid == 0) before[0] = 0;
-  __syncthreads();
-  return before[threads] * p.row_tiles * p.kv_heads;
-}
-
 // Where in the work list a tile is: sequence, item of the sequence (key head, row tile), tile.
 struct Place {
-  int b, item, tile;
+  int b, head, row_tile, tile;
 };
-__device__ __forceinline__ Place locate(const KvAttnParams& p, const long long* before, int threads,
-                                        long long flat) {
-  const int per_seq = p.row_tiles * p.kv_heads;
-  const int stretch = (p.batch + threads - 1) / threads;
-  int lo = 0, hi = threads;                        // before[lo] * per_seq <= flat < before[hi] * per_seq
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (before[mid] * per_seq <= flat) lo = mid; else hi = mid;
+
+// The work list as one warp sees it: lane i knows how many tiles a stretch of the sequences has and
+// how many come before it.  All lanes take part in every call.
+struct WorkList {
+  int stretch, before, sum;   // of this lane's stretch, for one (key head, row tile)
+  int total, largest;         // of all: tiles of one (key head, row tile), most of one sequence
+  int per_seq;
+
+  __device__ WorkList(const KvAttnParams& p) {
+    const int lane = threadIdx.x & 31;
+    per_seq = p.row_tiles * p.kv_heads;
+    stretch = (p.batch + 31) / 32;
+    sum = largest = 0;
+    for (int i = 0; i < stretch; ++i) {
+      const int b = lane * stretch + i;
+      if (b < p.batch) {
+        const int count = make_seq(p, __ldg(p.lengths + b)).count;
+        sum += count;
+        largest = max(largest, count);
+      }
+    }
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += other;
+    }
+    before = run - sum;
+    total = __shfl_sync(0xffffffffu, run, 31);
+    largest = __reduce_max_sync(0xffffffffu, largest);
   }
-  long long at = before[lo] * per_seq;
-  int b = lo * stretch;
-  int count = make_seq(p, p.lengths[b]).count;
-  while (flat >= at + (long long)count * per_seq) {
-    at += (long long)count * per_seq;
-    ++b;
-    count = make_seq(p, p.lengths[b]).count;
+  __device__ int tiles() const { return total * per_seq; }
+
+  // Shares of whole items where all are short (a cut would cost more than it evens out: below),
+  // of tiles otherwise.
+  __device__ bool whole_items() const { return largest <= kWholeItems; }
+
+  // first tile of share c, from 0 to tiles(); the same c in all lanes
+  __device__ int share_start(const KvAttnParams& p, int c) const {
+    if (!whole_items()) {
+      const int share = max((tiles() + p.shares - 1) / p.shares, kMinShare);
+      return (int)min((long long)c * share, (long long)tiles());
+    }
+    const int items = p.batch * per_seq;
+    const int i = (int)((long long)items * c / p.shares);
+    if (i >= items) return tiles();
+    const int b = i / per_seq, owner = b / stretch;
+    int at = __shfl_sync(0xffffffffu, before, owner);
+    for (int k = owner * stretch; k < b; ++k) at += make_seq(p, __ldg(p.lengths + k)).count;
+    return at * per_seq + (i - b * per_seq) * make_seq(p, __ldg(p.lengths + b)).count;
   }
-  Place w;
-  w.b = b;
-  w.item = (int)((flat - at) / count);
-  w.tile = (int)((flat - at) % count);
-  return w;
-}
-__device__ __forceinline__ long long share_of(const KvAttnParams& p, long long total) {
-  const long long share = (total + p.shares - 1) / p.shares;
-  return share > p.min_share ? share : p.min_share;
-}
+
+  // The place of a tile, 0 <= flat < tiles(), a tile of its own for every lane if need be.
+  __device__ Place locate(const KvAttnParams& p, int flat) const {
+    const int q = flat / per_seq;            // at * per_seq <= flat  <=>  at <= flat / per_seq
+    int owner = 0;
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1)
+      if (__shfl_sync(0xffffffffu, before, owner + step) <= q) owner += step;
+    int at = __shfl_sync(0xffffffffu, before, owner);
+    int b = owner * stretch;
+    int count = make_seq(p, __ldg(p.lengths + b)).count;
+    while (q >= at + count) {
+      at += count;
+      ++b;
+      count = make_seq(p, __ldg(p.lengths + b)).count;
+    }
+    flat -= at * per_seq;
+    const int item = flat / count;
+    return Place{b, item / p.row_tiles, item % p.row_tiles, flat % count};
+  }
+};
 
 // A walk over a share of the work list.
 struct Cursor {
   Place at;
   Seq seq;
-  long long left;      // tiles, this one among them
-  __device__ void start(const KvAttnParams& p, const Place& w, long long tiles) {
+  int left;      // tiles, this one among them
+  __device__ void start(const KvAttnParams& p, const Place& w, int tiles) {
     left = tiles;
-    at = Place{0, 0, 0};               // an empty share has no place
+    at = Place{0, 0, 0, 0};            // an empty share has no place
     if (left <= 0) return;
     at = w;
     seq = make_seq(p, __ldg(p.lengths + at.b));
   }
-  __device__ int head(const KvAttnParams& p) const { return at.item / p.row_tiles; }
-  __device__ int row_tile(const KvAttnParams& p) const { return at.item % p.row_tiles; }
   __device__ bool last_tile() const { return at.tile == seq.count - 1; }
-  __device__ void next(const KvAttnParams& p) {
-    --left;
-    if (++at.tile < seq.count) return;
-    at.tile = 0;
-    if (++at.item < p.row_tiles * p.kv_heads) return;
-    at.item = 0;
+  __device__ void next_item(const KvAttnParams& p) {
+    if (++at.row_tile < p.row_tiles) return;
+    at.row_tile = 0;
+    if (++at.head < p.kv_heads) return;
+    at.head = 0;
     ++at.b;
-    if (left > 0) seq = make_seq(p, __ldg(p.lengths + at.b));
+    seq = make_seq(p, __ldg(p.lengths + at.b));
+  }
+  __device__ void advance(const KvAttnParams& p, int tiles) {
+    left -= tiles;
+    at.tile += tiles;
+    while (left > 0 && at.tile >= seq.count) {
+      at.tile -= seq.count;
+      next_item(p);
+    }
   }
 };
 
@@ -197,25 +224,25 @@ struct Shape {
   static constexpr int kN = (RP * PARTS + 15) / 16 * 16;
   static constexpr int kTileBytes = kTile * D;                    // one K or V tile
   // ring of K0 V0 K1 V1 ...: what two CTAs per SM leave room for
-  static constexpr int kSlots = D == 128 ? (kN >= 48 ? 4 : 6) : (kN >= 64 ? 8 : 12);
+  static constexpr int kSlots = D == 128 ? (kN >= 32 ? 4 : 6) : (kN >= 48 ? 10 : 12);
   static constexpr int kQBytes = kN * D;
   static constexpr int kPBytes = kN * kTile;
-  static constexpr int kTmemCols = 3 * kN <= 64 ? 64 : 3 * kN <= 128 ? 128 : 256;
+  static constexpr int kTmemCols = 4 * kN <= 64 ? 64 : 4 * kN <= 128 ? 128 : 256;
 };
 
 template <int D, int RP, int PARTS>
 struct Shared {
   using S = Shape<D, RP, PARTS>;
   uint8_t ring[S::kSlots][S::kTileBytes];      // first: the swizzle counts from 1024-byte boundaries
-  uint8_t p[S::kPBytes];
+  uint8_t p[2][S::kPBytes];
   uint8_t q[2][S::kQBytes];
+  float4 scale[4][32];                         // of a step's pages: ks, log2 vs, 1 / vs, 1 if it is there
   float q_factor[2][RP];                       // what takes a row's product to log2 units
   int q_at[2][RP];                             // position of the row's query; -1: no such row
-  float most[2][RP][4];                        // the warps' maxima, alternating by tile
-  float sum[RP][4];
-  uint64_t full[S::kSlots], empty[S::kSlots], q_full[2], s_full[2], p_full, o_full;
-  long long before[kThreads + 1], warp_sum[kThreads / 32];
-  Place start;
+  float most[2][4][RP];                        // the warps' maxima, alternating by tile
+  float sum[4][RP];
+  uint64_t full[S::kSlots], empty[S::kSlots], scale_full[4];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
   uint32_t tmem_slot, abort_flag;
 };
 
@@ -255,12 +282,12 @@ struct Queries {
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       const int v = i * 128 + tid;
-      const int r = c.row_tile(p) * RP + v / kPerRow;
+      const int r = c.at.row_tile * RP + v / kPerRow;
       raw[i].raw = make_uint4(0, 0, 0, 0);
       if (v / kPerRow >= RP || r >= p.rows) continue;
       const T* src = static_cast<const T*>(p.q) + c.at.b * p.q_batch_stride +
                      r / p.group * p.q_token_stride +
-                     (c.head(p) * p.group + r % p.group) * p.q_head_stride + v % kPerRow * 8;
+                     (c.at.head * p.group + r % p.group) * p.q_head_stride + v % kPerRow * 8;
       if (p.q_aligned) {
         raw[i].raw = __ldg(reinterpret_cast<const uint4*>(src));
       } else {
@@ -297,7 +324,7 @@ struct Queries {
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
       if (r < RP) {
         if (col8 == 0) {
-          const int row = c.row_tile(p) * RP + r;
+          const int row = c.at.row_tile * RP + r;
           factor[r] = bad ? NAN : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale * kLog2e);
           at[r] = row < p.rows ? c.seq.len - p.nq + row / p.group : -1;
         }
@@ -335,66 +362,103 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(smem_u32(&sh.full[x]), 1);
       mbar_init(smem_u32(&sh.empty[x]), 1);
     }
+    for (int x = 0; x < 4; ++x) mbar_init(smem_u32(&sh.scale_full[x]), 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_u32(&sh.q_full[x]), 4);   // one arrival per softmax warp
       mbar_init(smem_u32(&sh.s_full[x]), 1);
+      mbar_init(smem_u32(&sh.p_full[x]), 4);
+      mbar_init(smem_u32(&sh.o_full[x]), 1);
     }
-    mbar_init(smem_u32(&sh.p_full), 4);
-    mbar_init(smem_u32(&sh.o_full), 1);
     mbar_init_fence();
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
   }
-  if (warp == 1) {
-    __syncwarp();
-    tmem_alloc(smem_u32(&sh.tmem_slot), S::kTmemCols);
-  }
-  const long long total = scan_sequences(p, sh.before, sh.warp_sum, kThreads);
-  const long long share = share_of(p, total);
-  const long long from = blockIdx.x * share;
-  const long long tiles = min(share, max(total - from, 0ll));
-  if (threadIdx.x == 0 && tiles > 0) sh.start = locate(p, sh.before, kThreads, from);
+  __syncwarp();
+  if (warp == 1) tmem_alloc(smem_u32(&sh.tmem_slot), S::kTmemCols);
+  // every warp finds the share's place for itself
+  const WorkList list(p);
+  const int from = list.share_start(p, blockIdx.x), to = list.share_start(p, blockIdx.x + 1);
+  Cursor c;
+  c.start(p, to > from ? list.locate(p, from) : Place{0, 0, 0, 0}, to - from);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_slot;
 
-  Cursor c;
-  c.start(p, sh.start, tiles);
-
   if (warp == 0) {
-    // ---- producer: each lane fetches one page of the tile ----
-    const int per_tile = kTile / p.page;
+    // ---- producer ----
+    // It works in steps of 32 pages, a lane per page: pages are looked up two steps ahead and their
+    // scales fetched one step ahead, so that neither latency is met per tile.  The scales go to the
+    // softmax warps through four turns of shared memory: a step begins when the ring has room for
+    // it, that is when all but the ring's tiles before it are done with, and the ring has at most
+    // 6 tiles where three steps have at least 12.
+    static_assert(SLOTS / 2 <= 12, "a turn of the scales would be overwritten too early");
+    const int per_tile = kTile >> p.page_shift, step_tiles = 32 / per_tile;
     const uint32_t page_bytes = (uint32_t)p.page * D;
-    bool ok = true;
-    int g = 0;                        // tiles of K and V so far: ring position
-    auto page_of = [&](const Cursor& at) {       // this lane's page of a tile, -1: not to be read
-      if (at.left <= 0 || lane >= per_tile) return -1;
-      const int token = tile_start(at.seq, at.at.tile) + lane * p.page;
+    const int my_tile = lane / per_tile, my_page = lane % per_tile;
+    Cursor mine = c;
+    auto page_of = [&](Cursor& at) {             // this lane's page, -1: not to be read
+      if (at.left <= 0) return -1;
+      const int token = tile_start(at.seq, at.at.tile) + (my_page << p.page_shift);
       if (!(token < at.seq.limit && (token + p.page > at.seq.low || token < at.seq.sink_end))) return -1;
-      const int id = __ldg(p.table + at.at.b * p.table_stride + token / p.page);
+      const int id = __ldg(p.table + at.at.b * p.table_stride + (token >> p.page_shift));
       return id >= 0 && id < p.pages ? id : -1;
     };
-    int id = page_of(c);
-    while (c.left > 0 && ok) {
-      const int head = c.head(p);
-      c.next(p);
-      const int ahead = page_of(c);   // the next tile's, under way while this one is issued
-      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, id >= 0)) * page_bytes;
+    // of this step, the next one and the one after
+    float ks[2], vs[2];
+    int id[3], head[3];
+    auto fetch_scales = [&](int page, int of_head, float& k_scale, float& v_scale) {
+      k_scale = page >= 0 ? __ldg(p.k_scales + page * p.k_scale_stride + of_head) : 0.0f;
+      v_scale = page >= 0 ? __ldg(p.v_scales + page * p.v_scale_stride + of_head) : 1.0f;
+    };
+    if (c.left > 0) mine.advance(p, my_tile);
+    id[0] = page_of(mine);
+    head[0] = mine.at.head;
+    if (mine.left > 0) mine.advance(p, step_tiles);
+    id[1] = page_of(mine);
+    head[1] = mine.at.head;
+    fetch_scales(id[0], head[0], ks[0], vs[0]);
+    bool ok = true;
+    int left = c.left;
+    for (int step = 0; left > 0 && ok; ++step) {
+      // the next step's scales and the one after's pages are under way while this one is issued
+      fetch_scales(id[1], head[1], ks[1], vs[1]);
+      if (mine.left > 0) mine.advance(p, step_tiles);
+      id[2] = page_of(mine);
+      head[2] = mine.at.head;
+      bool handed = false;
+      for (int k = 0; k < step_tiles && left > 0 && ok; ++k, --left) {
+        const int j = step * step_tiles + k;
+        const bool in_tile = my_tile == k && id[0] >= 0;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, in_tile)) * page_bytes;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv, ++g) {
-        const int x = g % SLOTS;
-        ok = ok && mbar_wait_nocall(smem_u32(&sh.empty[x]), ((g / SLOTS) & 1) ^ 1, ctx, ST_KV_EMPTY, g);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&sh.full[x]);
-        if (lane == 0) {
-          if (bytes) mbar_arrive_expect_tx(bar, bytes); else mbar_arrive(bar);
+        for (int kv = 0; kv < 2; ++kv) {
+          const int g = 2 * j + kv, x = g % SLOTS;
+          ok = ok && mbar_wait_nocall(smem_u32(&sh.empty[x]), ((g / SLOTS) & 1) ^ 1, ctx, ST_KV_EMPTY, g);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&sh.full[x]);
+          if (lane == 0) {
+            if (bytes) mbar_arrive_expect_tx(bar, bytes); else mbar_arrive(bar);
+          }
+          __syncwarp();
+          if (in_tile)
+            tma_load_4d(smem_u32(&sh.ring[x][my_page * page_bytes]), kv ? &map_v : &map_k, 0, 0, head[0], id[0], bar);
         }
-        __syncwarp();
-        if (id >= 0) tma_load_4d(smem_u32(&sh.ring[x][lane * page_bytes]), kv ? &map_v : &map_k, 0, 0, head, id, bar);
+        if (!handed) {                           // behind the first tile's copies
+          if (vs[0] < kLeastScale) vs[0] = kLeastScale;   // its logarithm is used; NaN stays
+          sh.scale[step & 3][lane] = make_float4(ks[0], __log2f(vs[0]), 1.0f / vs[0], id[0] >= 0 ? 1.0f : 0.0f);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.scale_full[step & 3]));
+          handed = true;
+        }
       }
-      id = ahead;
+      id[0] = id[1];
+      head[0] = head[1];
+      ks[0] = ks[1];
+      vs[0] = vs[1];
+      id[1] = id[2];
+      head[1] = head[2];
     }
   } else if (warp == 1) {
     // ---- issuer ----
@@ -433,24 +497,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (c.left > 0) begin(0, true);
     for (int j = 0; c.left > 0 && ok; ++j) {
       const bool ends = c.last_tile();
-      c.next(p);
+      c.advance(p, 1);
       if (c.left > 0) {
         if (ends) ++item;
         begin(j + 1, ends);
       }
       const int x = (2 * j + 1) % SLOTS;
       ok = ok && wait_all(&sh.full[x], ((2 * j + 1) / SLOTS) & 1, ST_KV_V, j);
-      ok = ok && wait_all(&sh.p_full, j & 1, ST_KV_P, j);
+      ok = ok && wait_all(&sh.p_full[j & 1], (j >> 1) & 1, ST_KV_P, j);
       if (!ok) break;
       tc_fence_after_sync();
-      const uint32_t vb = smem_u32(sh.ring[x]), pb = smem_u32(sh.p);
+      const uint32_t vb = smem_u32(sh.ring[x]), pb = smem_u32(sh.p[j & 1]);
 #pragma unroll
       for (int kk = 0; kk < kTile / 32; ++kk)      // 32 tokens: four groups of eight rows
         if (elected)
-          mma_f8_ss(tmem + 2 * N, with_address(kVDesc, vb + kk * 32 * D),
+          mma_f8_ss(tmem + (2 + (j & 1)) * N, with_address(kVDesc, vb + kk * 32 * D),
                     with_address(kPDesc, pb + kk * 4 * 128), kIdescPv, kk != 0);
       if (elected) {
-        mma_commit(smem_u32(&sh.o_full));
+        mma_commit(smem_u32(&sh.o_full[j & 1]));
         mma_commit(smem_u32(&sh.empty[x]));
       }
       __syncwarp();
@@ -463,81 +527,70 @@ __global__ void __launch_bounds__(kThreads, 2)
     bool ok = true;
 
     Queries<T, D, RP, PARTS> queries;
-    if (c.left > 0) queries.load(p, c, me);
-    // the scales of a token's page: two steps ahead the page, one step ahead its scales
-    auto page_id = [&](const Cursor& at) {
-      if (at.left <= 0) return -1;
-      const int token = tile_start(at.seq, at.at.tile) + me;
-      if (!seen_by_any(at.seq, token)) return -1;
-      const int id = __ldg(p.table + at.at.b * p.table_stride + token / p.page);
-      return id >= 0 && id < p.pages ? id : -1;
-    };
-    float ks = 0.0f, vs = 1.0f;
-    auto fetch_scales = [&](int id, int head, float& k_scale, float& v_scale) {
-      k_scale = id >= 0 ? __ldg(p.k_scales + id * p.k_scale_stride + head) : 0.0f;
-      v_scale = id >= 0 ? __ldg(p.v_scales + id * p.v_scale_stride + head) : 1.0f;
-    };
-    Cursor ahead = c;
-    int id = page_id(c);
-    int ahead_id = -1, ahead_head = 0;
     if (c.left > 0) {
-      ahead.next(p);
-      ahead_id = page_id(ahead);
-      if (ahead.left > 0) ahead_head = ahead.head(p);
+      queries.load(p, c, me);
       queries.stage(p, c, me, sh.q[0], sh.q_factor[0], sh.q_at[0]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[0]));
       all_of_group(true);            // the rows' factors and positions are written
     }
-    fetch_scales(id, c.left > 0 ? c.head(p) : 0, ks, vs);
 
     int item = 0;
-    bool whole = c.left > 0 && c.at.tile == 0;     // has the item's first tile
+    bool whole = c.at.tile == 0;                   // has the item's first tile
     bool first_part = true;                        // the item that the share begins with
-    float acc[RP], l[RP], m[RP];                   // m: log2 units
+    float acc[RP], l[RP], m[RP], now[RP];          // m: log2 units
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
-      acc[r] = l[r] = 0.0f;
+      acc[r] = l[r] = now[r] = 0.0f;
       m[r] = -INFINITY;
     }
-    for (int j = 0; c.left > 0; ++j) {
-      // what the next tile needs, on its way
-      const int next_id = ahead_id, next_head = ahead_head;
-      float next_ks, next_vs;
-      fetch_scales(next_id, next_head, next_ks, next_vs);
-      if (ahead.left > 0) {
-        ahead.next(p);
-        ahead_id = page_id(ahead);
-        if (ahead.left > 0) ahead_head = ahead.head(p);
+    // the product of tile j joins the sums with the factors that its own step left in `now`
+    auto add_product = [&](int j) {
+      ok = ok && mbar_wait_nocall(smem_u32(&sh.o_full[j & 1]), (j >> 1) & 1, ctx, ST_KV_O, j);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after_sync();
+      uint32_t raw[N];
+#pragma unroll
+      for (int n = 0; n < N; n += 16)
+        tmem_ld_32x32(tmem + lane_base + (2 + (j & 1)) * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
+      tmem_ld_wait(raw);
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
+#pragma unroll
+        for (int part = PARTS - 2; part >= 0; --part)
+          v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
+        acc[r] = fmaf(v, now[r], acc[r]);
       }
-      // the next item's queries, too: loaded at the start of an item, staged behind its first tile
-      const bool item_begins = j == 0 || c.at.tile == 0;
+    };
+    bool pending = false;                          // a product of this item has not joined yet
+    for (int j = 0; c.left > 0; ++j) {
+      // the next item's queries: loaded at the start of an item, staged behind its first tile
+      const int skip = c.seq.count - c.at.tile;    // tiles to the next item
+      const bool stage_next = (j == 0 || c.at.tile == 0) && c.left > skip;
       Cursor next_item = c;
-      bool stage_next = false;
-      if (item_begins) {
-        const int skip = c.seq.count - c.at.tile;  // tiles to the next item
-        if (c.left > skip) {
-          next_item.at.tile = c.seq.count - 1;
-          next_item.left = c.left - skip + 1;
-          next_item.next(p);
-          stage_next = true;
-          queries.load(p, next_item, me);
-        }
+      if (stage_next) {
+        next_item.advance(p, skip);
+        queries.load(p, next_item, me);
       }
 
       const int x = j & 1;
       const int t0 = tile_start(c.seq, c.at.tile);
       const int token = t0 + me;
-      const bool there = id >= 0;                  // seen by some query, and its page is there
-      // every query sees the whole tile: no masks but `there`
-      const int first_at = c.seq.len - p.nq;
-      const bool clean = t0 + kTile - 1 <= first_at &&
+      // every query sees the whole tile: no masks but whether the page is there
+      const bool clean = t0 + kTile <= c.seq.limit && t0 + kTile - 1 <= c.seq.len - p.nq &&
                          (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTile <= p.sinks);
-      float s[RP];
+      const int step = (unsigned)j >> (p.page_shift - 2);    // 32 pages: 2^(shift - 2) tiles
+      ok = ok && mbar_wait_nocall(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j);
       ok = ok && mbar_wait_nocall(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
       ok = __all_sync(0xffffffffu, ok);
-      const float lv = log2f(vs);
+      const float4 scale = sh.scale[step & 3][((j << (7 - p.page_shift)) + (me >> p.page_shift)) & 31];
+      const float lv = scale.y, inv_vs = scale.z;
+      // seen by some query, and its page is there
+      const bool there = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
+      float s[RP];
       if (ok) {
         tc_fence_after_sync();
         uint32_t raw[N];
@@ -545,62 +598,57 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int n = 0; n < N; n += 16)
           tmem_ld_32x32(tmem + lane_base + x * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
         tmem_ld_wait(raw);
-        const float* factor = sh.q_factor[item & 1];
+        float w[RP];
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
           float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
 #pragma unroll
           for (int part = PARTS - 2; part >= 0; --part)
             v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
-          s[r] = there ? v * (factor[r] * ks) : -INFINITY;
+          s[r] = there ? fmaf(v, sh.q_factor[item & 1][r] * scale.x, lv) : -INFINITY;
         }
-        if (!clean) {
+        if (!clean || p.rows < RP * p.row_tiles) {   // tokens that some rows do not see, rows that only pad
           const int* at = sh.q_at[item & 1];
 #pragma unroll
           for (int r = 0; r < RP; ++r) {
             const bool seen = token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks);
             if (!seen) s[r] = -INFINITY;
           }
-        } else if (p.rows < RP * p.row_tiles) {    // rows that only pad
-#pragma unroll
-          for (int r = 0; r < RP; ++r)
-            if (sh.q_at[item & 1][r] < 0) s[r] = -INFINITY;
         }
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float w = warp_max(s[r] + lv);
-          if (lane == 0) sh.most[x][r][quarter] = w;
+        for (int r = 0; r < RP; ++r) w[r] = warp_max(s[r]);
+        if (lane == 0) {
+#pragma unroll
+          for (int r = 0; r < RP; r += 4)
+            *reinterpret_cast<float4*>(&sh.most[x][quarter][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
         }
       }
       if (!all_of_group(ok)) break;
       float mt[RP];
-      uint32_t bytes[PARTS][RP / 4];
-      const float inv_vs = 1.0f / vs;
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        const float4 w = *reinterpret_cast<const float4*>(sh.most[x][r]);
-        mt[r] = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
+      for (int r = 0; r < RP; r += 4) {
+        float4 w = *reinterpret_cast<const float4*>(&sh.most[x][0][r]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+          const float4 o = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
+          w = make_float4(fmaxf(w.x, o.x), fmaxf(w.y, o.y), fmaxf(w.z, o.z), fmaxf(w.w, o.w));
+        }
+        mt[r] = w.x;
+        mt[r + 1] = w.y;
+        mt[r + 2] = w.z;
+        mt[r + 3] = w.w;
       }
+      // probabilities relative to the tile's maximum (0 where the row sees nothing of it), in parts
+      uint32_t bytes[PARTS][RP / 4];
+      float pr[RP];
+#pragma unroll
+      for (int r = 0; r < RP; ++r) pr[r] = exp2_approx(s[r] - (mt[r] == -INFINITY ? 0.0f : mt[r]));
 #pragma unroll
       for (int r = 0; r < RP; r += 2) {
-        float pr[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float ref = mt[r + h] == -INFINITY ? 0.0f : mt[r + h];
-          pr[h] = exp2_approx(s[r + h] + lv - ref);
-          // the running sums move to the larger of the two references
-          const float top = fmaxf(m[r + h], ref);
-          const float old = m[r + h] == -INFINITY ? 0.0f : exp2_approx(m[r + h] - top);
-          const float now = mt[r + h] == -INFINITY ? 0.0f : exp2_approx(ref - top);
-          if (mt[r + h] != -INFINITY) m[r + h] = top;
-          l[r + h] = mt[r + h] == -INFINITY ? l[r + h] : fmaf(pr[h] * inv_vs, now, l[r + h] * old);
-          acc[r + h] = mt[r + h] == -INFINITY ? acc[r + h] : acc[r + h] * old;
-          mt[r + h] = now * (1.0f / kProbScale);   // from here on: the tile's factor
-          pr[h] *= kProbScale;
-        }
+        float a = pr[r] * kProbScale, b = pr[r + 1] * kProbScale;
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) {
-          const uint32_t q = split2(pr[0], pr[1]);
+          const uint32_t q = split2(a, b);
           if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
         }
       }
@@ -613,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int at = (n + 4 * i) / RP, r = (n + 4 * i) % RP;
           w[i] = at < PARTS ? bytes[at < PARTS ? at : 0][r / 4] : 0u;
         }
-        st_shared_v4(smem_u32(sh.p) + (n / 16) * (kTile * 16) + me * 16, w[0], w[1], w[2], w[3]);
+        st_shared_v4(smem_u32(sh.p[x]) + (n / 16) * (kTile * 16) + me * 16, w[0], w[1], w[2], w[3]);
       }
       if (__any_sync(0xffffffffu, !there)) {
         const int g = 2 * j + 1;
@@ -627,57 +675,54 @@ __global__ void __launch_bounds__(kThreads, 2)
       fence_proxy_async_smem();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
+      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[x]));
 
       if (stage_next) {
-        queries.stage(p, next_item, me, sh.q[(item + 1) & 1], sh.q_factor[(item + 1) & 1], sh.q_at[(item + 1) & 1]);
+        const int y = (item + 1) & 1;
+        queries.stage(p, next_item, me, sh.q[y], sh.q_factor[y], sh.q_at[y]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[(item + 1) & 1]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[y]));
       }
 
-      ok = ok && mbar_wait_nocall(smem_u32(&sh.o_full), j & 1, ctx, ST_KV_O, j);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        tc_fence_after_sync();
-        uint32_t raw[N];
+      // the tile before joins the sums while the tensor core works on this one; then they move to
+      // the larger of the two references
+      if (pending) add_product(j - 1);
 #pragma unroll
-        for (int n = 0; n < N; n += 16)
-          tmem_ld_32x32(tmem + lane_base + 2 * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
-        tmem_ld_wait(raw);
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
-#pragma unroll
-          for (int part = PARTS - 2; part >= 0; --part)
-            v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
-          acc[r] = fmaf(v, mt[r], acc[r]);
-        }
+      for (int r = 0; r < RP; ++r) {
+        const float top = fmaxf(m[r], mt[r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float old = exp2_approx(m[r] - ref), to = exp2_approx(mt[r] - ref);
+        m[r] = top;
+        l[r] = fmaf(pr[r] * inv_vs, to, l[r] * old);
+        acc[r] *= old;
+        now[r] = to * (1.0f / kProbScale);
       }
+      pending = true;
 
       const bool last = c.last_tile();
       if (last || c.left == 1) {
+        add_product(j);
+        pending = false;
         // the row sums over the 128 tokens' threads
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
-          float v = l[r];
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (lane == 0) sh.sum[r][quarter] = v;
+          for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+          if (lane == 0) sh.sum[quarter][r] = l[r];
         }
         if (!all_of_group(ok)) break;
-        const int row0 = c.row_tile(p) * RP;
+        const int row0 = c.at.row_tile * RP;
         const bool direct = whole && last;
         float* part = p.parts + (2ll * blockIdx.x + (first_part ? 0 : 1)) * RP * (D + 2);
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
-          const float4 w = *reinterpret_cast<const float4*>(sh.sum[r]);
-          const float sum = (w.x + w.y) + (w.z + w.w);
+          const float sum = (sh.sum[0][r] + sh.sum[1][r]) + (sh.sum[2][r] + sh.sum[3][r]);
           const int row = row0 + r;
           if (direct) {
             if (me < D && row < p.rows) {
               T* dst = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + row / p.group * p.o_token_stride +
-                       (c.head(p) * p.group + row % p.group) * p.o_head_stride + me;
+                       (c.at.head * p.group + row % p.group) * p.o_head_stride + me;
               *dst = Elem<T>::from_f32(sum > 0.0f ? acc[r] / sum : acc[r] * 0.0f);   // nothing seen: 0
             }
           } else {
@@ -694,10 +739,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         first_part = false;
         if (last) ++item;
       }
-      c.next(p);
-      id = next_id;
-      ks = next_ks;
-      vs = next_vs;
+      c.advance(p, 1);
     }
   }
 
@@ -717,45 +759,42 @@ __global__ void __launch_bounds__(kThreads, 2)
 // boundary between two shares inside it; thread i looks at boundary i + 1.
 template <typename T, int D, int RP>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParams p) {
-  __shared__ long long before[kJoinThreads + 1], warp_sum[kJoinThreads / 32];
-  __shared__ struct { Place place; int first, last, skip; } found[kJoinThreads];
-  __shared__ int warp_found[kJoinThreads / 32];
-  __shared__ float column[kJoinThreads / 128][128], best[kJoinThreads / 32], weight[kJoinThreads / 128];
+  constexpr int kWarps = kJoinThreads / 32;
+  struct Cut { Place place; int first, last, skip; };
+  __shared__ Cut cuts[kMaxShares];
+  __shared__ int found[kMaxShares];
+  __shared__ float column[kJoinThreads / 128][128], best[kWarps], weight[kJoinThreads / 128];
   const int tid = threadIdx.x;
-  const long long total = scan_sequences(p, before, warp_sum, kJoinThreads);
-  const long long share = share_of(p, total);
-  const long long flat = (tid + 1) * share;
-  bool mine = false;
-  Place w;
-  long long begin = 0, end = 0;
-  if (tid + 1 < p.shares && flat < total) {
-    w = locate(p, before, kJoinThreads, flat);
-    begin = flat - w.tile;
-    end = begin + make_seq(p, p.lengths[w.b]).count;
-    mine = w.tile > 0 && begin / share == tid;
+  const WorkList list(p);
+  int count = 0;
+  if (!list.whole_items()) {
+    const int share = list.share_start(p, 1);          // all but the last are as long as the first
+    const int flat = (int)min((tid + 1ll) * share, (long long)list.tiles() - 1);
+    const Place w = list.locate(p, flat);
+    const int begin = flat - w.tile;
+    const bool mine = tid < p.shares - 1 && flat == (tid + 1ll) * share && w.tile > 0 && begin / share == tid;
+    if (mine) {
+      const int end = begin + make_seq(p, __ldg(p.lengths + w.b)).count;
+      cuts[tid] = Cut{w, tid, (end - 1) / share, begin != tid * share};
+    }
+    // in the order of the boundaries, so that every block has the same list
+    const uint32_t in_warp = __ballot_sync(0xffffffffu, mine);
+    if ((tid & 31) == 0) best[tid >> 5] = (float)__popc(in_warp);
+    __syncthreads();
+    int index = __popc(in_warp & ((1u << (tid & 31)) - 1));
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < (tid >> 5)) index += (int)best[i];
+      count += (int)best[i];
+    }
+    if (mine) found[index] = tid;
+    __syncthreads();
   }
-  // every block lists the items in the same order, so that they divide the work
-  const uint32_t in_warp = __ballot_sync(0xffffffffu, mine);
-  if ((tid & 31) == 0) warp_found[tid >> 5] = __popc(in_warp);
-  __syncthreads();
-  int index = __popc(in_warp & ((1u << (tid & 31)) - 1)), count = 0;
-  for (int i = 0; i < kJoinThreads / 32; ++i) {
-    if (i < (tid >> 5)) index += warp_found[i];
-    count += warp_found[i];
-  }
-  if (mine) {
-    found[index].place = w;
-    found[index].first = (int)(begin / share);
-    found[index].last = (int)((end - 1) / share);
-    found[index].skip = begin != found[index].first * share;   // the item is its first share's second part
-  }
-  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int group = tid / 128, lane = tid % 128;
   for (int u = blockIdx.x; u < count * RP; u += gridDim.x) {
-    const auto& f = found[u / RP];
+    const Cut& f = cuts[found[u / RP]];
     const int r = u % RP;
-    const int row = (f.place.item % p.row_tiles) * RP + r;
+    const int row = f.place.row_tile * RP + r;
     if (row >= p.rows) continue;                   // the same in every thread
     const int n = f.last - f.first + 1;
     auto part = [&](int i) {
@@ -766,7 +805,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
     m = warp_max(m);
     if ((tid & 31) == 0) best[tid >> 5] = m;
     __syncthreads();
-    for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, best[i]);
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, best[i]);
     float acc = 0.0f, sum = 0.0f;
     for (int i = group; i < n; i += kJoinThreads / 128) {
       const float* q = part(i);
@@ -785,7 +824,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
         sum += weight[i];
       }
       T* dst = static_cast<T*>(p.out) + f.place.b * p.o_batch_stride + row / p.group * p.o_token_stride +
-               (f.place.item / p.row_tiles * p.group + row % p.group) * p.o_head_stride + tid;
+               (f.place.head * p.group + row % p.group) * p.o_head_stride + tid;
       *dst = Elem<T>::from_f32(sum > 0.0f ? acc / sum : acc * 0.0f);
     }
     __syncthreads();
@@ -794,12 +833,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
 
 // ---- host ------------------------------------------------------------------------------------------
 
-constexpr int kMaxShares = kJoinThreads;
-
-int row_tile_of(int64_t rows, bool bf16) {
-  const int most = bf16 ? 32 : 16;       // more columns than 64 would need more tensor memory than half an SM's
-  int rp = 8;
-  while (rp < rows && rp < most) rp *= 2;
+int row_tile_of(int64_t rows) {
+  int rp = 4;
+  while (rp < rows && rp < 16) rp *= 2;
   return rp;
 }
 int shares_of() {
@@ -831,10 +867,11 @@ template <int D>
 int dispatch_kv(const KvAttnParams& p, const CUtensorMap& mk, const CUtensorMap& mv, bool bf16, int rp,
                 cudaStream_t stream) {
   if (bf16) {
+    if (rp == 4) return launch_kv<__nv_bfloat16, D, 4, 2>(p, mk, mv, stream);
     if (rp == 8) return launch_kv<__nv_bfloat16, D, 8, 2>(p, mk, mv, stream);
-    if (rp == 16) return launch_kv<__nv_bfloat16, D, 16, 2>(p, mk, mv, stream);
-    return launch_kv<__nv_bfloat16, D, 32, 2>(p, mk, mv, stream);
+    return launch_kv<__nv_bfloat16, D, 16, 2>(p, mk, mv, stream);
   }
+  if (rp == 4) return launch_kv<__half, D, 4, 3>(p, mk, mv, stream);
   if (rp == 8) return launch_kv<__half, D, 8, 3>(p, mk, mv, stream);
   return launch_kv<__half, D, 16, 3>(p, mk, mv, stream);
 }
@@ -855,7 +892,7 @@ using namespace nb200;
 extern "C" int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cache, int64_t batch,
                                                       int64_t queries, int64_t heads, int dtype) {
   if (!cache || cache->heads <= 0 || batch <= 0 || queries <= 0 || heads <= 0) return 0;
-  const int rp = row_tile_of(queries * (heads / cache->heads), dtype == NB200_BF16);
+  const int rp = row_tile_of(queries * (heads / cache->heads));
   return 2ll * shares_of() * rp * (cache->head_dim + 2) * (int64_t)sizeof(float);
 }
 
@@ -915,16 +952,20 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   p.group = (int)(heads / cache->heads);
   if (queries * p.group > INT32_MAX / 64) return fail(NB200_E_INVALID, "kv attention: too many rows per key head");
   p.rows = (int)queries * p.group;
-  const int rp = row_tile_of(p.rows, bf16);
+  const int rp = row_tile_of(p.rows);
   p.row_tiles = (p.rows + rp - 1) / rp;
-  if ((int64_t)p.row_tiles * p.kv_heads > INT32_MAX) return fail(NB200_E_INVALID, "kv attention: too many rows");
+  // the work list is counted in 32 bits
+  const int64_t most_tiles = cdiv64(max_pages * cache->page_size, kTile) + 1;
+  if ((double)most_tiles * batch * p.row_tiles * p.kv_heads > 2e9)
+    return fail(NB200_E_UNSUPPORTED, "kv attention: %lld sequences of up to %lld tokens, %lld query tokens: split the batch",
+                (long long)batch, (long long)(max_pages * cache->page_size), (long long)queries);
   p.pages = (int)cache->pages;
   p.page = (int)cache->page_size;
+  p.page_shift = p.page == 16 ? 4 : p.page == 32 ? 5 : p.page == 64 ? 6 : 7;
   p.max_pages = (int)max_pages;
   p.window = (int)window;
   p.sinks = (int)sinks;
   p.shares = shares_of();
-  p.min_share = 2;
   p.q_aligned = at16(q) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   p.scale = scale;
   p.wait_limit_ns = wait_limit_ns();
