@@ -42,12 +42,13 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kTile = 128;               // tokens
+constexpr int kHalf = 128;               // tokens of one product: a thread's and a tensor-memory lane's
+constexpr int kSmemPerCta = 106 * 1024;
 constexpr int kThreads = 192;            // producer, issuer, four softmax warps
 constexpr int kSoftmaxWarp = 2;
 constexpr int kJoinThreads = 512;
-constexpr int kMinShare = 2;             // tiles
-constexpr int kWholeItems = 4;           // tiles
+constexpr int kMinShare = 1;             // tiles
+constexpr int kWholeItems = 3;           // tiles
 constexpr int kMaxShares = kJoinThreads;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastScale = 8.67361738e-19f;   // 2^-60
@@ -63,13 +64,14 @@ struct KvAttnParams {
   const float *k_scales, *v_scales;
   const int32_t* table;
   const int32_t* lengths;
-  float* parts;                          // [2 * shares][rows padded][head_dim + 2]
+  float* parts;                          // [2 * shares][RP][head_dim]: sums of the parts of cut items
+  float2* marks;                         // [2 * shares][RP]: their reference and weight
   int64_t q_batch_stride, q_token_stride, q_head_stride;
   int64_t o_batch_stride, o_token_stride, o_head_stride;
   int64_t table_stride, k_scale_stride, v_scale_stride;
   int batch, nq, kv_heads, group;        // group: query heads per key head
   int rows, row_tiles;                   // nq * group, and how many pieces of RP rows
-  int pages, page, page_shift, max_pages, window, sinks;
+  int pages, page, page_shift, tile_shift, max_pages, window, sinks;
   int shares, q_aligned;
   float scale;
   unsigned long long wait_limit_ns;
@@ -89,22 +91,23 @@ __device__ __forceinline__ Seq make_seq(const KvAttnParams& p, int len) {
   s.limit = min(len, p.max_pages << p.page_shift);
   s.low = p.window ? max(max(len, p.nq) - p.nq + 1 - p.window, 0) : 0;   // of the first query there is
   s.sink_end = min(p.sinks, s.limit);
-  const int tiles = (s.limit + kTile - 1) / kTile;
+  const int shift = p.tile_shift, round = (1 << shift) - 1;
+  const int tiles = (s.limit + round) >> shift;
   s.first = s.from = 0;
   s.count = tiles;
   if (s.low > 0) {
-    const int sink_tiles = (s.sink_end + kTile - 1) / kTile;
-    if (s.low / kTile > sink_tiles) {
+    const int sink_tiles = (s.sink_end + round) >> shift;
+    if ((s.low >> shift) > sink_tiles) {
       s.first = sink_tiles;
-      s.from = s.low / kTile;
+      s.from = s.low >> shift;
       s.count = sink_tiles + max(tiles - s.from, 0);
     }
   }
   s.count = max(s.count, 1);       // a sequence without tokens has its zeros to write
   return s;
 }
-__device__ __forceinline__ int tile_start(const Seq& s, int t) {
-  return (t < s.first ? t : t - s.first + s.from) * kTile;
+__device__ __forceinline__ int tile_start(const KvAttnParams& p, const Seq& s, int t) {
+  return (t < s.first ? t : t - s.first + s.from) << p.tile_shift;
 }
 // Does any query of the call see this token, as far as positions go?
 __device__ __forceinline__ bool seen_by_any(const Seq& s, int token) {
@@ -219,22 +222,33 @@ struct Cursor {
   }
 };
 
+// Tiles of 256 tokens, two per thread, halve what a tile costs besides its data (the exchange of
+// maxima, the joining of a product); 16 rows have registers for one.
+template <int RP>
+struct Halves {
+  static constexpr int kCount = RP <= 8 ? 2 : 1;
+};
+
 template <int D, int RP, int PARTS>
 struct Shape {
   static constexpr int kN = (RP * PARTS + 15) / 16 * 16;
-  static constexpr int kTileBytes = kTile * D;                    // one K or V tile
-  // ring of K0 V0 K1 V1 ...: what two CTAs per SM leave room for
-  static constexpr int kSlots = D == 128 ? (kN >= 32 ? 4 : 6) : (kN >= 48 ? 10 : 12);
+  static constexpr int kH = Halves<RP>::kCount;
+  static constexpr int kSlotBytes = kHalf * D;                    // 128 tokens of K or of V
   static constexpr int kQBytes = kN * D;
-  static constexpr int kPBytes = kN * kTile;
-  static constexpr int kTmemCols = 4 * kN <= 64 ? 64 : 4 * kN <= 128 ? 128 : 256;
+  static constexpr int kPBytes = kN * kHalf;
+  // ring of a tile's K halves, its V halves, the next tile's ...: what two CTAs per SM, and the
+  // joining kernel beside them, leave room for
+  static constexpr int kRoom = (kSmemPerCta - 4096 - 2 * kH * kPBytes - 2 * kQBytes) / kSlotBytes;
+  static constexpr int kSlots = kRoom < 12 ? kRoom : 12;
+  static constexpr int kTmemO = 2 * kH * kN;                      // behind the scores of two tiles
+  static constexpr int kTmemCols = kTmemO + 2 * kN <= 64 ? 64 : kTmemO + 2 * kN <= 128 ? 128 : 256;
 };
 
 template <int D, int RP, int PARTS>
 struct Shared {
   using S = Shape<D, RP, PARTS>;
-  uint8_t ring[S::kSlots][S::kTileBytes];      // first: the swizzle counts from 1024-byte boundaries
-  uint8_t p[2][S::kPBytes];
+  uint8_t ring[S::kSlots][S::kSlotBytes];      // first: the swizzle counts from 1024-byte boundaries
+  uint8_t p[2][S::kH][S::kPBytes];
   uint8_t q[2][S::kQBytes];
   float4 scale[4][32];                         // of a step's pages: ks, log2 vs, 1 / vs, 1 if it is there
   float q_factor[2][RP];                       // what takes a row's product to log2 units
@@ -349,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     kv_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const KvAttnParams p) {
   using S = Shape<D, RP, PARTS>;
-  constexpr int N = S::kN, SLOTS = S::kSlots;
+  constexpr int N = S::kN, SLOTS = S::kSlots, H = S::kH;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Shared<D, RP, PARTS>& sh = *reinterpret_cast<Shared<D, RP, PARTS>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -390,16 +404,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     // It works in steps of 32 pages, a lane per page: pages are looked up two steps ahead and their
     // scales fetched one step ahead, so that neither latency is met per tile.  The scales go to the
     // softmax warps through four turns of shared memory: a step begins when the ring has room for
-    // it, that is when all but the ring's tiles before it are done with, and the ring has at most
-    // 6 tiles where three steps have at least 12.
-    static_assert(SLOTS / 2 <= 12, "a turn of the scales would be overwritten too early");
-    const int per_tile = kTile >> p.page_shift, step_tiles = 32 / per_tile;
+    // it, that is when all but the ring's tiles before it are done with, and the ring has fewer
+    // tiles than the three steps that are in the other turns.
+    static_assert(SLOTS <= 3 * 2 * H * (4 / H), "a turn of the scales would be overwritten too early");
+    const int per_half = kHalf >> p.page_shift, step_tiles = 32 / (per_half * H);
     const uint32_t page_bytes = (uint32_t)p.page * D;
-    const int my_tile = lane / per_tile, my_page = lane % per_tile;
+    const int my_tile = lane / (per_half * H), my_half = lane / per_half % H, my_page = lane % per_half;
     Cursor mine = c;
     auto page_of = [&](Cursor& at) {             // this lane's page, -1: not to be read
       if (at.left <= 0) return -1;
-      const int token = tile_start(at.seq, at.at.tile) + (my_page << p.page_shift);
+      const int token = tile_start(p, at.seq, at.at.tile) + my_half * kHalf + (my_page << p.page_shift);
       if (!(token < at.seq.limit && (token + p.page > at.seq.low || token < at.seq.sink_end))) return -1;
       const int id = __ldg(p.table + at.at.b * p.table_stride + (token >> p.page_shift));
       return id >= 0 && id < p.pages ? id : -1;
@@ -429,11 +443,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       bool handed = false;
       for (int k = 0; k < step_tiles && left > 0 && ok; ++k, --left) {
         const int j = step * step_tiles + k;
-        const bool in_tile = my_tile == k && id[0] >= 0;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, in_tile)) * page_bytes;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int g = 2 * j + kv, x = g % SLOTS;
+        for (int i = 0; i < 2 * H; ++i) {        // the halves of K, then those of V
+          const int g = 2 * H * j + i, x = g % SLOTS;
+          const bool in_slot = my_tile == k && my_half == i % H && id[0] >= 0;
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, in_slot)) * page_bytes;
           ok = ok && mbar_wait_nocall(smem_u32(&sh.empty[x]), ((g / SLOTS) & 1) ^ 1, ctx, ST_KV_EMPTY, g);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
@@ -442,8 +456,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (bytes) mbar_arrive_expect_tx(bar, bytes); else mbar_arrive(bar);
           }
           __syncwarp();
-          if (in_tile)
-            tma_load_4d(smem_u32(&sh.ring[x][my_page * page_bytes]), kv ? &map_v : &map_k, 0, 0, head[0], id[0], bar);
+          if (in_slot)
+            tma_load_4d(smem_u32(&sh.ring[x][my_page * page_bytes]), i < H ? &map_k : &map_v, 0, 0, head[0], id[0], bar);
         }
         if (!handed) {                           // behind the first tile's copies
           if (vs[0] < kLeastScale) vs[0] = kLeastScale;   // its logarithm is used; NaN stays
@@ -463,35 +477,35 @@ __global__ void __launch_bounds__(kThreads, 2)
   } else if (warp == 1) {
     // ---- issuer ----
     const bool elected = elect_one();
-    constexpr uint32_t kIdescQk = instr_desc_e4m3(kTile, N, false, false);
-    constexpr uint32_t kIdescPv = instr_desc_e4m3(kTile, N, true, true);
+    constexpr uint32_t kIdescQk = instr_desc_e4m3(kHalf, N, false, false);
+    constexpr uint32_t kIdescPv = instr_desc_e4m3(kHalf, N, true, true);
     constexpr uint64_t kKMajor = D == 128 ? smem_desc_sw128(16, 1024) : smem_desc_sw64(16, 512);
     // head_dim 64 fills half of the 128 rows: the second slab of 64 is the first one again
     constexpr uint64_t kVDesc = D == 128 ? smem_desc_sw128(16, 1024) : smem_desc_sw64(0, 512);
-    constexpr uint64_t kPDesc = smem_desc_plain(128, kTile * 16);
+    constexpr uint64_t kPDesc = smem_desc_plain(128, kHalf * 16);
     auto wait_all = [&](uint64_t* bar, uint32_t parity, unsigned int code, int detail) -> bool {
       return __all_sync(0xffffffffu, mbar_wait_nocall(smem_u32(bar), parity, ctx, code, detail));
     };
-    auto scores = [&](int j, int item) {           // S(j) = K(j) Q of the item
-      const uint32_t kb = smem_u32(sh.ring[2 * j % SLOTS]), qb = smem_u32(sh.q[item & 1]);
-#pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk)
-        if (elected)
-          mma_f8_ss(tmem + (j & 1) * N, with_address(kKMajor, kb + kk * 32),
-                    with_address(kKMajor, qb + kk * 32), kIdescQk, kk != 0);
-      if (elected) {
-        mma_commit(smem_u32(&sh.s_full[j & 1]));
-        mma_commit(smem_u32(&sh.empty[2 * j % SLOTS]));
-      }
-    };
     bool ok = true;
     int item = 0;                    // items begun
-    auto begin = [&](int j, bool new_item) {
+    auto begin = [&](int j, bool new_item) {       // S(j) = K(j) Q of the item
       if (new_item) ok = wait_all(&sh.q_full[item & 1], (item >> 1) & 1, ST_KV_Q, item);
-      ok = ok && wait_all(&sh.full[2 * j % SLOTS], (2 * j / SLOTS) & 1, ST_KV_K, j);
-      if (!ok) return;
-      tc_fence_after_sync();
-      scores(j, item);
+      const uint32_t qb = smem_u32(sh.q[item & 1]);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int g = 2 * H * j + h, x = g % SLOTS;
+        ok = ok && wait_all(&sh.full[x], (g / SLOTS) & 1, ST_KV_K, j);
+        if (!ok) return;
+        tc_fence_after_sync();
+        const uint32_t kb = smem_u32(sh.ring[x]);
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk)
+          if (elected)
+            mma_f8_ss(tmem + ((j & 1) * H + h) * N, with_address(kKMajor, kb + kk * 32),
+                      with_address(kKMajor, qb + kk * 32), kIdescQk, kk != 0);
+        if (elected) mma_commit(smem_u32(&sh.empty[x]));
+      }
+      if (elected) mma_commit(smem_u32(&sh.s_full[j & 1]));
       __syncwarp();
     };
     if (c.left > 0) begin(0, true);
@@ -502,21 +516,23 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (ends) ++item;
         begin(j + 1, ends);
       }
-      const int x = (2 * j + 1) % SLOTS;
-      ok = ok && wait_all(&sh.full[x], ((2 * j + 1) / SLOTS) & 1, ST_KV_V, j);
       ok = ok && wait_all(&sh.p_full[j & 1], (j >> 1) & 1, ST_KV_P, j);
-      if (!ok) break;
-      tc_fence_after_sync();
-      const uint32_t vb = smem_u32(sh.ring[x]), pb = smem_u32(sh.p[j & 1]);
 #pragma unroll
-      for (int kk = 0; kk < kTile / 32; ++kk)      // 32 tokens: four groups of eight rows
-        if (elected)
-          mma_f8_ss(tmem + (2 + (j & 1)) * N, with_address(kVDesc, vb + kk * 32 * D),
-                    with_address(kPDesc, pb + kk * 4 * 128), kIdescPv, kk != 0);
-      if (elected) {
-        mma_commit(smem_u32(&sh.o_full[j & 1]));
-        mma_commit(smem_u32(&sh.empty[x]));
+      for (int h = 0; h < H; ++h) {
+        const int g = 2 * H * j + H + h, x = g % SLOTS;
+        ok = ok && wait_all(&sh.full[x], (g / SLOTS) & 1, ST_KV_V, j);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t vb = smem_u32(sh.ring[x]), pb = smem_u32(sh.p[j & 1][h]);
+#pragma unroll
+        for (int kk = 0; kk < kHalf / 32; ++kk)    // 32 tokens: four groups of eight rows
+          if (elected)
+            mma_f8_ss(tmem + S::kTmemO + (j & 1) * N, with_address(kVDesc, vb + kk * 32 * D),
+                      with_address(kPDesc, pb + kk * 4 * 128), kIdescPv, h != 0 || kk != 0);
+        if (elected) mma_commit(smem_u32(&sh.empty[x]));
       }
+      if (!ok) break;
+      if (elected) mma_commit(smem_u32(&sh.o_full[j & 1]));
       __syncwarp();
     }
   } else {
@@ -537,7 +553,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
 
     int item = 0;
-    bool whole = c.at.tile == 0;                   // has the item's first tile
     bool first_part = true;                        // the item that the share begins with
     float acc[RP], l[RP], m[RP], now[RP];          // m: log2 units
 #pragma unroll
@@ -554,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       uint32_t raw[N];
 #pragma unroll
       for (int n = 0; n < N; n += 16)
-        tmem_ld_32x32(tmem + lane_base + (2 + (j & 1)) * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
+        tmem_ld_32x32(tmem + lane_base + S::kTmemO + (j & 1) * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
       tmem_ld_wait(raw);
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
@@ -565,181 +580,206 @@ __global__ void __launch_bounds__(kThreads, 2)
         acc[r] = fmaf(v, now[r], acc[r]);
       }
     };
-    bool pending = false;                          // a product of this item has not joined yet
-    for (int j = 0; c.left > 0; ++j) {
-      // the next item's queries: loaded at the start of an item, staged behind its first tile
-      const int skip = c.seq.count - c.at.tile;    // tiles to the next item
-      const bool stage_next = (j == 0 || c.at.tile == 0) && c.left > skip;
-      Cursor next_item = c;
+    const int step_shift = p.page_shift - 2 - (H - 1);       // 32 pages are 2^step_shift tiles
+    bool alive = true;
+    for (int j = 0; c.left > 0 && alive; ++item) {
+      // one item, as much of it as the share has
+      const int to_end = c.seq.count - c.at.tile;
+      const int n = min(to_end, c.left);
+      // the next item's queries are loaded now and staged behind this one's first tile
+      const bool stage_next = c.left > to_end;
+      Cursor next = c;
       if (stage_next) {
-        next_item.advance(p, skip);
-        queries.load(p, next_item, me);
+        next.advance(p, to_end);
+        queries.load(p, next, me);
       }
+      float factor[RP];
+#pragma unroll
+      for (int r = 0; r < RP; ++r) factor[r] = sh.q_factor[item & 1][r];
 
-      const int x = j & 1;
-      const int t0 = tile_start(c.seq, c.at.tile);
-      const int token = t0 + me;
-      // every query sees the whole tile: no masks but whether the page is there
-      const bool clean = t0 + kTile <= c.seq.limit && t0 + kTile - 1 <= c.seq.len - p.nq &&
-                         (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTile <= p.sinks);
-      const int step = (unsigned)j >> (p.page_shift - 2);    // 32 pages: 2^(shift - 2) tiles
-      ok = ok && mbar_wait_nocall(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j);
-      ok = ok && mbar_wait_nocall(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
-      ok = __all_sync(0xffffffffu, ok);
-      const float4 scale = sh.scale[step & 3][((j << (7 - p.page_shift)) + (me >> p.page_shift)) & 31];
-      const float lv = scale.y, inv_vs = scale.z;
-      // seen by some query, and its page is there
-      const bool there = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
-      float s[RP];
-      if (ok) {
-        tc_fence_after_sync();
-        uint32_t raw[N];
+      for (int k = 0; k < n; ++k, ++j) {
+        const int x = j & 1;
+        const int t0 = tile_start(p, c.seq, c.at.tile + k);
+        constexpr int kTokens = kHalf * H;
+        // every query sees the whole tile: no masks but whether the page is there
+        const bool clean = t0 + kTokens <= c.seq.limit && t0 + kTokens - 1 <= c.seq.len - p.nq &&
+                           (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTokens <= p.sinks);
+        const int step = j >> step_shift;
+        ok = ok && mbar_wait_nocall(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j);
+        ok = ok && mbar_wait_nocall(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
+        ok = __all_sync(0xffffffffu, ok);
+        float s[H][RP], inv_vs[H];
+        bool there[H];
+        if (ok) {
+          tc_fence_after_sync();
+          uint32_t raw[H][N];
 #pragma unroll
-        for (int n = 0; n < N; n += 16)
-          tmem_ld_32x32(tmem + lane_base + x * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
-        tmem_ld_wait(raw);
-        float w[RP];
+          for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
+            for (int i = 0; i < N; i += 16)
+              tmem_ld_32x32(tmem + lane_base + (x * H + h) * N + i, *reinterpret_cast<uint32_t (*)[16]>(&raw[h][i]));
+          tmem_ld_wait(raw[0]);
+          if constexpr (H == 2) tmem_ld_wait(raw[H - 1]);
 #pragma unroll
-          for (int part = PARTS - 2; part >= 0; --part)
-            v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
-          s[r] = there ? fmaf(v, sh.q_factor[item & 1][r] * scale.x, lv) : -INFINITY;
-        }
-        if (!clean || p.rows < RP * p.row_tiles) {   // tokens that some rows do not see, rows that only pad
-          const int* at = sh.q_at[item & 1];
+          for (int h = 0; h < H; ++h) {
+            const int token = t0 + h * kHalf + me;
+            const int entry = (((j * H + h) << (7 - p.page_shift)) + (me >> p.page_shift)) & 31;
+            const float4 scale = sh.scale[step & 3][entry];
+            inv_vs[h] = scale.z;
+            // seen by some query, and its page is there
+            there[h] = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
 #pragma unroll
-          for (int r = 0; r < RP; ++r) {
-            const bool seen = token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks);
-            if (!seen) s[r] = -INFINITY;
+            for (int r = 0; r < RP; ++r) {
+              float v = __uint_as_float(raw[h][(PARTS - 1) * RP + r]);
+#pragma unroll
+              for (int part = PARTS - 2; part >= 0; --part)
+                v = fmaf(v, 0.0625f, __uint_as_float(raw[h][part * RP + r]));
+              // a row that only pads has a product of zero and is as good as any: nobody reads it
+              s[h][r] = there[h] ? fmaf(v, factor[r] * scale.x, scale.y) : -INFINITY;
+            }
+            if (!clean) {                          // tokens that some rows do not see
+              const int* at = sh.q_at[item & 1];
+#pragma unroll
+              for (int r = 0; r < RP; ++r) {
+                const bool seen = token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks);
+                if (!seen) s[h][r] = -INFINITY;
+              }
+            }
+          }
+          float w[RP];
+#pragma unroll
+          for (int r = 0; r < RP; ++r) w[r] = warp_max(H == 2 ? fmaxf(s[0][r], s[H - 1][r]) : s[0][r]);
+          if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < RP; r += 4)
+              *reinterpret_cast<float4*>(&sh.most[x][quarter][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
           }
         }
-#pragma unroll
-        for (int r = 0; r < RP; ++r) w[r] = warp_max(s[r]);
-        if (lane == 0) {
-#pragma unroll
-          for (int r = 0; r < RP; r += 4)
-            *reinterpret_cast<float4*>(&sh.most[x][quarter][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
+        if (!all_of_group(ok)) {
+          alive = false;
+          break;
         }
-      }
-      if (!all_of_group(ok)) break;
-      float mt[RP];
+        float mt[RP];
 #pragma unroll
-      for (int r = 0; r < RP; r += 4) {
-        float4 w = *reinterpret_cast<const float4*>(&sh.most[x][0][r]);
+        for (int r = 0; r < RP; r += 4) {
+          float4 w = *reinterpret_cast<const float4*>(&sh.most[x][0][r]);
 #pragma unroll
-        for (int i = 1; i < 4; ++i) {
-          const float4 o = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
-          w = make_float4(fmaxf(w.x, o.x), fmaxf(w.y, o.y), fmaxf(w.z, o.z), fmaxf(w.w, o.w));
+          for (int i = 1; i < 4; ++i) {
+            const float4 o = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
+            w = make_float4(fmaxf(w.x, o.x), fmaxf(w.y, o.y), fmaxf(w.z, o.z), fmaxf(w.w, o.w));
+          }
+          mt[r] = w.x;
+          mt[r + 1] = w.y;
+          mt[r + 2] = w.z;
+          mt[r + 3] = w.w;
         }
-        mt[r] = w.x;
-        mt[r + 1] = w.y;
-        mt[r + 2] = w.z;
-        mt[r + 3] = w.w;
-      }
-      // probabilities relative to the tile's maximum (0 where the row sees nothing of it), in parts
-      uint32_t bytes[PARTS][RP / 4];
-      float pr[RP];
+        // probabilities relative to the tile's maximum (0 where the row sees nothing of it), in parts
+        float lt[RP];                              // this thread's part of the tile's row sums
 #pragma unroll
-      for (int r = 0; r < RP; ++r) pr[r] = exp2_approx(s[r] - (mt[r] == -INFINITY ? 0.0f : mt[r]));
+        for (int h = 0; h < H; ++h) {
+          uint32_t bytes[PARTS][RP / 4];
 #pragma unroll
-      for (int r = 0; r < RP; r += 2) {
-        float a = pr[r] * kProbScale, b = pr[r + 1] * kProbScale;
+          for (int r = 0; r < RP; r += 2) {
+            float pr[2];
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          const uint32_t q = split2(a, b);
-          if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
+            for (int i = 0; i < 2; ++i) {
+              pr[i] = exp2_approx(s[h][r + i] - (mt[r + i] == -INFINITY ? 0.0f : mt[r + i]));
+              lt[r + i] = h == 0 ? pr[i] * inv_vs[0] : fmaf(pr[i], inv_vs[h], lt[r + i]);
+              pr[i] *= kProbScale;
+            }
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+              const uint32_t q = split2(pr[0], pr[1]);
+              if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
+            }
+          }
+          // the token's row of P: N bytes, 16 at a time
+#pragma unroll
+          for (int i = 0; i < N; i += 16) {
+            uint32_t w[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const int at = (i + 4 * b) / RP, r = (i + 4 * b) % RP;
+              w[b] = at < PARTS ? bytes[at < PARTS ? at : 0][r / 4] : 0u;
+            }
+            st_shared_v4(smem_u32(sh.p[x][h]) + (i / 16) * (kHalf * 16) + me * 16, w[0], w[1], w[2], w[3]);
+          }
+          if (__any_sync(0xffffffffu, !there[h])) {
+            const int g = 2 * H * j + H + h;
+            ok = ok && mbar_wait_nocall(smem_u32(&sh.full[g % SLOTS]), (g / SLOTS) & 1, ctx, ST_KV_ZERO, j);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!there[h]) {
+#pragma unroll
+              for (int i = 0; i < D; i += 16) st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + i]), 0, 0, 0, 0);
+            }
+          }
         }
-      }
-      // the token's row of P: N bytes, 16 at a time
-#pragma unroll
-      for (int n = 0; n < N; n += 16) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = (n + 4 * i) / RP, r = (n + 4 * i) % RP;
-          w[i] = at < PARTS ? bytes[at < PARTS ? at : 0][r / 4] : 0u;
-        }
-        st_shared_v4(smem_u32(sh.p[x]) + (n / 16) * (kTile * 16) + me * 16, w[0], w[1], w[2], w[3]);
-      }
-      if (__any_sync(0xffffffffu, !there)) {
-        const int g = 2 * j + 1;
-        ok = mbar_wait_nocall(smem_u32(&sh.full[g % SLOTS]), (g / SLOTS) & 1, ctx, ST_KV_ZERO, j);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!there) {
-#pragma unroll
-          for (int i = 0; i < D; i += 16) st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + i]), 0, 0, 0, 0);
-        }
-      }
-      fence_proxy_async_smem();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[x]));
-
-      if (stage_next) {
-        const int y = (item + 1) & 1;
-        queries.stage(p, next_item, me, sh.q[y], sh.q_factor[y], sh.q_at[y]);
         fence_proxy_async_smem();
+        tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[y]));
-      }
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[x]));
 
-      // the tile before joins the sums while the tensor core works on this one; then they move to
-      // the larger of the two references
-      if (pending) add_product(j - 1);
+        if (stage_next && k == 0) {
+          const int y = (item + 1) & 1;
+          queries.stage(p, next, me, sh.q[y], sh.q_factor[y], sh.q_at[y]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[y]));
+        }
+
+        // the tile before joins the sums while the tensor core works on this one; then they move to
+        // the larger of the two references
+        if (k > 0) add_product(j - 1);
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          const float top = fmaxf(m[r], mt[r]);
+          const float ref = top == -INFINITY ? 0.0f : top;
+          const float old = exp2_approx(m[r] - ref), to = exp2_approx(mt[r] - ref);
+          m[r] = top;
+          l[r] = fmaf(lt[r], to, l[r] * old);
+          acc[r] *= old;
+          now[r] = to * (1.0f / kProbScale);
+        }
+      }
+      if (!alive) break;
+
+      add_product(j - 1);
+      // the row sums over the 128 tokens' threads
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
-        const float top = fmaxf(m[r], mt[r]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        const float old = exp2_approx(m[r] - ref), to = exp2_approx(mt[r] - ref);
-        m[r] = top;
-        l[r] = fmaf(pr[r] * inv_vs, to, l[r] * old);
-        acc[r] *= old;
-        now[r] = to * (1.0f / kProbScale);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
       }
-      pending = true;
-
-      const bool last = c.last_tile();
-      if (last || c.left == 1) {
-        add_product(j);
-        pending = false;
-        // the row sums over the 128 tokens' threads
+      if (lane == 0) {
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
+        for (int r = 0; r < RP; r += 4)
+          *reinterpret_cast<float4*>(&sh.sum[quarter][r]) = make_float4(l[r], l[r + 1], l[r + 2], l[r + 3]);
+      }
+      alive = all_of_group(ok);
+      if (!alive) break;
+      const int row0 = c.at.row_tile * RP;
+      const bool direct = c.at.tile == 0 && n == to_end;
+      const int part = (2 * blockIdx.x + (first_part ? 0 : 1)) * RP;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-          if (lane == 0) sh.sum[quarter][r] = l[r];
-        }
-        if (!all_of_group(ok)) break;
-        const int row0 = c.at.row_tile * RP;
-        const bool direct = whole && last;
-        float* part = p.parts + (2ll * blockIdx.x + (first_part ? 0 : 1)) * RP * (D + 2);
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float sum = (sh.sum[0][r] + sh.sum[1][r]) + (sh.sum[2][r] + sh.sum[3][r]);
-          const int row = row0 + r;
-          if (direct) {
-            if (me < D && row < p.rows) {
-              T* dst = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + row / p.group * p.o_token_stride +
-                       (c.at.head * p.group + row % p.group) * p.o_head_stride + me;
-              *dst = Elem<T>::from_f32(sum > 0.0f ? acc[r] / sum : acc[r] * 0.0f);   // nothing seen: 0
-            }
-          } else {
-            if (me < D) part[r * (D + 2) + me] = acc[r];
-            if (me == 0) {
-              part[r * (D + 2) + D] = m[r];
-              part[r * (D + 2) + D + 1] = sum;
-            }
+      for (int r = 0; r < RP; ++r) {
+        const float sum = (sh.sum[0][r] + sh.sum[1][r]) + (sh.sum[2][r] + sh.sum[3][r]);
+        const int row = row0 + r;
+        if (direct) {
+          if (me < D && row < p.rows) {
+            T* dst = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + row / p.group * p.o_token_stride +
+                     (c.at.head * p.group + row % p.group) * p.o_head_stride + me;
+            *dst = Elem<T>::from_f32(sum > 0.0f ? acc[r] / sum : acc[r] * 0.0f);   // nothing seen: 0
           }
-          acc[r] = l[r] = 0.0f;
-          m[r] = -INFINITY;
+        } else {
+          if (me < D) p.parts[(part + r) * D + me] = acc[r];
+          if (me == 0) p.marks[part + r] = make_float2(m[r], sum);
         }
-        whole = true;
-        first_part = false;
-        if (last) ++item;
+        acc[r] = l[r] = 0.0f;
+        m[r] = -INFINITY;
       }
-      c.advance(p, 1);
+      first_part = false;
+      c = next;
+      if (!stage_next) c.left = 0;
     }
   }
 
@@ -756,78 +796,88 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // Joins the parts of the items that were cut, in token order.  An item is found by the first
-// boundary between two shares inside it; thread i looks at boundary i + 1.
+// boundary between two shares inside it; thread i looks at boundary i + 1.  A row of an item is
+// one warp's work, or one block's where there are too few rows to fill the chip (then the items
+// have many parts).
 template <typename T, int D, int RP>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParams p) {
-  constexpr int kWarps = kJoinThreads / 32;
-  struct Cut { Place place; int first, last, skip; };
-  __shared__ Cut cuts[kMaxShares];
-  __shared__ int found[kMaxShares];
-  __shared__ float column[kJoinThreads / 128][128], best[kWarps], weight[kJoinThreads / 128];
-  const int tid = threadIdx.x;
+  constexpr int kWarps = kJoinThreads / 32, kCols = D / 32;     // columns per lane
+  __shared__ short found[kMaxShares];      // boundaries that are the first inside their item
+  __shared__ int in_warps[kWarps];
+  __shared__ float column[kWarps][D], weight[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const WorkList list(p);
+  const int share = list.share_start(p, 1);            // all but the last are as long as the first
   int count = 0;
   if (!list.whole_items()) {
-    const int share = list.share_start(p, 1);          // all but the last are as long as the first
     const int flat = (int)min((tid + 1ll) * share, (long long)list.tiles() - 1);
     const Place w = list.locate(p, flat);
-    const int begin = flat - w.tile;
-    const bool mine = tid < p.shares - 1 && flat == (tid + 1ll) * share && w.tile > 0 && begin / share == tid;
-    if (mine) {
-      const int end = begin + make_seq(p, __ldg(p.lengths + w.b)).count;
-      cuts[tid] = Cut{w, tid, (end - 1) / share, begin != tid * share};
-    }
+    const bool mine = tid < p.shares - 1 && flat == (tid + 1ll) * share && w.tile > 0 && (flat - w.tile) / share == tid;
     // in the order of the boundaries, so that every block has the same list
     const uint32_t in_warp = __ballot_sync(0xffffffffu, mine);
-    if ((tid & 31) == 0) best[tid >> 5] = (float)__popc(in_warp);
+    if (lane == 0) in_warps[warp] = __popc(in_warp);
     __syncthreads();
-    int index = __popc(in_warp & ((1u << (tid & 31)) - 1));
+    int index = __popc(in_warp & ((1u << lane) - 1));
     for (int i = 0; i < kWarps; ++i) {
-      if (i < (tid >> 5)) index += (int)best[i];
-      count += (int)best[i];
+      if (i < warp) index += in_warps[i];
+      count += in_warps[i];
     }
     if (mine) found[index] = tid;
     __syncthreads();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int group = tid / 128, lane = tid % 128;
-  for (int u = blockIdx.x; u < count * RP; u += gridDim.x) {
-    const Cut& f = cuts[found[u / RP]];
-    const int r = u % RP;
-    const int row = f.place.row_tile * RP + r;
-    if (row >= p.rows) continue;                   // the same in every thread
-    const int n = f.last - f.first + 1;
-    auto part = [&](int i) {
-      return p.parts + ((2ll * (f.first + i) + (i == 0 ? f.skip : 0)) * RP + r) * (D + 2);
-    };
+  const int units = count * RP;
+  const bool by_block = units <= 2 * (int)gridDim.x;   // the same everywhere
+  const int step = by_block ? kWarps : 1, mine = by_block ? warp : 0;
+  for (int u = by_block ? blockIdx.x : blockIdx.x * kWarps + warp; u < units;
+       u += by_block ? gridDim.x : gridDim.x * kWarps) {
+    const int r = u % RP, first = found[u / RP];
+    const Place at = list.locate(p, (first + 1) * share);
+    const int begin = (first + 1) * share - at.tile;
+    const int end = begin + make_seq(p, __ldg(p.lengths + at.b)).count;
+    const int skip = begin != first * share;           // the item is its first share's second part
+    const int row = at.row_tile * RP + r;
+    if (row >= p.rows) continue;                       // by block: the same in every thread
+    const int n = (end - 1) / share - first + 1;
+    // part i: the first share's first or second part, the first parts of the shares behind it
+    auto part = [&](int i) { return (2 * (first + i) + (i == 0 ? skip : 0)) * RP + r; };
     float m = -INFINITY;
-    for (int i = tid; i < n; i += kJoinThreads) m = fmaxf(m, part(i)[D]);
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, p.marks[part(i)].x);
     m = warp_max(m);
-    if ((tid & 31) == 0) best[tid >> 5] = m;
-    __syncthreads();
-    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, best[i]);
-    float acc = 0.0f, sum = 0.0f;
-    for (int i = group; i < n; i += kJoinThreads / 128) {
-      const float* q = part(i);
-      const float w = q[D] == -INFINITY ? 0.0f : exp2_approx(q[D] - m);
-      if (lane < D) acc = fmaf(q[lane], w, acc);
-      sum = fmaf(q[D + 1], w, sum);
-    }
-    column[group][lane] = acc;
-    if (lane == 0) weight[group] = sum;
-    __syncthreads();
-    if (tid < D) {
-      acc = sum = 0.0f;
+    float acc[kCols], sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kJoinThreads / 128; ++i) {
-        acc += column[i][tid];
+    for (int k = 0; k < kCols; ++k) acc[k] = 0.0f;
+#pragma unroll 4
+    for (int i = mine; i < n; i += step) {
+      const float2 mark = p.marks[part(i)];
+      const float* q = p.parts + part(i) * D + lane;
+      const float w = mark.x == -INFINITY ? 0.0f : exp2_approx(mark.x - m);
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) acc[k] = fmaf(q[k * 32], w, acc[k]);
+      sum = fmaf(mark.y, w, sum);
+    }
+    if (by_block) {
+      __syncthreads();                                 // the row before has been read
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) column[warp][k * 32 + lane] = acc[k];
+      if (lane == 0) weight[warp] = sum;
+      __syncthreads();
+      if (warp != 0) continue;
+      sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) acc[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) acc[k] += column[i][k * 32 + lane];
         sum += weight[i];
       }
-      T* dst = static_cast<T*>(p.out) + f.place.b * p.o_batch_stride + row / p.group * p.o_token_stride +
-               (f.place.head * p.group + row % p.group) * p.o_head_stride + tid;
-      *dst = Elem<T>::from_f32(sum > 0.0f ? acc / sum : acc * 0.0f);
     }
-    __syncthreads();
+    T* dst = static_cast<T*>(p.out) + at.b * p.o_batch_stride + row / p.group * p.o_token_stride +
+             (at.head * p.group + row % p.group) * p.o_head_stride + lane;
+#pragma unroll
+    for (int k = 0; k < kCols; ++k)
+      dst[k * 32] = Elem<T>::from_f32(sum > 0.0f ? acc[k] / sum : acc[k] * 0.0f);
   }
 }
 
@@ -847,7 +897,7 @@ template <typename T, int D, int RP, int PARTS>
 int launch_kv(KvAttnParams p, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t stream) {
   auto kern = kv_attn_kernel<T, D, RP, PARTS>;
   const int smem = (int)sizeof(Shared<D, RP, PARTS>);
-  static_assert(sizeof(Shared<D, RP, PARTS>) <= 113 * 1024, "two CTAs per SM");
+  static_assert(sizeof(Shared<D, RP, PARTS>) <= kSmemPerCta, "two CTAs per SM, and room for the joining kernel");
   if (int rc = prepare_kernel((const void*)kern, smem)) return rc;
   kern<<<p.shares, kThreads, smem, stream>>>(mk, mv, p);
   if (int rc = cuda_check(cudaGetLastError(), "kv attention launch")) return rc;
@@ -893,7 +943,7 @@ extern "C" int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cach
                                                       int64_t queries, int64_t heads, int dtype) {
   if (!cache || cache->heads <= 0 || batch <= 0 || queries <= 0 || heads <= 0) return 0;
   const int rp = row_tile_of(queries * (heads / cache->heads));
-  return 2ll * shares_of() * rp * (cache->head_dim + 2) * (int64_t)sizeof(float);
+  return 2ll * shares_of() * rp * (cache->head_dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }
 
 extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, void* out,
@@ -955,7 +1005,7 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   const int rp = row_tile_of(p.rows);
   p.row_tiles = (p.rows + rp - 1) / rp;
   // the work list is counted in 32 bits
-  const int64_t most_tiles = cdiv64(max_pages * cache->page_size, kTile) + 1;
+  const int64_t most_tiles = cdiv64(max_pages * cache->page_size, kHalf) + 1;
   if ((double)most_tiles * batch * p.row_tiles * p.kv_heads > 2e9)
     return fail(NB200_E_UNSUPPORTED, "kv attention: %lld sequences of up to %lld tokens, %lld query tokens: split the batch",
                 (long long)batch, (long long)(max_pages * cache->page_size), (long long)queries);
@@ -965,7 +1015,9 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   p.max_pages = (int)max_pages;
   p.window = (int)window;
   p.sinks = (int)sinks;
+  p.tile_shift = rp <= 8 ? 8 : 7;
   p.shares = shares_of();
+  p.marks = reinterpret_cast<float2*>(p.parts + 2ll * p.shares * rp * cache->head_dim);
   p.q_aligned = at16(q) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   p.scale = scale;
   p.wait_limit_ns = wait_limit_ns();
