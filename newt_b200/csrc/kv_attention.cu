@@ -901,6 +901,9 @@ int launch_kv(KvAttnParams p, const CUtensorMap& mk, const CUtensorMap& mv, cuda
   if (int rc = prepare_kernel((const void*)kern, smem)) return rc;
   kern<<<p.shares, kThreads, smem, stream>>>(mk, mv, p);
   if (int rc = cuda_check(cudaGetLastError(), "kv attention launch")) return rc;
+  // no sequence of the table can be long enough to be cut
+  const int64_t most = ((int64_t)p.max_pages << p.page_shift) + (1 << p.tile_shift) - 1;
+  if ((most >> p.tile_shift) <= kWholeItems) return 0;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)device_info().sm_count);
   config.blockDim = dim3(kJoinThreads);

@@ -22,7 +22,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .runtime import abi, kernels
+from .runtime import abi
 
 E4M3 = torch.float8_e4m3fn
 _CODES = {torch.float32: abi.F32, torch.float16: abi.F16, torch.bfloat16: abi.BF16, E4M3: abi.E4M3}
@@ -60,29 +60,44 @@ def new_kv_cache(pages, heads, page_size, head_dim, device=None):
                    torch.ones(pages, heads, device=device))
 
 
-def _on_device(**tensors):
-    """Every tensor given is a CUDA tensor of the current device."""
-    current = kernels.current_device() if torch.cuda.is_available() else None
-    for name, t in tensors.items():
+# The checks below run on every call of a step whose kernels take a few microseconds: they compare
+# first and word the complaint only when there is one.
+
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _launch_stream(names, *tensors):
+    """The current stream's handle, once every tensor given (None: not given) is seen to be a CUDA
+    tensor of the current device."""
+    first = tensors[0].get_device()
+    if first >= 0 and first == _device():
+        for t in tensors:
+            if t is not None and t.get_device() != first:
+                break
+        else:
+            return _stream(first)
+    for name, t in zip(names.split(), tensors):
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        if not t.is_cuda:
             raise TypeError(f"argument '{name}' must be a CUDA tensor")
-        if t.get_device() != current:
+        if t.get_device() != _device():
             raise ValueError(f"tensor '{name}' is on {t.device} but the current device is "
-                             f"cuda:{current}; newt launches on the current device")
+                             f"cuda:{_device()}; newt launches on the current device")
+    raise AssertionError("a tensor changed its device")
 
 
 def _shaped(name, t, shape, dtype=None):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"'{name}' has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"'{name}' is {t.dtype}, expected {dtype}")
 
 
 def _dense_rows(name, t):
     """Rows may lie anywhere, the elements of a row side by side."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"'{name}' must have unit stride along its last dimension")
 
 
@@ -93,6 +108,13 @@ def _contiguous(name, t):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _rows_like(x, dtype):
+    """A fresh contiguous tensor of x's shape."""
+    if x.is_contiguous():
+        return torch.empty_like(x, dtype=dtype)
+    return torch.empty(x.shape, dtype=dtype, device=x.device)
 
 
 def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=None, scales=None,
@@ -117,9 +139,10 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
     _shaped("weight", weight, (n,), dtype)
     _contiguous("weight", weight)
     if out is None:
-        out = torch.empty((rows, n), dtype=out_dtype, device=x.device)
+        out = _rows_like(x, out_dtype)
     else:
         _shaped("out", out, (rows, n), out_dtype)
+        _dense_rows("out", out)
     if out_dtype is E4M3:
         if group not in (0, 32, 64, 128):
             raise ValueError(f"rmsnorm: group {group} (0: one scale per row; 32, 64, 128 columns)")
@@ -135,22 +158,21 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
         _shaped("residual", residual, (rows, n), dtype)
         _dense_rows("residual", residual)
         if residual_out is None:
-            residual_out = torch.empty((rows, n), dtype=dtype, device=x.device)
+            residual_out = _rows_like(x, dtype)
         else:
             _shaped("residual_out", residual_out, (rows, n), dtype)
             _dense_rows("residual_out", residual_out)
     elif residual_out is not None:
         raise ValueError("rmsnorm: 'residual_out' goes with a residual")
     _dense_rows("x", x)
-    _dense_rows("out", out)
-    _on_device(x=x, weight=weight, residual=residual, out=out, scales=scales,
-               residual_out=residual_out)
+    stream = _launch_stream("x weight residual out scales residual_out", x, weight, residual, out,
+                            scales, residual_out)
     abi.check(abi.load().nb200_rmsnorm(
         x.data_ptr(), _ptr(residual), weight.data_ptr(), out.data_ptr(), _ptr(residual_out),
         _ptr(scales), rows, n, x.stride(0), residual.stride(0) if residual is not None else 0,
         out.stride(0), residual_out.stride(0) if residual_out is not None else 0,
         scales.stride(0) if scales is not None else 0, group, eps, _CODES[dtype],
-        _CODES[out_dtype], kernels.raw_stream()))
+        _CODES[out_dtype], stream))
     return RmsNorm(out, scales, residual_out)
 
 
@@ -159,9 +181,10 @@ def _pack_cache(cache):
     k, v, ks, vs = cache
     if k.dim() != 4:
         raise ValueError(f"'cache.k' must be [pages, heads, page_size, head_dim], got {tuple(k.shape)}")
-    pages, heads, page, d = k.shape
-    if v.shape != k.shape:
-        raise ValueError(f"'cache.v' has shape {tuple(v.shape)}, 'cache.k' {tuple(k.shape)}")
+    shape = k.shape
+    pages, heads, page, d = shape
+    if v.shape != shape:
+        raise ValueError(f"'cache.v' has shape {tuple(v.shape)}, 'cache.k' {tuple(shape)}")
     if k.dtype is not E4M3 or v.dtype is not E4M3:
         raise TypeError(f"the cache holds {k.dtype} and {v.dtype}, expected float8_e4m3fn")
     _shaped("cache.k_scales", ks, (pages, heads), torch.float32)
@@ -170,15 +193,20 @@ def _pack_cache(cache):
     vp, vh, vt, vu = v.stride()
     if ku != 1 or vu != 1:
         raise ValueError("the cache must have unit stride along head_dim")
-    if heads > 1 and (ks.stride(1) != 1 or vs.stride(1) != 1):
+    ksp, ksh = ks.stride()
+    vsp, vsh = vs.stride()
+    if heads > 1 and (ksh != 1 or vsh != 1):
         raise ValueError("the cache's scales must have unit stride over heads")
-    # the stride of a dimension of one element is never used: torch may say anything there
-    dense = page * d
-    return abi.KV_CACHE.pack(
-        k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, page, d,
-        kp if pages > 1 else heads * dense, kh if heads > 1 else dense, kt,
-        vp if pages > 1 else heads * dense, vh if heads > 1 else dense, vt,
-        ks.stride(0) if pages > 1 else heads, vs.stride(0) if pages > 1 else heads)
+    if pages <= 1 or heads <= 1:
+        # the stride of a dimension of one element is never used: torch may say anything there
+        dense = page * d
+        if heads <= 1:
+            kh = vh = dense
+        if pages <= 1:
+            kp = vp = heads * dense
+            ksp = vsp = heads
+    return abi.KV_CACHE.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads,
+                             page, d, kp, kh, kt, vp, vh, vt, ksp, vsp)
 
 
 def _page_table(table, batch):
@@ -202,7 +230,7 @@ def kv_append(cache, k, v, page_table, starts, offsets, max_new):
     pages they write to.  Tokens whose page the table lacks are not written."""
     packed = _pack_cache(cache)
     pages, heads, page, d = cache.k.shape
-    if k.dim() != 3 or tuple(k.shape[1:]) != (heads, d):
+    if k.dim() != 3 or k.shape[1:] != (heads, d):
         raise ValueError(f"'k' has shape {tuple(k.shape)}, expected (tokens, {heads}, {d})")
     _shaped("v", v, k.shape, k.dtype)
     if k.dtype not in (torch.bfloat16, torch.float16):
@@ -215,13 +243,13 @@ def kv_append(cache, k, v, page_table, starts, offsets, max_new):
     _contiguous("starts", starts)
     _contiguous("offsets", offsets)
     _page_table(page_table, batch)
-    _on_device(k=k, v=v, page_table=page_table, starts=starts, offsets=offsets, cache_k=cache.k,
-               cache_v=cache.v, cache_k_scales=cache.k_scales, cache_v_scales=cache.v_scales)
+    stream = _launch_stream(
+        "k v page_table starts offsets cache.k cache.v cache.k_scales cache.v_scales", k, v,
+        page_table, starts, offsets, cache.k, cache.v, cache.k_scales, cache.v_scales)
     abi.check(abi.load().nb200_kv_append(
         packed, k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), v.stride(0),
         v.stride(1), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-        starts.data_ptr(), offsets.data_ptr(), batch, max_new, _CODES[k.dtype],
-        kernels.raw_stream()))
+        starts.data_ptr(), offsets.data_ptr(), batch, max_new, _CODES[k.dtype], stream))
 
 
 def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, out=None):
@@ -246,12 +274,13 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     _contiguous("lengths", lengths)
     _page_table(page_table, batch)
     if out is None:
-        out = torch.empty((batch, queries, heads, d), dtype=dtype, device=q.device)
+        out = _rows_like(q, dtype)
     else:
         _shaped("out", out, q.shape, dtype)
         _dense_rows("out", out)
-    _on_device(q=q, page_table=page_table, lengths=lengths, out=out, cache_k=cache.k,
-               cache_v=cache.v, cache_k_scales=cache.k_scales, cache_v_scales=cache.v_scales)
+    stream = _launch_stream(
+        "q page_table lengths out cache.k cache.v cache.k_scales cache.v_scales", q, page_table,
+        lengths, out, cache.k, cache.v, cache.k_scales, cache.v_scales)
     lib = abi.load()
     code = _CODES[dtype]
     need = lib.nb200_kv_attention_workspace_bytes(packed, batch, queries, heads, code)
@@ -260,8 +289,7 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
         q.data_ptr(), packed, out.data_ptr(), batch, queries, heads, q.stride(0), q.stride(1),
         q.stride(2), out.stride(0), out.stride(1), out.stride(2), page_table.data_ptr(),
         page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
-        d ** -0.5 if scale is None else scale, window, sinks, code, _ptr(ws), need,
-        kernels.raw_stream()))
+        d ** -0.5 if scale is None else scale, window, sinks, code, _ptr(ws), need, stream))
     return out
 
 
@@ -290,7 +318,7 @@ def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
     _row_values(rows, torch.int64, tokens=tokens)
     if not 0 <= top <= 32:
         raise ValueError(f"token_logprobs: {top} alternatives (0 to 32)")
-    _on_device(logits=logits, tokens=tokens)
+    stream = _launch_stream("logits tokens", logits, tokens)
     device = logits.device
     both = torch.empty((3, rows), dtype=torch.float32, device=device)
     logprob, entropy, lse = both.unbind(0)
@@ -303,7 +331,7 @@ def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
     abi.check(abi.load().nb200_token_logprobs(
         logits.data_ptr(), _ptr(tokens), _ptr(logprob), entropy.data_ptr(), lse.data_ptr(),
         _ptr(best), _ptr(index), rows, vocab, logits.stride(0), top, inv_temperature,
-        _CODES[logits.dtype], kernels.raw_stream()))
+        _CODES[logits.dtype], stream))
     return TokenLogprobs(logprob, entropy, lse, best, index)
 
 
@@ -317,14 +345,14 @@ def token_logprobs_backward(logits, tokens, lse, entropy, grad_logprob=None, gra
     _row_values(rows, torch.float32, lse=lse, entropy=entropy, grad_logprob=grad_logprob,
                 grad_entropy=grad_entropy)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = _rows_like(logits, logits.dtype)
     else:
         _shaped("out", out, (rows, vocab), logits.dtype)
         _dense_rows("out", out)
-    _on_device(logits=logits, tokens=tokens, lse=lse, entropy=entropy, grad_logprob=grad_logprob,
-               grad_entropy=grad_entropy, out=out)
+    stream = _launch_stream("logits tokens lse entropy grad_logprob grad_entropy out", logits, tokens,
+                            lse, entropy, grad_logprob, grad_entropy, out)
     abi.check(abi.load().nb200_token_logprobs_bwd(
         logits.data_ptr(), _ptr(tokens), _ptr(lse), _ptr(entropy), _ptr(grad_logprob),
         _ptr(grad_entropy), out.data_ptr(), rows, vocab, logits.stride(0), out.stride(0),
-        inv_temperature, _CODES[logits.dtype], kernels.raw_stream()))
+        inv_temperature, _CODES[logits.dtype], stream))
     return out
