@@ -375,7 +375,8 @@ int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, void* out, in
  * to the lower index, NaN lowest) and top_logprob, both [rows, top].  All results are fp32, the
  * indices int64.  A negative token stands for none: logprob 0; one beyond the vocabulary gives
  * NaN.  A row of nothing but -inf: logprobs and lse -inf, entropy 0.  A row with NaN or +inf gives NaN.
- * tokens / logprob, entropy and lse may be null where they are not wanted.  One pass over the row;
+ * `inv_temperature` is between 1e-20 and 1e20.  tokens / logprob, entropy and lse may be null where
+ * they are not wanted.  One pass over the row;
  * results do not depend on the launch's other rows. */
 int nb200_token_logprobs(const void* logits, const int64_t* tokens, float* logprob, float* entropy,
                          float* lse, float* top_logprob, int64_t* top_index, int64_t rows,

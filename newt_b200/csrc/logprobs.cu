@@ -3,10 +3,16 @@
 //   lse = log sum_j e^z_j,  logprob = z_t - lse,  H = lse - sum_j p_j z_j,  p_j = e^(z_j - lse)
 //   d logits_j = inv_temperature * (g ([j = t] - p_j) - gH p_j (z_j - lse + H))
 //
-// Forward: one pass over the row.  Every thread keeps a running maximum m and, in units of 2^x,
-// S = sum 2^(x_j - m) and E = sum 2^(x_j - m) (x_j - m); both are rescaled when m moves.  Then
-// log S and E / S give all three results, and nothing larger than a difference to the maximum is
-// ever multiplied, so logits of the type's lowest value do not overflow.
+// Forward: one pass over the row, in log2 units: y_j = x_j * (inv_temperature * log2 e).  Every
+// thread keeps a reference R (the largest y so far, rounded), S = sum 2^(y_j - R) and
+// E = sum 2^(y_j - R) (y_j - R); both are rescaled when R moves.  y_j - R is one fused
+// multiply-add, exact but for its rounding, and R is only ever used as the rounded number it is, so
+// nothing is lost by its rounding; two lanes of packed fp32 share an instruction.  What the special
+// function unit does -- one 2^x per element -- takes three quarters of the time HBM does for 16-bit
+// logits, which is why everything else is kept to four or five instructions per element.  Logits
+// are raised to -1e30 at least, where 2^x is 0: -inf would make E a NaN.  log S and E / S give all
+// three results.  Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest value of a
+// wide type, +inf) are done again, from differences to the maximum, by the row's first CTA.
 //
 // Alternatives: an element's key is (order-preserving bits of the value, ~index), so keys differ
 // and ties go to the lowest index.  A CTA keeps a list of candidate keys in shared memory and the
@@ -22,12 +28,14 @@
 
 #include "common.cuh"
 #include "elem.cuh"
+#include "sm100.cuh"
 
 namespace nb200 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+using namespace sm100;
+
+constexpr int kThreads = 256;            // of the gradient; the forward pass says its own
 constexpr int kMaxCluster = 8;
 constexpr int kTopMax = 32;
 constexpr int kListKept = 4 * kTopMax;   // candidates that may stay in the list between chunks
@@ -47,12 +55,6 @@ struct LogprobParams {
   float inv_temperature;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // Larger key = larger value, then lower index.  -0 counts as 0, NaN as the lowest value.
 __device__ __forceinline__ unsigned long long make_key(float v, int index) {
   v = v != v ? -INFINITY : v + 0.0f;
@@ -66,36 +68,76 @@ __device__ __forceinline__ float key_value(unsigned long long key) {
 }
 __device__ __forceinline__ int key_index(unsigned long long key) { return (int)~(uint32_t)key; }
 
-struct Partial {   // of some of a row's elements; m is a raw logit, s and e are relative to it
-  float m, s, e;
+// Of some of a row's elements: the largest, and sums relative to 2^r.  r is kNone where there are none.
+struct Partial {
+  float m, r, s, e;
 };
+constexpr float kLowest = -1e30f, kNone = -3e38f, kWide = 1e29f;
 
-// sums relative to `m` from sums relative to `from` <= m
-__device__ __forceinline__ void rescale(float from, float m, float factor, float& s, float& e) {
-  if (from == -INFINITY) {        // nothing but -inf so far: both sums are 0 (or NaN, which stays)
-    return;
-  }
-  const float d = fmaxf((from - m) * factor, -1000.0f);
-  const float r = exp2_fast(d);
-  e = r * fmaf(d, s, e);
-  s *= r;
+// sums relative to 2^to from sums relative to 2^from, from <= to (or both sums 0)
+__device__ __forceinline__ void rescale(float from, float to, float& s, float& e) {
+  const float d = fminf(fmaxf(from - to, -1000.0f), 0.0f);
+  const float f = exp2_approx(d);
+  e = f * fmaf(d, s, e);
+  s *= f;
 }
 
-__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float raised(float v) {   // NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(kLowest));
+  return r;
+}
+// What a 16-byte vector holds, raised to kLowest, and the largest of it.  NaN is kept among the values
+// and passed over by the maximum.
+__device__ __forceinline__ void unpack(const Vec<float>& v, float (&f)[4], float& most) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[j] = raised(v.e[j]);
+    most = fmaxf(most, f[j]);
+  }
+}
+__device__ __forceinline__ void unpack(const Vec<__nv_bfloat16>& v, float (&f)[8], float& most) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v.raw);
+  const __nv_bfloat162 low = __float2bfloat162_rn(kLowest);
+  __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 x = __hmax2_nan(h[j], low);
+    f[2 * j] = __low2float(x);
+    f[2 * j + 1] = __high2float(x);
+  }
+  most = fmaxf(most, fmaxf(__low2float(m), __high2float(m)));
+}
+__device__ __forceinline__ void unpack(const Vec<__half>& v, float (&f)[8], float& most) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v.raw);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = __half22float2(h[j]);
+    f[2 * j] = raised(x.x);
+    f[2 * j + 1] = raised(x.y);
+  }
+  most = fmaxf(most, fmaxf(__low2float(m), __high2float(m)));
+}
 
-template <typename T>
-struct Chunk {   // what a CTA reads between two looks at its candidates
-  static constexpr int kVectors = sizeof(T) == 2 ? 2 : 4;     // per thread
+// How a CTA reads: `kVectors` 16-byte vectors per thread at a time, a chunk, with the next two chunks
+// under way.  With alternatives a chunk is also what is read between two looks at the candidates.
+// The CTAs per SM are what the registers and 80 KB or so of loads in flight come to.
+template <typename T, bool TOP>
+struct Chunk {
+  static constexpr int kThreads = TOP ? 512 : 256, kWarps = kThreads / 32;
+  static constexpr int kCtas = TOP ? 2 : 5;
+  static constexpr int kVectors = 2;
   static constexpr int kElems = kThreads * kVectors * Elem<T>::kPerVec;
 };
 
 struct ClusterShared {
   Partial part[kMaxCluster];
-  unsigned long long keys[kMaxCluster * kTopMax];
+  alignas(16) unsigned long long keys[kMaxCluster * kTopMax + 2];
 };
 
 struct TopState {
-  unsigned long long* list;   // kListKept + a chunk + kThreads
+  unsigned long long* list;   // kListKept + a chunk + the elements around the vectors
   unsigned long long* sorted; // kTopMax
   unsigned long long* warp_best;
   int* count;
@@ -103,49 +145,58 @@ struct TopState {
   int k;
 };
 
+// How many of keys[0, n) are larger than `mine`; keys are 16-byte aligned, with room for one more.
+__device__ __forceinline__ int count_larger(const unsigned long long* keys, int n, unsigned long long mine) {
+  int rank = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; i += 2) {
+    const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + i);
+    rank += (two.x > mine) + (i + 1 < n && two.y > mine);
+  }
+  return rank;
+}
+__device__ __forceinline__ unsigned long long warp_max_key(unsigned long long key) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+  return ((unsigned long long)hi << 32) | lo;
+}
+
 // The k largest of list[0, count) to the front, in order; everyone's threshold becomes the k-th.
 // All threads, after a barrier; ends with one.
+template <int THREADS>
 __device__ __forceinline__ void compact(TopState& t) {
   const int n = *t.count;
   const int tid = threadIdx.x;
-  if (tid < t.k) t.sorted[tid] = 0;
-  __syncthreads();
-  if (n <= kThreads) {
-    if (tid < n) {
-      const unsigned long long mine = t.list[tid];
-      int rank = 0;
-      for (int i = 0; i < n; ++i) rank += t.list[i] > mine;
-      if (rank < t.k) t.sorted[rank] = mine;
-    }
+  if (n <= THREADS) {
+    const unsigned long long mine = tid < n ? t.list[tid] : 0ull;
+    const int rank = tid < n ? count_larger(t.list, n, mine) : THREADS;
+    __syncthreads();
+    if (rank < t.k) t.list[rank] = mine;
+    if (tid >= n && tid < t.k) t.list[tid] = 0;
   } else {
     // k rounds: the largest key below the last one
     unsigned long long last = ~0ull;
     for (int r = 0; r < t.k; ++r) {
       unsigned long long best = 0;
-      for (int i = tid; i < n; i += kThreads) {
+      for (int i = tid; i < n; i += THREADS) {
         const unsigned long long key = t.list[i];
         if (key < last && key > best) best = key;
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-        best = other > best ? other : best;
-      }
+      best = warp_max_key(best);
       if ((tid & 31) == 0) t.warp_best[tid >> 5] = best;
       __syncthreads();
       best = 0;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) best = t.warp_best[w] > best ? t.warp_best[w] : best;
+      for (int w = 0; w < THREADS / 32; ++w) best = t.warp_best[w] > best ? t.warp_best[w] : best;
       last = best;
       if (tid == 0) t.sorted[r] = best;
       __syncthreads();
     }
+    if (tid < t.k) t.list[tid] = t.sorted[tid];
   }
-  __syncthreads();
-  if (tid < t.k) t.list[tid] = t.sorted[tid];
   if (tid == 0) *t.count = n < t.k ? n : t.k;
-  t.threshold = t.sorted[t.k - 1];     // 0 while fewer than k keys are known
   __syncthreads();
+  t.threshold = t.list[t.k - 1];       // 0 while fewer than k keys are known
 }
 
 // Returns whether the list has grown past where it should be cut back.
@@ -157,28 +208,22 @@ __device__ __forceinline__ bool offer(TopState& t, float v, int index) {
   return at >= kListKept;
 }
 
-// In every warp the k-th largest of the lanes' best keys; the largest over the warps, less one so
-// that the key itself passes.
-__device__ __forceinline__ void first_threshold(TopState& t, unsigned long long best) {
-  const int lane = threadIdx.x & 31;
-  // bitonic sort of the 32 keys, descending by lane
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      const bool descending = (lane & size) == 0;
-      const bool lower = (lane & o) == 0;
-      const bool keep_larger = descending == lower;
-      best = (keep_larger == (best > other)) ? best : other;
-    }
-  const unsigned long long kth = __shfl_sync(0xffffffffu, best, t.k - 1);
-  if (lane == 0) t.warp_best[threadIdx.x >> 5] = kth;
+// A lower bound of the k-th largest of the chunk from the threads' best keys, less one so that the key
+// itself passes: over the W warps that have elements, the smallest of their ceil(k / W)-th largest.
+// For values in no order it lets through two or three times k.
+template <int THREADS>
+__device__ __forceinline__ void first_threshold(TopState& t, unsigned long long best, int vectors) {
+  const int w = min((vectors + 31) / 32, THREADS / 32);
+  unsigned long long kth = ~0ull;
+  for (int i = 0; i < (t.k + w - 1) / w; ++i) {
+    kth = warp_max_key(best);
+    if (best == kth) best = 0;
+  }
+  if ((threadIdx.x & 31) == 0) t.warp_best[threadIdx.x >> 5] = kth;
   __syncthreads();
-  unsigned long long most = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) most = t.warp_best[w] > most ? t.warp_best[w] : most;
-  t.threshold = most > 0 ? most - 1 : 0;
+  unsigned long long least = ~0ull;
+  for (int i = 0; i < w; ++i) least = t.warp_best[i] < least ? t.warp_best[i] : least;
+  t.threshold = least > 0 ? least - 1 : 0;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -205,15 +250,52 @@ __device__ __forceinline__ P* in_first_cta(P* p) {
   return reinterpret_cast<P*>(r);
 }
 
+// The row once more, by one CTA: its maximum, then sums of 2^((x - m) * factor), which no size of
+// the logits breaks.  `slots`: one per warp.  All threads; every thread gets the result.
+template <typename T, int THREADS>
+__device__ __noinline__ Partial whole_row(const T* x, int vocab, float factor, Partial* slots) {
+  const int tid = threadIdx.x;
+  float m = -INFINITY;
+  for (int i = tid; i < vocab; i += THREADS) m = fmaxf(m, Elem<T>::to_f32(x[i]));
+  m = warp_max(m);
+  if ((tid & 31) == 0) slots[tid >> 5].m = m;
+  __syncthreads();
+  for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, slots[w].m);
+  float s = 0.0f, e = 0.0f;
+  for (int i = tid; i < vocab; i += THREADS) {
+    const float v = Elem<T>::to_f32(x[i]);
+    if (v == -INFINITY) continue;
+    const float z = (v - m) * factor, q = exp2_approx(z);
+    s += q;
+    e = fmaf(q, fmaxf(z, -1000.0f), e);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    e += __shfl_xor_sync(0xffffffffu, e, o);
+  }
+  if ((tid & 31) == 0) {
+    slots[tid >> 5].s = s;
+    slots[tid >> 5].e = e;
+  }
+  __syncthreads();
+  Partial total{m, 0.0f, 0.0f, 0.0f};
+  for (int w = 0; w < THREADS / 32; ++w) {
+    total.s += slots[w].s;
+    total.e += slots[w].e;
+  }
+  return total;
+}
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p) {
-  constexpr int E = Elem<T>::kPerVec;
-  constexpr int U = Chunk<T>::kVectors;
+__global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas) logprob_kernel(const LogprobParams p) {
+  using C = Chunk<T, TOP>;
+  constexpr int E = Elem<T>::kPerVec, U = C::kVectors, kThreads = C::kThreads, kWarps = C::kWarps;
   __shared__ ClusterShared meet;       // filled by the cluster, in the first CTA
   __shared__ Partial warp_part[kWarps];
   __shared__ unsigned long long sorted[kTopMax], warp_best[kWarps];
   __shared__ int count;
-  extern __shared__ unsigned long long list[];
+  extern __shared__ __align__(16) unsigned long long list[];
 
   const int rank = (int)cluster_rank(), ranks = (int)cluster_size();
   const int row = blockIdx.x / ranks;
@@ -245,46 +327,61 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p
     __syncthreads();
   }
 
-  float m = -INFINITY, s = 0.0f, e = 0.0f;
-  auto take = [&](float v, int index) {      // one element
-    if (v > m) {
-      rescale(m, v, factor, s, e);
-      m = v;
-    }
-    const float z = (v - finite_max(m)) * factor;
-    const float q = exp2_fast(z);
-    s += q;
-    e = fmaf(q, fmaxf(z, -1000.0f), e);
-    if constexpr (TOP) offer(top, v, index);
+  float largest = -INFINITY;           // of the logits as they are
+  float ref = 0.0f;                    // means something once `largest` does
+  unsigned long long s2 = 0ull, e2 = 0ull;         // the sums, in two lanes each
+  const unsigned long long factor2 = pack2(factor, factor);
+  auto raise = [&](float most) {       // the reference moves up to y of `most`
+    largest = most;
+    const float to = fmaxf(fmaxf(most, kLowest) * factor, kLowest);   // never below a raised logit's
+    const float d = fminf(fmaxf(ref - to, -1000.0f), 0.0f);
+    const float f = exp2_approx(d);
+    const unsigned long long f2 = pack2(f, f);
+    e2 = mul2(f2, fma2(pack2(d, d), s2, e2));
+    s2 = mul2(f2, s2);
+    ref = to;
   };
-  bool first = true;
-  for (int base = v0; base < v1; base += kThreads * U) {
-    float v[U * E];
+  auto take2 = [&](float a, float b) {
+    const unsigned long long z2 = fma2(pack2(a, b), factor2, pack2(-ref, -ref));
+    float za, zb;
+    unpack2(z2, za, zb);
+    const unsigned long long q2 = pack2(exp2_approx(za), exp2_approx(zb));
+    s2 = add2(s2, q2);
+    e2 = fma2(q2, z2, e2);
+  };
+  Vec<T> raw[2][U];
+  auto load = [&](Vec<T> (&to)[U], int base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = base + u * kThreads + tid;
-      Vec<T> raw;
-      if (at < v1) raw.raw = ld_once(body + (int64_t)at * E);
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[u * E + j] = at < v1 ? Elem<T>::to_f32(raw.e[j]) : -INFINITY;
+      if (at < v1) to[u].raw = ld_once(body + (int64_t)at * E);
     }
-    float most = v[0];
+  };
+  constexpr int kStep = kThreads * U;
+  auto work = [&](Vec<T> (&from)[U], int base) {
+    float f[U][E], most = -INFINITY;
 #pragma unroll
-    for (int j = 1; j < U * E; ++j) most = fmaxf(most, v[j]);
-    if (most > m) {
-      rescale(m, most, factor, s, e);
-      m = most;
-    }
-    const float ref = finite_max(m);
+    for (int u = 0; u < U; ++u) {
+      if (base + u * kThreads + tid < v1) {
+        unpack(from[u], f[u], most);
+      } else {
 #pragma unroll
-    for (int j = 0; j < U * E; ++j) {
-      const float z = (v[j] - ref) * factor;
-      const float q = exp2_fast(z);
-      s += q;
-      e = fmaf(q, fmaxf(z, -1000.0f), e);
+        for (int j = 0; j < E; ++j) f[u][j] = kLowest;
+      }
     }
+    load(from, base + 2 * kStep);
+    if (most > largest) raise(most);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < E; j += 2) take2(f[u][j], f[u][j + 1]);
     if constexpr (TOP) {
-      if (first) {
+      // a raised logit is one of the few cases where the row itself is asked again
+      auto value = [&](int u, int j, int index) {
+        return f[u][j] < 0.9f * kLowest ? Elem<T>::to_f32(x[index]) : f[u][j];
+      };
+      bool grown = base == v0;
+      if (base == v0) {
         unsigned long long best = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -292,56 +389,76 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p
           if (at < v1) {
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-              const unsigned long long key = make_key(v[u * E + j], head + at * E + j);
+              const unsigned long long key = make_key(value(u, j, head + at * E + j), head + at * E + j);
               best = key > best ? key : best;
             }
           }
         }
-        first_threshold(top, best);
+        first_threshold<kThreads>(top, best, v1 - v0);
       }
-      bool grown = first;
       if (!(most < key_value(top.threshold))) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int at = base + u * kThreads + tid;
           if (at < v1) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) grown |= offer(top, v[u * E + j], head + at * E + j);
+            for (int j = 0; j < E; ++j) grown |= offer(top, value(u, j, head + at * E + j), head + at * E + j);
           }
         }
       }
-      if (__syncthreads_or(grown)) compact(top);     // the same answer in every thread
-      first = false;
+      if (__syncthreads_or(grown)) compact<kThreads>(top);     // the same answer in every thread
     }
+  };
+  load(raw[0], v0);
+  load(raw[1], v0 + kStep);
+  for (int base = v0; base < v1; base += 2 * kStep) {
+    work(raw[0], base);
+    if (base + kStep < v1) work(raw[1], base + kStep);
   }
-  if (rank == 0 && tid < head) take(Elem<T>::to_f32(x[tid]), tid);
-  if (rank == ranks - 1 && tail + tid < vocab) take(Elem<T>::to_f32(x[tail + tid]), tail + tid);
+  // the elements around the vectors, one per thread
+  auto take = [&](int index) {
+    const float v = Elem<T>::to_f32(x[index]);
+    if (v > largest) raise(v);
+    take2(raised(v), kLowest);
+    if constexpr (TOP) offer(top, v, index);
+  };
+  if (rank == 0 && tid < head) take(tid);
+  if (rank == ranks - 1 && tail + tid < vocab) take(tail + tid);
   if constexpr (TOP) {
     __syncthreads();
-    compact(top);
+    compact<kThreads>(top);
   }
 
-  // the CTA's sums: relative to the warp's maximum, then to the CTA's
-  float wm = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-  if (wm > m) rescale(m, wm, factor, s, e);
+  // the CTA's sums: relative to the warp's reference, then to the CTA's
+  float sa, sb, ea, eb;
+  unpack2(s2, sa, sb);
+  unpack2(e2, ea, eb);
+  sa += sb;
+  ea += eb;
+  if (largest == -INFINITY) ref = kNone;
+  const float wr = warp_max(ref);
+  rescale(ref, wr, sa, ea);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    e += __shfl_xor_sync(0xffffffffu, e, o);
+    sa += __shfl_xor_sync(0xffffffffu, sa, o);
+    ea += __shfl_xor_sync(0xffffffffu, ea, o);
   }
-  if ((tid & 31) == 0) warp_part[tid >> 5] = Partial{wm, s, e};
+  largest = warp_max(largest);
+  if ((tid & 31) == 0) warp_part[tid >> 5] = Partial{largest, wr, sa, ea};
   __syncthreads();
+  // n <= 32: a lane per part, the same result in every lane of every warp
   auto merge = [&](const Partial* parts, int n) {
-    Partial sum{-INFINITY, 0.0f, 0.0f};
-    for (int i = 0; i < n; ++i) sum.m = fmaxf(sum.m, parts[i].m);
-    for (int i = 0; i < n; ++i) {
-      Partial q = parts[i];
-      if (sum.m > q.m) rescale(q.m, sum.m, factor, q.s, q.e);
-      sum.s += q.s;
-      sum.e += q.e;
+    const int lane = tid & 31;
+    Partial q = lane < n ? parts[lane] : Partial{-INFINITY, kNone, 0.0f, 0.0f};
+    Partial sum{warp_max(q.m), warp_max(q.r), 0.0f, 0.0f};
+    rescale(q.r, sum.r, q.s, q.e);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      q.s += __shfl_xor_sync(0xffffffffu, q.s, o);
+      q.e += __shfl_xor_sync(0xffffffffu, q.e, o);
     }
+    sum.s = q.s;
+    sum.e = q.e;
     return sum;
   };
   Partial total = merge(warp_part, kWarps);
@@ -349,40 +466,46 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobParams p
     cluster_wait();
     if (tid == 0) *in_first_cta(&meet.part[rank]) = total;
     if constexpr (TOP) {
-      if (tid < p.top) *in_first_cta(&meet.keys[rank * p.top + tid]) = sorted[tid];
+      if (tid < p.top) *in_first_cta(&meet.keys[rank * p.top + tid]) = list[tid];
     }
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
     total = merge(meet.part, ranks);
     if constexpr (TOP) {
-      // at most kMaxCluster * kTopMax = kThreads keys; 0 stands for none
+      // at most kMaxCluster * kTopMax <= kThreads keys; 0 stands for none
       const int n = ranks * p.top;
-      if (tid < p.top) sorted[tid] = 0;
+      if (tid < p.top) list[tid] = 0;
       __syncthreads();
       if (tid < n && meet.keys[tid] != 0) {
         const unsigned long long mine = meet.keys[tid];
-        int r = 0;
-        for (int i = 0; i < n; ++i) r += meet.keys[i] > mine;
-        if (r < p.top) sorted[r] = mine;
+        const int r = count_larger(meet.keys, n, mine);
+        if (r < p.top) list[r] = mine;
       }
       __syncthreads();
     }
   }
-  // a row of nothing but -inf: no probability anywhere
+  float behind = fmaf(total.m, factor, -total.r);    // what rounding took from the reference
+  if (!(fabsf(total.m) < kWide && fabsf(total.m * factor) < kWide)) {   // the same in every thread
+    __syncthreads();                                 // warp_part has been read
+    total = whole_row<T, kThreads>(x, vocab, factor, warp_part);
+    behind = 0.0f;
+  }
+  // a row of nothing but -inf has no probability anywhere
   const bool empty = total.m == -INFINITY && total.s == 0.0f;
-  const float log_s = logf(total.s);
-  auto log_p = [&](float v) { return empty ? -INFINITY : (v - total.m) * p.inv_temperature - log_s; };
+  const float log_s = log2f(total.s);
+  const float ln_s = kLn2 * (log_s - behind);        // of the sum relative to e^(m / T)
+  auto log_p = [&](float v) { return empty ? -INFINITY : fmaf(v - total.m, p.inv_temperature, -ln_s); };
   if (tid == 0) {
-    if (p.lse) p.lse[row] = empty ? -INFINITY : fmaf(total.m, p.inv_temperature, log_s);
-    if (p.entropy) p.entropy[row] = empty ? 0.0f : log_s - kLn2 * (total.e / total.s);
+    if (p.lse) p.lse[row] = empty ? -INFINITY : fmaf(total.m, p.inv_temperature, ln_s);
+    if (p.entropy) p.entropy[row] = empty ? 0.0f : kLn2 * (log_s - total.e / total.s);
     if (p.logprob) p.logprob[row] = token < 0 ? 0.0f : token >= vocab ? NAN : log_p(given);
   }
   if constexpr (TOP) {
     if (tid < p.top) {
-      const int index = key_index(sorted[tid]);
+      const int index = key_index(list[tid]);
       p.top_index[(int64_t)row * p.top + tid] = index;
-      p.top_logprob[(int64_t)row * p.top + tid] = log_p(key_value(sorted[tid]));
+      p.top_logprob[(int64_t)row * p.top + tid] = log_p(key_value(list[tid]));
     }
   }
 }
@@ -429,7 +552,7 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
   const bool empty = lse < -1e30f;
   auto grad = [&](float v, int index) {
     const float z = fmaf(v, p.inv_temperature, -lse);       // log p
-    const float q = exp2_fast(z * kLog2e);
+    const float q = exp2_approx(z * kLog2e);
     const float d = -q * fmaf(ge, fmaxf(z, -1000.0f), shift) + (index == token ? g : 0.0f);
     return empty ? 0.0f : d * p.inv_temperature;
   };
@@ -470,18 +593,20 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
 template <typename T, bool TOP>
 int launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
   auto kern = logprob_kernel<T, TOP>;
-  constexpr int kList = kListKept + Chunk<T>::kElems + kThreads;
-  static_assert(kList * 8 + sizeof(ClusterShared) + 1024 <= 48 * 1024, "no opt-in is asked for");
+  using C = Chunk<T, TOP>;
+  constexpr int kList = kListKept + C::kElems + 16;
   const int smem = TOP ? kList * (int)sizeof(unsigned long long) : 0;
+  if (TOP)
+    if (int rc = prepare_kernel((const void*)kern, smem)) return rc;
   // CTAs per row: until the rows fill the chip twice over, as long as each has a chunk to read
   const int sms = device_info().sm_count;
   int ranks = 1;
   while (ranks < kMaxCluster && (int64_t)p.rows * ranks * 2 <= 4 * sms &&
-         p.vocab >= ranks * 2 * Chunk<T>::kElems)
+         p.vocab >= ranks * 2 * C::kElems)
     ranks *= 2;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)p.rows * ranks);
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(C::kThreads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr;
@@ -511,8 +636,8 @@ int check_logits(const char* what, int64_t rows, int64_t vocab, float inv_temper
   if (rows > (1 << 24) || vocab > (1 << 30))
     return fail(NB200_E_INVALID, "%s: too large (rows=%lld vocab=%lld)", what, (long long)rows,
                 (long long)vocab);
-  if (!(inv_temperature > 0.0f) || inv_temperature > 1e30f)
-    return fail(NB200_E_INVALID, "%s: the inverse temperature must be positive and finite", what);
+  if (!(inv_temperature >= 1e-20f && inv_temperature <= 1e20f))
+    return fail(NB200_E_INVALID, "%s: the inverse temperature must be between 1e-20 and 1e20", what);
   if (dtype != NB200_F32 && dtype != NB200_F16 && dtype != NB200_BF16)
     return fail(NB200_E_INVALID, "%s: unknown dtype code %d", what, dtype);
   return 0;

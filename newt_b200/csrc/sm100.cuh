@@ -565,6 +565,12 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   return r;
 }
 
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 __device__ __forceinline__ unsigned long long sub2(unsigned long long a, unsigned long long b) {
   unsigned long long r;
   asm("sub.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
