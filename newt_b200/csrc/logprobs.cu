@@ -26,7 +26,6 @@
 // Rows of any alignment are read in 16-byte vectors from their first 16-byte boundary on, with
 // the elements before and after them one by one.
 
-#include "common.cuh"
 #include "elem.cuh"
 #include "sm100.cuh"
 
@@ -126,7 +125,7 @@ __device__ __forceinline__ void unpack(const Vec<__half>& v, float (&f)[8], floa
 template <typename T, bool TOP>
 struct Chunk {
   static constexpr int kThreads = TOP ? 512 : 256, kWarps = kThreads / 32;
-  static constexpr int kCtas = TOP ? 2 : 5;
+  static constexpr int kCtas = TOP ? 2 : 4;
   static constexpr int kVectors = 2;
   static constexpr int kElems = kThreads * kVectors * Elem<T>::kPerVec;
 };
@@ -350,19 +349,25 @@ __global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas)
     e2 = fma2(q2, z2, e2);
   };
   Vec<T> raw[2][U];
-  auto load = [&](Vec<T> (&to)[U], int base) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = base + u * kThreads + tid;
-      if (at < v1) to[u].raw = ld_once(body + (int64_t)at * E);
-    }
-  };
   constexpr int kStep = kThreads * U;
-  auto work = [&](Vec<T> (&from)[U], int base) {
+  const T* next = body + (int64_t)(v0 + tid) * E;      // of the next chunk to be loaded
+  auto load = [&](Vec<T> (&to)[U], int base) {
+    if (base + kStep <= v1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) to[u].raw = ld_once(next + u * kThreads * E);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (base + u * kThreads + tid < v1) to[u].raw = ld_once(next + u * kThreads * E);
+    }
+    next += kStep * E;
+  };
+  // full: every thread has all of its vectors (a constant wherever this is inlined)
+  auto work = [&](const bool full, Vec<T> (&from)[U], int base) {
     float f[U][E], most = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (base + u * kThreads + tid < v1) {
+      if (full || base + u * kThreads + tid < v1) {
         unpack(from[u], f[u], most);
       } else {
 #pragma unroll
@@ -411,10 +416,13 @@ __global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas)
   };
   load(raw[0], v0);
   load(raw[1], v0 + kStep);
-  for (int base = v0; base < v1; base += 2 * kStep) {
-    work(raw[0], base);
-    if (base + kStep < v1) work(raw[1], base + kStep);
+  int base = v0;
+  for (; base + 2 * kStep <= v1; base += 2 * kStep) {
+    work(true, raw[0], base);
+    work(true, raw[1], base + kStep);
   }
+  if (base < v1) work(false, raw[0], base);
+  if (base + kStep < v1) work(false, raw[1], base + kStep);
   // the elements around the vectors, one per thread
   auto take = [&](int index) {
     const float v = Elem<T>::to_f32(x[index]);
