@@ -115,10 +115,25 @@ __device__ __forceinline__ void store_elems(T* row, int col, int n, const float*
 
 // Two fp32 values as e4m3, `lo` in the low byte; beyond +-448 they become +-448, NaN stays NaN.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-  return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+      "mov.b32 %0, {lo, hi};\n\t}"
+      : "=r"(r)
+      : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+// Two e4m3 numbers (low byte first) as fp16, exactly.
+__device__ __forceinline__ float2 e4m3x2_values(uint32_t q) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)q));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 // E values times `inv` as e4m3, at columns [col, col + E) of a row of n.

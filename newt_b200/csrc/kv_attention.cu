@@ -263,8 +263,7 @@ struct Shared {
 // Two values as e4m3 (low and high byte), and what is left of them, times 16.
 __device__ __forceinline__ uint32_t split2(float& a, float& b) {
   const uint32_t q = e4m3x2(a, b);
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q, __NV_E4M3);
-  const float2 f = __half22float2(__half2(h));
+  const float2 f = e4m3x2_values(q);
   a = (a - f.x) * 16.0f;
   b = (b - f.y) * 16.0f;
   return q;
