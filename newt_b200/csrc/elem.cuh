@@ -1,5 +1,4 @@
-// Element types as fp32 arithmetic sees them, and 16-byte vectors of them with an element-wise
-// form for rows that are not aligned.  Used by the norm, cache and log-probability kernels.
+// Element types as fp32 arithmetic sees them, 16-byte vectors of them, and conversions to e4m3.  Used by the norm, cache and log-probability kernels.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -61,29 +60,6 @@ __device__ __forceinline__ void st_once(void* p, uint4 v) {
 
 __host__ __device__ __forceinline__ bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// The vector of columns [col, col + kPerVec) of a row of n; columns past n give 0.
-// FAST: the row is 16-byte aligned and n a multiple of the vector.
-template <typename T, bool FAST, bool ONCE>
-__device__ __forceinline__ Vec<T> load_row_vec(const T* row, int col, int n) {
-  constexpr int E = Elem<T>::kPerVec;
-  Vec<T> v;
-  if ((FAST || at16(row)) && col + E <= n) {
-    v.raw = ONCE ? ld_once(row + col) : __ldg(reinterpret_cast<const uint4*>(row + col));
-  } else {
-#pragma unroll
-    for (int j = 0; j < E; ++j) v.e[j] = (!FAST && col + j < n) ? row[col + j] : Elem<T>::from_f32(0.0f);
-  }
-  return v;
-}
-template <typename T, bool FAST>
-__device__ __forceinline__ Vec<T> load_elems(const T* row, int col, int n) {
-  return load_row_vec<T, FAST, true>(row, col, n);
-}
-template <typename T, bool FAST>
-__device__ __forceinline__ Vec<T> load_cached(const T* row, int col, int n) {
-  return load_row_vec<T, FAST, false>(row, col, n);
-}
-
 // kPerVec fp32 values as one vector of T, each rounded once.
 template <typename T>
 __device__ __forceinline__ Vec<T> round_elems(const float* v) {
@@ -98,19 +74,6 @@ __device__ __forceinline__ Vec<T> round_elems(const float* v) {
     for (int j = 0; j < E; ++j) o.e[j] = v[j];
   }
   return o;
-}
-
-template <typename T, bool FAST>
-__device__ __forceinline__ void store_elems(T* row, int col, int n, const float* v) {
-  constexpr int E = Elem<T>::kPerVec;
-  const Vec<T> o = round_elems<T>(v);
-  if ((FAST || at16(row)) && col + E <= n) {
-    st_once(row + col, o.raw);
-  } else if constexpr (!FAST) {
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (col + j < n) row[col + j] = o.e[j];
-  }
 }
 
 // Two fp32 values as e4m3, `lo` in the low byte; beyond +-448 they become +-448, NaN stays NaN.
@@ -136,23 +99,17 @@ __device__ __forceinline__ float2 e4m3x2_values(uint32_t q) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// E values times `inv` as e4m3, at columns [col, col + E) of a row of n.
-template <int E, bool FAST>
-__device__ __forceinline__ void store_e4m3(uint8_t* row, int col, int n, const float* v, float inv) {
+// E values times `factor` as e4m3; `to` is E-byte aligned.
+template <int E>
+__device__ __forceinline__ void store_e4m3(uint8_t* to, const float* v, float factor) {
   uint32_t words[E / 4];
 #pragma unroll
   for (int j = 0; j < E; j += 4)
-    words[j / 4] = e4m3x4(v[j] * inv, v[j + 1] * inv, v[j + 2] * inv, v[j + 3] * inv);
-  if ((FAST || reinterpret_cast<uintptr_t>(row) % E == 0) && col + E <= n) {
-    if constexpr (E == 8)
-      *reinterpret_cast<uint2*>(row + col) = make_uint2(words[0], words[1]);
-    else
-      *reinterpret_cast<uint32_t*>(row + col) = words[0];
-  } else if constexpr (!FAST) {
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (col + j < n) row[col + j] = (uint8_t)(words[j / 4] >> (8 * (j % 4)));
-  }
+    words[j / 4] = e4m3x4(v[j] * factor, v[j + 1] * factor, v[j + 2] * factor, v[j + 3] * factor);
+  if constexpr (E == 8)
+    *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
+  else
+    *reinterpret_cast<uint32_t*>(to) = words[0];
 }
 
 }  // namespace nb200

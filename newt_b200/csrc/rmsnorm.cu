@@ -16,17 +16,23 @@
 
 #include "common.cuh"
 #include "elem.cuh"
+#include "sm100.cuh"
 
 namespace nb200 {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;
 
-// The scale of values of magnitude up to `most`: 1 where they are all zero, or so small that the
-// quotient is no normal number (they become zeros).
+// The scale of values of magnitude up to `most`, and what they are multiplied with: 1 where they are
+// all zero, or so small that the scale is no normal number (they become zeros).  Neither is the
+// correctly rounded quotient (2^-22 relative, against e4m3's 2^-4): a division per vector would be a
+// third of the kernel's instructions.
 __device__ __forceinline__ float e4m3_scale(float most) {
-  const float s = most / kE4m3Max;
+  const float s = most * (1.0f / kE4m3Max);
   return s >= 1.17549435e-38f ? s : 1.0f;
+}
+__device__ __forceinline__ float e4m3_factor(float most) {
+  return most * (1.0f / kE4m3Max) >= 1.17549435e-38f ? __fdividef(kE4m3Max, most) : 1.0f;
 }
 
 struct RmsParams {
@@ -36,7 +42,8 @@ struct RmsParams {
   void* out;
   void* residual_out;     // null: not wanted
   float* scales;          // e4m3 only: [rows, ceil(n / group)]
-  int rows, n, group;     // group: columns per scale (n: one scale per row)
+  int rows, n;
+  int group_shift;        // log2 of the columns per scale; 0: one scale per row
   int threads;            // per row
   int64_t stride_x, stride_residual, stride_out, stride_residual_out, stride_scales;
   float eps;
@@ -64,14 +71,17 @@ struct Max {   // of magnitudes: 0 is neutral
 };
 
 // FAST: every row of every tensor starts on a 16-byte boundary (8-byte for the e4m3 output of a
-// 16-bit type) and n is a multiple of the vector, so no element-wise path is compiled.
-template <typename T, bool E4M3, int ITEMS, bool FAST>
-__global__ void __launch_bounds__(1024) rms_kernel(const RmsParams p) {
+// 16-bit type) and n is a multiple of the vector: a thread's E columns are neighbours.  Otherwise a
+// warp's 32 * E columns are the same but a thread's lie 32 apart, so that every access of a warp is
+// one run of elements whatever the row's alignment (8191 x 4097 fp16: 162 us with E neighbours read
+// one by one and as many stores of a byte or two, 160 like this: the count of accesses is what is left).
+template <typename T, bool E4M3, int ITEMS, bool FAST, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
   constexpr int E = Elem<T>::kPerVec;
   __shared__ float slots[2][32];
   const int warps = p.threads >> 5;
   const int per_cta = blockDim.x / p.threads;
-  const int lane = threadIdx.x % p.threads;
+  const int lane = threadIdx.x % p.threads;       // of the row
   const int64_t row = (int64_t)blockIdx.x * per_cta + threadIdx.x / p.threads;
   if (warps > 1) {
     if (threadIdx.x < 64) slots[threadIdx.x >> 5][threadIdx.x & 31] = 0.0f;
@@ -82,89 +92,138 @@ __global__ void __launch_bounds__(1024) rms_kernel(const RmsParams p) {
   const T* x = static_cast<const T*>(p.x) + row * p.stride_x;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.stride_residual : nullptr;
   const T* w = static_cast<const T*>(p.w);
+  const int col0 = FAST ? lane * E : (lane >> 5) * 32 * E + (lane & 31), col_step = p.threads * E;
+  auto column = [&](int i, int j) { return col0 + i * col_step + (FAST ? j : 32 * j); };
 
-  Vec<T> xv[ITEMS], rv[ITEMS];
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) xv[i] = load_elems<T, FAST>(x, (i * p.threads + lane) * E, n);
-  if (res) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) rv[i] = load_elems<T, FAST>(res, (i * p.threads + lane) * E, n);
-  }
-  float v[ITEMS * E];
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      float h = Elem<T>::to_f32(xv[i].e[j]);
-      if (res) h += Elem<T>::to_f32(rv[i].e[j]);
-      v[i * E + j] = h;          // columns past n hold 0
-      sum = fmaf(h, h, sum);
-    }
-  if (p.residual_out) {
-    T* out = static_cast<T*>(p.residual_out) + row * p.stride_residual_out;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      store_elems<T, FAST>(out, (i * p.threads + lane) * E, n, &v[i * E]);
-  }
-  sum = reduce_row<Add>(sum, slots[0], warps);
-  const float rstd = rsqrtf(sum / (float)n + p.eps);
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const Vec<T> wv = load_cached<T, FAST>(w, (i * p.threads + lane) * E, n);
-#pragma unroll
-    for (int j = 0; j < E; ++j) v[i * E + j] = v[i * E + j] * rstd * Elem<T>::to_f32(wv.e[j]);
-  }
-
-  if constexpr (!E4M3) {
-    T* out = static_cast<T*>(p.out) + row * p.stride_out;
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      store_elems<T, FAST>(out, (i * p.threads + lane) * E, n, &v[i * E]);
-  } else {
-    float amax[ITEMS];
+  // this thread's part of a row; columns past n are 0
+  auto read = [&](const T* from, bool once, Vec<T> (&to)[ITEMS]) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      amax[i] = 0.0f;
+      if constexpr (FAST) {
+        to[i].raw = make_uint4(0, 0, 0, 0);
+        if (column(i, 0) < n)
+          to[i].raw = once ? ld_once(from + column(i, 0)) : __ldg(reinterpret_cast<const uint4*>(from + column(i, 0)));
+      } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) amax[i] = fmaxf(amax[i], fabsf(v[i * E + j]));
+        for (int j = 0; j < E; ++j)
+          to[i].e[j] = column(i, j) < n ? from[column(i, j)] : Elem<T>::from_f32(0.0f);
+      }
+    }
+  };
+  auto write = [&](T* to, const float (&from)[ITEMS * E]) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if constexpr (FAST) {
+        if (column(i, 0) < n) st_once(to + column(i, 0), round_elems<T>(&from[i * E]).raw);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (column(i, j) < n) to[column(i, j)] = Elem<T>::from_f32(from[i * E + j]);
+      }
+    }
+  };
+
+  Vec<T> xv[ITEMS], rv[ITEMS];
+  read(x, true, xv);
+  if (res) read(res, true, rv);
+  float v[ITEMS * E];
+#pragma unroll
+  for (int k = 0; k < ITEMS * E; ++k) v[k] = Elem<T>::to_f32(xv[k / E].e[k % E]);
+  if (res) {
+#pragma unroll
+    for (int k = 0; k < ITEMS * E; ++k) v[k] += Elem<T>::to_f32(rv[k / E].e[k % E]);
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < ITEMS * E; ++k) sum = fmaf(v[k], v[k], sum);
+  if (p.residual_out) write(static_cast<T*>(p.residual_out) + row * p.stride_residual_out, v);
+  sum = reduce_row<Add>(sum, slots[0], warps);
+  const float rstd = rsqrtf(sum / (float)n + p.eps);
+  read(w, false, xv);
+#pragma unroll
+  for (int k = 0; k < ITEMS * E; ++k) v[k] = v[k] * rstd * Elem<T>::to_f32(xv[k / E].e[k % E]);
+
+  if constexpr (!E4M3) {
+    write(static_cast<T*>(p.out) + row * p.stride_out, v);
+  } else {
+    float amax[ITEMS][FAST ? 1 : E];      // of a thread's columns: one scale for all of them, or for each
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      amax[i][0] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) amax[i][0] = fmaxf(amax[i][0], fabsf(v[i * E + j]));
     }
     float* scales = p.scales + row * p.stride_scales;
-    if (p.group >= n) {
+    if (p.group_shift == 0) {
+      float most = amax[0][0];
 #pragma unroll
-      for (int i = 1; i < ITEMS; ++i) amax[0] = fmaxf(amax[0], amax[i]);
-      const float most = reduce_row<Max>(amax[0], slots[1], warps);
+      for (int i = 1; i < ITEMS; ++i) most = fmaxf(most, amax[i][0]);
+      most = reduce_row<Max>(most, slots[1], warps);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) amax[i] = most;
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int j = 0; j < (FAST ? 1 : E); ++j) amax[i][j] = most;
       if (lane == 0) scales[0] = e4m3_scale(most);
-    } else {
-      // `group` is 32, 64 or 128: E columns per lane, so 4 to 32 neighbouring lanes share a group
-      const int lanes = p.group / E;
+    } else if constexpr (FAST) {
+      // a group is 32, 64 or 128 columns: 4 to 32 neighbouring lanes
+      const int lanes = (1 << p.group_shift) / E;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         for (int o = lanes >> 1; o > 0; o >>= 1)
-          amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
-        const int col = (i * p.threads + lane) * E;
-        if (lane % lanes == 0 && col < n) scales[col / p.group] = e4m3_scale(amax[i]);
+          amax[i][0] = fmaxf(amax[i][0], __shfl_xor_sync(0xffffffffu, amax[i][0], o));
+        const int col = column(i, 0);
+        if ((lane & (lanes - 1)) == 0 && col < n) scales[col >> p.group_shift] = e4m3_scale(amax[i][0]);
+      }
+    } else {
+      // a group is one, two or four neighbouring runs of 32 columns
+      const int runs = 1 << (p.group_shift - 5);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) amax[i][j] = sm100::warp_max(fabsf(v[i * E + j]));
+#pragma unroll
+        for (int step = 1; step < 4; step *= 2) {
+          if (step >= runs) break;
+#pragma unroll
+          for (int j = 0; j < E; j += 2 * step) {
+            const float most = fmaxf(amax[i][j], amax[i][j + step]);
+#pragma unroll
+            for (int k = 0; k < 2 * step; ++k) amax[i][j + k] = most;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const int col = column(i, j) - (lane & 31);
+          if ((lane & 31) == 0 && (j & (runs - 1)) == 0 && col < n) scales[col >> p.group_shift] = e4m3_scale(amax[i][j]);
+        }
       }
     }
     uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.stride_out;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      store_e4m3<E, FAST>(out, (i * p.threads + lane) * E, n, &v[i * E], 1.0f / e4m3_scale(amax[i]));
+      if constexpr (FAST) {
+        if (column(i, 0) < n) store_e4m3<E>(out + column(i, 0), &v[i * E], e4m3_factor(amax[i][0]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (column(i, j) < n) out[column(i, j)] = (uint8_t)e4m3x2(v[i * E + j] * e4m3_factor(amax[i][j]), 0.0f);
+      }
     }
   }
 }
 
 template <typename T, bool E4M3, int ITEMS>
 int launch_rms(const RmsParams& p, bool fast, cudaStream_t stream) {
-  const int per_cta = p.threads == 32 ? 8 : 1;
-  const int64_t grid = cdiv64(p.rows, per_cta);
-  if (fast)
-    rms_kernel<T, E4M3, ITEMS, true><<<(int)grid, p.threads * per_cta, 0, stream>>>(p);
-  else
-    rms_kernel<T, E4M3, ITEMS, false><<<(int)grid, p.threads * per_cta, 0, stream>>>(p);
-  return cuda_check(cudaGetLastError(), "rmsnorm launch");
+  const int threads = p.threads == 32 ? 256 : p.threads;
+  const int64_t grid = cdiv64(p.rows, threads / p.threads);
+  auto go = [&](auto kern) {
+    kern<<<(int)grid, threads, 0, stream>>>(p);
+    return cuda_check(cudaGetLastError(), "rmsnorm launch");
+  };
+  // up to 256 threads a CTA may have 255 registers a thread, 1024 have 64
+  if (threads <= 256)
+    return fast ? go(rms_kernel<T, E4M3, ITEMS, true, 256>) : go(rms_kernel<T, E4M3, ITEMS, false, 256>);
+  return fast ? go(rms_kernel<T, E4M3, ITEMS, true, 1024>) : go(rms_kernel<T, E4M3, ITEMS, false, 1024>);
 }
 
 template <typename T, bool E4M3>
@@ -182,9 +241,13 @@ int dispatch_rms(RmsParams p, cudaStream_t stream) {
   const int64_t vectors = cdiv64(p.n, E);
   int items = 1;
   p.threads = 32;
+  // Few rows: as many threads as there are vectors, the row's latency counts (8 rows of 4096 bf16:
+  // 2.7 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
+  // rows of 4096 fp16: 49.7 us with one, 41.5 with two, 40.2 with four).
+  const int most = p.rows >= 2 * device_info().sm_count ? 4 : 1;
   while ((int64_t)p.threads * items < vectors) {
-    if (items < 2) items = 2;
-    else if (p.threads < 1024) p.threads = p.threads * 2;
+    if (items < most) items *= 2;
+    else if (p.threads < 1024) p.threads *= 2;
     else items *= 2;
   }
   switch (items) {
@@ -235,7 +298,7 @@ extern "C" int nb200_rmsnorm(const void* x, const void* residual, const void* w,
   p.scales = scales;
   p.rows = (int)rows;
   p.n = (int)n;
-  p.group = group ? (int)group : (int)n;
+  p.group_shift = group == 0 ? 0 : group == 32 ? 5 : group == 64 ? 6 : 7;
   p.threads = 0;
   p.stride_x = stride_x;
   p.stride_residual = stride_residual;
