@@ -550,19 +550,27 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
   const int tail = head + vectors * E;
   const bool out_ok = at16(out + head);
 
+  // d_j = q_j (slope max(log p_j, -1000) + offset), and at the token `hit` more; everything times 1/T
   const int64_t token = p.tokens ? p.tokens[row] : -1;
-  const float lse = p.lse[row];
+  float lse = p.lse[row];
   // a token outside the vocabulary has no gradient; neither has a row without any probability
-  const float g = (p.grad_logprob && token >= 0 && token < p.vocab) ? p.grad_logprob[row] : 0.0f;
-  const float ge = p.grad_entropy ? p.grad_entropy[row] : 0.0f;
-  const float shift = p.grad_entropy ? fmaf(ge, p.entropy[row], g) : g;   // g + gH H
   // (all -inf, or all at the lowest value of a wide type, where fp32 has no room for log p)
-  const bool empty = lse < -1e30f;
-  auto grad = [&](float v, int index) {
-    const float z = fmaf(v, p.inv_temperature, -lse);       // log p
-    const float q = exp2_approx(z * kLog2e);
-    const float d = -q * fmaf(ge, fmaxf(z, -1000.0f), shift) + (index == token ? g : 0.0f);
-    return empty ? 0.0f : d * p.inv_temperature;
+  const bool empty = lse < -1e30f, given = token >= 0 && token < p.vocab && !empty;
+  const float g = (p.grad_logprob && given) ? p.grad_logprob[row] : 0.0f;
+  const float ge = (p.grad_entropy && !empty) ? p.grad_entropy[row] : 0.0f;
+  const float hit = g * p.inv_temperature, slope = -ge * p.inv_temperature;
+  const float offset = (p.grad_entropy && !empty ? fmaf(slope, p.entropy[row], -hit) : -hit);
+  const int at_token = given ? (int)token : -1;
+  if (empty) lse = INFINITY;                         // every p is 0
+  const unsigned long long inv2 = pack2(p.inv_temperature, p.inv_temperature), lse2 = pack2(-lse, -lse);
+  const unsigned long long log2e2 = pack2(kLog2e, kLog2e), slope2 = pack2(slope, slope), offset2 = pack2(offset, offset);
+  auto grad2 = [&](float& a, float& b) {             // two logits become their gradients
+    const unsigned long long z2 = fma2(pack2(a, b), inv2, lse2);       // log p
+    float za, zb, ya, yb;
+    unpack2(z2, za, zb);
+    unpack2(mul2(z2, log2e2), ya, yb);
+    const unsigned long long c2 = pack2(fmaxf(za, -1000.0f), fmaxf(zb, -1000.0f));   // 0 times -inf is none of ours
+    unpack2(mul2(pack2(exp2_approx(ya), exp2_approx(yb)), fma2(slope2, c2, offset2)), a, b);
   };
   const int base = blockIdx.x * kThreads * kGradVectors + threadIdx.x;
   Vec<T> raw[kGradVectors];
@@ -578,7 +586,14 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
     const int col = head + at * E;
     float d[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) d[j] = grad(Elem<T>::to_f32(raw[u].e[j]), col + j);
+    for (int j = 0; j < E; ++j) d[j] = Elem<T>::to_f32(raw[u].e[j]);
+#pragma unroll
+    for (int j = 0; j < E; j += 2) grad2(d[j], d[j + 1]);
+    if ((unsigned)(at_token - col) < (unsigned)E) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (col + j == at_token) d[j] += hit;
+    }
     const Vec<T> o = round_elems<T>(d);
     if (out_ok) {
       st_once(out + col, o.raw);
@@ -591,7 +606,9 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
     const int extra = head + (p.vocab - tail);
     if ((int)threadIdx.x < extra) {
       const int col = (int)threadIdx.x < head ? threadIdx.x : tail + threadIdx.x - head;
-      out[col] = Elem<T>::from_f32(grad(Elem<T>::to_f32(x[col]), col));
+      float d = Elem<T>::to_f32(x[col]), none = 0.0f;
+      grad2(d, none);
+      out[col] = Elem<T>::from_f32(col == at_token ? d + hit : d);
     }
   }
 }
