@@ -46,16 +46,16 @@ constexpr int kHalf = 128;               // tokens of one product: a thread's an
 constexpr int kSmemPerCta = 106 * 1024;
 constexpr int kThreads = 192;            // producer, issuer, four softmax warps
 constexpr int kSoftmaxWarp = 2;
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
 constexpr int kMinShare = 1;             // tiles
 constexpr int kWholeItems = 3;           // tiles
-constexpr int kMaxShares = kJoinThreads;
+constexpr int kMaxShares = 320;          // two CTAs on each of 148 SMs
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastScale = 8.67361738e-19f;   // 2^-60
-constexpr float kProbScale = 256.0f;     // probabilities of a tile are at most 1
+constexpr float kProbLog2 = 8.0f;        // a tile's largest probability is 2^8 as an operand: e4m3 ends at 448
 
 enum : unsigned int {
-  ST_KV_Q = 32, ST_KV_K, ST_KV_V, ST_KV_EMPTY, ST_KV_SCALES, ST_KV_S, ST_KV_P, ST_KV_O, ST_KV_ZERO
+  ST_KV_Q = 32, ST_KV_K, ST_KV_V, ST_KV_EMPTY, ST_KV_SCALES, ST_KV_S, ST_KV_P, ST_KV_O, ST_KV_ZERO, ST_KV_MOST, ST_KV_SUM
 };
 
 struct KvAttnParams {
@@ -256,7 +256,7 @@ struct Shared {
   float most[2][4][RP];                        // the warps' maxima, alternating by tile
   float sum[4][RP];
   uint64_t full[S::kSlots], empty[S::kSlots], scale_full[4];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], most_full[2], sum_full;
   uint32_t tmem_slot, abort_flag;
 };
 
@@ -268,19 +268,14 @@ __device__ __forceinline__ uint32_t split2(float& a, float& b) {
   b = (b - f.y) * 16.0f;
   return q;
 }
-
-// Softmax threads: 0..127 here.  `ok` of all of them, behind a barrier.
-__device__ __forceinline__ bool all_of_group(bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)ok)
-      : "memory");
-  return r != 0;
+// The same for a pair of fp16.
+__device__ __forceinline__ uint32_t split2(__half2& h) {
+  uint16_t q;
+  uint32_t back;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q));
+  h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.0f));
+  return q;
 }
 
 // Queries of one item on their way from global memory to their e4m3 parts: 8 columns of a row per
@@ -381,7 +376,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_init(smem_u32(&sh.s_full[x]), 1);
       mbar_init(smem_u32(&sh.p_full[x]), 4);
       mbar_init(smem_u32(&sh.o_full[x]), 1);
+      mbar_init(smem_u32(&sh.most_full[x]), 4);
     }
+    mbar_init(smem_u32(&sh.sum_full), 4);
     mbar_init_fence();
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
@@ -548,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[0]));
-      all_of_group(true);            // the rows' factors and positions are written
+      named_barrier_sync(1, 128);    // the rows' factors and positions are written
     }
 
     int item = 0;
@@ -580,8 +577,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     };
     const int step_shift = p.page_shift - 2 - (H - 1);       // 32 pages are 2^step_shift tiles
-    bool alive = true;
-    for (int j = 0; c.left > 0 && alive; ++item) {
+    for (int j = 0; c.left > 0 && ok; ++item) {
       // one item, as much of it as the share has
       const int to_end = c.seq.count - c.at.tile;
       const int n = min(to_end, c.left);
@@ -596,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int r = 0; r < RP; ++r) factor[r] = sh.q_factor[item & 1][r];
 
-      for (int k = 0; k < n; ++k, ++j) {
+      for (int k = 0; k < n && ok; ++k, ++j) {
         const int x = j & 1;
         const int t0 = tile_start(p, c.seq, c.at.tile + k);
         constexpr int kTokens = kHalf * H;
@@ -604,12 +600,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         const bool clean = t0 + kTokens <= c.seq.limit && t0 + kTokens - 1 <= c.seq.len - p.nq &&
                            (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTokens <= p.sinks);
         const int step = j >> step_shift;
-        ok = ok && mbar_wait_nocall(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j);
-        ok = ok && mbar_wait_nocall(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
+        ok = mbar_wait_nocall(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j) &&
+             mbar_wait_nocall(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
         ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         float s[H][RP], inv_vs[H];
         bool there[H];
-        if (ok) {
+        {
           tc_fence_after_sync();
           uint32_t raw[H][N];
 #pragma unroll
@@ -634,7 +631,11 @@ __global__ void __launch_bounds__(kThreads, 2)
               for (int part = PARTS - 2; part >= 0; --part)
                 v = fmaf(v, 0.0625f, __uint_as_float(raw[h][part * RP + r]));
               // a row that only pads has a product of zero and is as good as any: nobody reads it
-              s[h][r] = there[h] ? fmaf(v, factor[r] * scale.x, scale.y) : -INFINITY;
+              s[h][r] = fmaf(v, factor[r] * scale.x, scale.y);
+            }
+            if (!there[h]) {
+#pragma unroll
+              for (int r = 0; r < RP; ++r) s[h][r] = -INFINITY;
             }
             if (!clean) {                          // tokens that some rows do not see
               const int* at = sh.q_at[item & 1];
@@ -652,27 +653,26 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int r = 0; r < RP; r += 4)
               *reinterpret_cast<float4*>(&sh.most[x][quarter][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
+            mbar_arrive(smem_u32(&sh.most_full[x]));
           }
         }
-        if (!all_of_group(ok)) {
-          alive = false;
-          break;
-        }
-        float mt[RP];
+        // the tile before joins the sums while the warps' maxima get together
+        if (k > 0) add_product(j - 1);
+        ok = ok && mbar_wait_nocall(smem_u32(&sh.most_full[x]), (j >> 1) & 1, ctx, ST_KV_MOST, j);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float mt[RP];      // the reference the tile's probabilities are relative to
 #pragma unroll
         for (int r = 0; r < RP; r += 4) {
-          float4 w = *reinterpret_cast<const float4*>(&sh.most[x][0][r]);
+          float4 w[4];
 #pragma unroll
-          for (int i = 1; i < 4; ++i) {
-            const float4 o = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
-            w = make_float4(fmaxf(w.x, o.x), fmaxf(w.y, o.y), fmaxf(w.z, o.z), fmaxf(w.w, o.w));
-          }
-          mt[r] = w.x;
-          mt[r + 1] = w.y;
-          mt[r + 2] = w.z;
-          mt[r + 3] = w.w;
+          for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
+          mt[r] = fmaxf(max3(w[0].x, w[1].x, w[2].x), w[3].x) - kProbLog2;
+          mt[r + 1] = fmaxf(max3(w[0].y, w[1].y, w[2].y), w[3].y) - kProbLog2;
+          mt[r + 2] = fmaxf(max3(w[0].z, w[1].z, w[2].z), w[3].z) - kProbLog2;
+          mt[r + 3] = fmaxf(max3(w[0].w, w[1].w, w[2].w), w[3].w) - kProbLog2;
         }
-        // probabilities relative to the tile's maximum (0 where the row sees nothing of it), in parts
+        // probabilities (0 where the row sees nothing of the tile), rounded to fp16, in parts
         float lt[RP];                              // this thread's part of the tile's row sums
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -684,11 +684,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int i = 0; i < 2; ++i) {
               pr[i] = exp2_approx(s[h][r + i] - (mt[r + i] == -INFINITY ? 0.0f : mt[r + i]));
               lt[r + i] = h == 0 ? pr[i] * inv_vs[0] : fmaf(pr[i], inv_vs[h], lt[r + i]);
-              pr[i] *= kProbScale;
             }
+            __half2 pair = __floats2half2_rn(pr[0], pr[1]);
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
-              const uint32_t q = split2(pr[0], pr[1]);
+              const uint32_t q = split2(pair);
               if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
             }
           }
@@ -709,7 +709,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             ok = __all_sync(0xffffffffu, ok);
             if (!there[h]) {
 #pragma unroll
-              for (int i = 0; i < D; i += 16) st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + i]), 0, 0, 0, 0);
+              for (int i = 0; i < D; i += 16)     // neighbours start at different banks
+                st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + ((i + me * 16) & (D - 1))]), 0, 0, 0, 0);
             }
           }
         }
@@ -726,9 +727,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[y]));
         }
 
-        // the tile before joins the sums while the tensor core works on this one; then they move to
-        // the larger of the two references
-        if (k > 0) add_product(j - 1);
+        // the sums move to the larger of the two references
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
           const float top = fmaxf(m[r], mt[r]);
@@ -737,12 +736,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           m[r] = top;
           l[r] = fmaf(lt[r], to, l[r] * old);
           acc[r] *= old;
-          now[r] = to * (1.0f / kProbScale);
+          now[r] = to;
         }
       }
-      if (!alive) break;
-
-      add_product(j - 1);
+      if (ok) add_product(j - 1);
+      if (!ok) break;
       // the row sums over the 128 tokens' threads
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
@@ -753,9 +751,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int r = 0; r < RP; r += 4)
           *reinterpret_cast<float4*>(&sh.sum[quarter][r]) = make_float4(l[r], l[r + 1], l[r + 2], l[r + 3]);
+        mbar_arrive(smem_u32(&sh.sum_full));
       }
-      alive = all_of_group(ok);
-      if (!alive) break;
+      ok = mbar_wait_nocall(smem_u32(&sh.sum_full), item & 1, ctx, ST_KV_SUM, item);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       const int row0 = c.at.row_tile * RP;
       const bool direct = c.at.tile == 0 && n == to_end;
       const int part = (2 * blockIdx.x + (first_part ? 0 : 1)) * RP;
@@ -795,13 +795,14 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // Joins the parts of the items that were cut, in token order.  An item is found by the first
-// boundary between two shares inside it; thread i looks at boundary i + 1.  A row of an item is
+// boundary between two shares inside it; a thread looks at a boundary.  A row of an item is
 // one warp's work, or one block's where there are too few rows to fill the chip (then the items
 // have many parts).
 template <typename T, int D, int RP>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParams p) {
   constexpr int kWarps = kJoinThreads / 32, kCols = D / 32;     // columns per lane
-  __shared__ short found[kMaxShares];      // boundaries that are the first inside their item
+  __shared__ Place places[kMaxShares];     // of the boundaries that are the first inside their item
+  __shared__ short found[kMaxShares];      // which boundaries those are
   __shared__ int in_warps[kWarps];
   __shared__ float column[kWarps][D], weight[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -809,20 +810,26 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
   const int share = list.share_start(p, 1);            // all but the last are as long as the first
   int count = 0;
   if (!list.whole_items()) {
-    const int flat = (int)min((tid + 1ll) * share, (long long)list.tiles() - 1);
-    const Place w = list.locate(p, flat);
-    const bool mine = tid < p.shares - 1 && flat == (tid + 1ll) * share && w.tile > 0 && (flat - w.tile) / share == tid;
     // in the order of the boundaries, so that every block has the same list
-    const uint32_t in_warp = __ballot_sync(0xffffffffu, mine);
-    if (lane == 0) in_warps[warp] = __popc(in_warp);
-    __syncthreads();
-    int index = __popc(in_warp & ((1u << lane) - 1));
-    for (int i = 0; i < kWarps; ++i) {
-      if (i < warp) index += in_warps[i];
-      count += in_warps[i];
+    for (int c0 = 0; c0 < p.shares - 1; c0 += kJoinThreads) {
+      const int c = c0 + tid;
+      const int flat = (int)min((c + 1ll) * share, (long long)list.tiles() - 1);
+      const Place w = list.locate(p, flat);
+      const bool mine = c < p.shares - 1 && flat == (c + 1ll) * share && w.tile > 0 && (flat - w.tile) / share == c;
+      const uint32_t in_warp = __ballot_sync(0xffffffffu, mine);
+      if (lane == 0) in_warps[warp] = __popc(in_warp);
+      __syncthreads();
+      int index = count + __popc(in_warp & ((1u << lane) - 1));
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) index += in_warps[i];
+        count += in_warps[i];
+      }
+      if (mine) {
+        places[index] = w;
+        found[index] = (short)c;
+      }
+      __syncthreads();
     }
-    if (mine) found[index] = tid;
-    __syncthreads();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int units = count * RP;
@@ -831,7 +838,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
   for (int u = by_block ? blockIdx.x : blockIdx.x * kWarps + warp; u < units;
        u += by_block ? gridDim.x : gridDim.x * kWarps) {
     const int r = u % RP, first = found[u / RP];
-    const Place at = list.locate(p, (first + 1) * share);
+    const Place at = places[u / RP];
     const int begin = (first + 1) * share - at.tile;
     const int end = begin + make_seq(p, __ldg(p.lengths + at.b)).count;
     const int skip = begin != first * share;           // the item is its first share's second part
