@@ -42,9 +42,11 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kHalf = 128;               // tokens of one product: a thread's and a tensor-memory lane's
+constexpr int kHalf = 128;               // tokens of one product: tensor-memory lanes
+constexpr int kTile = 256;               // tokens of a step: a thread's each
+constexpr int kTileShift = 8;
 constexpr int kSmemPerCta = 106 * 1024;
-constexpr int kThreads = 192;            // producer, issuer, four softmax warps
+constexpr int kThreads = 320;            // producer, issuer, eight softmax warps
 constexpr int kSoftmaxWarp = 2;
 constexpr int kJoinThreads = 256;
 constexpr int kMinShare = 1;             // tiles
@@ -71,7 +73,7 @@ struct KvAttnParams {
   int64_t table_stride, k_scale_stride, v_scale_stride;
   int batch, nq, kv_heads, group;        // group: query heads per key head
   int rows, row_tiles;                   // nq * group, and how many pieces of RP rows
-  int pages, page, page_shift, tile_shift, max_pages, window, sinks;
+  int pages, page, page_shift, max_pages, window, sinks;
   int shares, q_aligned;
   float scale;
   unsigned long long wait_limit_ns;
@@ -91,7 +93,7 @@ __device__ __forceinline__ Seq make_seq(const KvAttnParams& p, int len) {
   s.limit = min(len, p.max_pages << p.page_shift);
   s.low = p.window ? max(max(len, p.nq) - p.nq + 1 - p.window, 0) : 0;   // of the first query there is
   s.sink_end = min(p.sinks, s.limit);
-  const int shift = p.tile_shift, round = (1 << shift) - 1;
+  const int shift = kTileShift, round = (1 << shift) - 1;
   const int tiles = (s.limit + round) >> shift;
   s.first = s.from = 0;
   s.count = tiles;
@@ -107,7 +109,7 @@ __device__ __forceinline__ Seq make_seq(const KvAttnParams& p, int len) {
   return s;
 }
 __device__ __forceinline__ int tile_start(const KvAttnParams& p, const Seq& s, int t) {
-  return (t < s.first ? t : t - s.first + s.from) << p.tile_shift;
+  return (t < s.first ? t : t - s.first + s.from) << kTileShift;
 }
 // Does any query of the call see this token, as far as positions go?
 __device__ __forceinline__ bool seen_by_any(const Seq& s, int token) {
@@ -131,6 +133,7 @@ struct WorkList {
     per_seq = p.row_tiles * p.kv_heads;
     stretch = (p.batch + 31) / 32;
     sum = largest = 0;
+#pragma unroll 1
     for (int i = 0; i < stretch; ++i) {
       const int b = lane * stretch + i;
       if (b < p.batch) {
@@ -166,6 +169,7 @@ struct WorkList {
     if (i >= items) return tiles();
     const int b = i / per_seq, owner = b / stretch;
     int at = __shfl_sync(0xffffffffu, before, owner);
+#pragma unroll 1
     for (int k = owner * stretch; k < b; ++k) at += make_seq(p, __ldg(p.lengths + k)).count;
     return at * per_seq + (i - b * per_seq) * make_seq(p, __ldg(p.lengths + b)).count;
   }
@@ -180,6 +184,7 @@ struct WorkList {
     int at = __shfl_sync(0xffffffffu, before, owner);
     int b = owner * stretch;
     int count = make_seq(p, __ldg(p.lengths + b)).count;
+#pragma unroll 1
     while (q >= at + count) {
       at += count;
       ++b;
@@ -215,6 +220,7 @@ struct Cursor {
   __device__ void advance(const KvAttnParams& p, int tiles) {
     left -= tiles;
     at.tile += tiles;
+#pragma unroll 1
     while (left > 0 && at.tile >= seq.count) {
       at.tile -= seq.count;
       next_item(p);
@@ -222,41 +228,36 @@ struct Cursor {
   }
 };
 
-// Tiles of 256 tokens, two per thread, halve what a tile costs besides its data (the exchange of
-// maxima, the joining of a product); 16 rows have registers for one.
-template <int RP>
-struct Halves {
-  static constexpr int kCount = RP <= 8 ? 2 : 1;
-};
-
 template <int D, int RP, int PARTS>
 struct Shape {
   static constexpr int kN = (RP * PARTS + 15) / 16 * 16;
-  static constexpr int kH = Halves<RP>::kCount;
   static constexpr int kSlotBytes = kHalf * D;                    // 128 tokens of K or of V
   static constexpr int kQBytes = kN * D;
   static constexpr int kPBytes = kN * kHalf;
   // ring of a tile's K halves, its V halves, the next tile's ...: what two CTAs per SM, and the
   // joining kernel beside them, leave room for
-  static constexpr int kRoom = (kSmemPerCta - 4096 - 2 * kH * kPBytes - 2 * kQBytes) / kSlotBytes;
+  static constexpr int kRoom = (kSmemPerCta - 5120 - 2 * kPBytes - 2 * kQBytes) / kSlotBytes;
   static constexpr int kSlots = kRoom < 12 ? kRoom : 12;
-  static constexpr int kTmemO = 2 * kH * kN;                      // behind the scores of two tiles
-  static constexpr int kTmemCols = kTmemO + 2 * kN <= 64 ? 64 : kTmemO + 2 * kN <= 128 ? 128 : 256;
+  static constexpr int kTmemO = 4 * kN;                           // behind the scores of two tiles
+  static constexpr int kTmemCols = 5 * kN <= 128 ? 128 : 256;
 };
 
 template <int D, int RP, int PARTS>
 struct Shared {
   using S = Shape<D, RP, PARTS>;
   uint8_t ring[S::kSlots][S::kSlotBytes];      // first: the swizzle counts from 1024-byte boundaries
-  uint8_t p[2][S::kH][S::kPBytes];
+  uint8_t p[2][S::kPBytes];                    // of a tile's halves
   uint8_t q[2][S::kQBytes];
   float4 scale[4][32];                         // of a step's pages: ks, log2 vs, 1 / vs, 1 if it is there
   float q_factor[2][RP];                       // what takes a row's product to log2 units
   int q_at[2][RP];                             // position of the row's query; -1: no such row
-  float most[2][4][RP];                        // the warps' maxima, alternating by tile
-  float sum[4][RP];
+  // where its output is in its sequence and head; -1: no such row.  Three turns: an item's are read
+  // while the one after the next is staged.
+  int64_t q_out[3][RP];
+  float most[2][8][RP];                        // the warps' maxima, alternating by tile
+  float sum[2][8][RP];                         // the warps' row sums, alternating by item
   uint64_t full[S::kSlots], empty[S::kSlots], scale_full[4];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], most_full[2], sum_full;
+  uint64_t q_full[2], s_full[2], most_full[2], p_full, o_full, sum_full;
   uint32_t tmem_slot, abort_flag;
 };
 
@@ -279,85 +280,88 @@ __device__ __forceinline__ uint32_t split2(__half2& h) {
 }
 
 // Queries of one item on their way from global memory to their e4m3 parts: 8 columns of a row per
-// vector, kVectors per thread.
+// softmax thread, as many threads as that takes.
 template <typename T, int D, int RP, int PARTS>
 struct Queries {
   static constexpr int kPerRow = D / 8;
-  static constexpr int kVectors = RP * kPerRow / 128 > 0 ? RP * kPerRow / 128 : 1;
-  Vec<T> raw[kVectors];
+  static_assert(RP * kPerRow <= 256, "a vector per thread");
+  Vec<T> raw;
+  int64_t offset;                  // of the row and column; -1: no such row
+  int row_tile = -1;               // that the offset is for
 
   __device__ void load(const KvAttnParams& p, const Cursor& c, int tid) {
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int v = i * 128 + tid;
-      const int r = c.at.row_tile * RP + v / kPerRow;
-      raw[i].raw = make_uint4(0, 0, 0, 0);
-      if (v / kPerRow >= RP || r >= p.rows) continue;
-      const T* src = static_cast<const T*>(p.q) + c.at.b * p.q_batch_stride +
-                     r / p.group * p.q_token_stride +
-                     (c.at.head * p.group + r % p.group) * p.q_head_stride + v % kPerRow * 8;
-      if (p.q_aligned) {
-        raw[i].raw = __ldg(reinterpret_cast<const uint4*>(src));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) raw[i].e[j] = src[j];
-      }
+    if (row_tile != c.at.row_tile) {
+      row_tile = c.at.row_tile;
+      const int r = row_tile * RP + tid / kPerRow;
+      offset = tid / kPerRow < RP && r < p.rows
+                   ? r / p.group * p.q_token_stride + r % p.group * p.q_head_stride + tid % kPerRow * 8
+                   : -1;
     }
-  }
-
-  // Row r times 2^-e fits e4m3's range; 2^e goes into the row's factor.  Parts of row r are rows r,
-  // RP + r, ... of the operand, K-major under the swizzle of its row length.
-  __device__ void stage(const KvAttnParams& p, const Cursor& c, int tid, uint8_t* q, float* factor, int* at) {
+    raw.raw = make_uint4(0, 0, 0, 0);
+    if (offset < 0) return;
+    const T* src = static_cast<const T*>(p.q) + c.at.b * p.q_batch_stride +
+                   (int64_t)c.at.head * p.group * p.q_head_stride + offset;
+    if (p.q_aligned) {
+      raw.raw = __ldg(reinterpret_cast<const uint4*>(src));
+    } else {
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int v = i * 128 + tid;
-      const int r = v / kPerRow, col8 = v % kPerRow;
-      float f[8], most = 0.0f;
-      bool bad = false;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        f[j] = Elem<T>::to_f32(raw[i].e[j]);
-        most = fmaxf(most, fabsf(f[j]));
-        bad |= !(fabsf(f[j]) < INFINITY);
-      }
-#pragma unroll
-      for (int o = kPerRow / 2; o > 0; o >>= 1) {
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
-      }
-      // most <= 448 * 2^e: 448 = 1.75 * 2^8
-      const uint32_t bits = __float_as_uint(most);
-      int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-      e = max(e, -100);
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (r < RP) {
-        if (col8 == 0) {
-          const int row = c.at.row_tile * RP + r;
-          factor[r] = bad ? NAN : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale * kLog2e);
-          at[r] = row < p.rows ? c.seq.len - p.nq + row / p.group : -1;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= down;
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          const uint32_t w0 = split2(f[0], f[1]), w1 = split2(f[2], f[3]);
-          const uint32_t w2 = split2(f[4], f[5]), w3 = split2(f[6], f[7]);
-          const int n = part * RP + r;
-          const int chunk = (col8 >> 1) ^ (D == 128 ? (n & 7) : ((n >> 1) & 3));
-          *reinterpret_cast<uint2*>(q + n * D + chunk * 16 + (col8 & 1) * 8) =
-              make_uint2(w0 | (w1 << 16), w2 | (w3 << 16));
-        }
-      }
+      for (int j = 0; j < 8; ++j) raw.e[j] = src[j];
     }
   }
 };
 
+// Row r times 2^-e fits e4m3's range; 2^e goes into the row's factor.  Parts of row r are rows r,
+// RP + r, ... of the operand, K-major under the swizzle of its row length.  Out of line: it runs once
+// an item, and the tiles' loop has to fit the instruction cache.
+template <typename T, int D, int RP, int PARTS>
+__device__ __noinline__ void stage_queries(const KvAttnParams& p, Vec<T> raw, int first_at, int row_tile, int tid,
+                                           uint8_t* q, float* factor, int* at, int64_t* out) {
+  constexpr int kPerRow = D / 8;
+  const int r = tid / kPerRow, col8 = tid % kPerRow;
+  float f[8], most = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f[j] = Elem<T>::to_f32(raw.e[j]);
+    most = fmaxf(most, fabsf(f[j]));
+    bad |= !(fabsf(f[j]) < INFINITY);
+  }
+#pragma unroll
+  for (int o = kPerRow / 2; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
+  }
+  if (r >= RP) return;
+  // most <= 448 * 2^e: 448 = 1.75 * 2^8
+  const uint32_t bits = __float_as_uint(most);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = max(e, -100);
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+  if (col8 == 0) {
+    const int row = row_tile * RP + r;
+    const bool is = row < p.rows;
+    factor[r] = bad ? NAN : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale * kLog2e);
+    at[r] = is ? first_at + row / p.group : -1;
+    out[r] = is ? row / p.group * p.o_token_stride + row % p.group * p.o_head_stride : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] *= down;
+#pragma unroll
+  for (int part = 0; part < PARTS; ++part) {
+    const uint32_t w0 = split2(f[0], f[1]), w1 = split2(f[2], f[3]);
+    const uint32_t w2 = split2(f[4], f[5]), w3 = split2(f[6], f[7]);
+    const int n = part * RP + r;
+    const int chunk = (col8 >> 1) ^ (D == 128 ? (n & 7) : ((n >> 1) & 3));
+    *reinterpret_cast<uint2*>(q + n * D + chunk * 16 + (col8 & 1) * 8) = make_uint2(w0 | (w1 << 16), w2 | (w3 << 16));
+  }
+}
+
 template <typename T, int D, int RP, int PARTS>
 __global__ void __launch_bounds__(kThreads, 2)
     kv_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                   const KvAttnParams p) {
+                   const __grid_constant__ KvAttnParams p) {
   using S = Shape<D, RP, PARTS>;
-  constexpr int N = S::kN, SLOTS = S::kSlots, H = S::kH;
+  constexpr int N = S::kN, SLOTS = S::kSlots, H = 2;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Shared<D, RP, PARTS>& sh = *reinterpret_cast<Shared<D, RP, PARTS>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -372,13 +376,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     for (int x = 0; x < 4; ++x) mbar_init(smem_u32(&sh.scale_full[x]), 1);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(smem_u32(&sh.q_full[x]), 4);   // one arrival per softmax warp
+      mbar_init(smem_u32(&sh.q_full[x]), 8);   // one arrival per softmax warp
       mbar_init(smem_u32(&sh.s_full[x]), 1);
-      mbar_init(smem_u32(&sh.p_full[x]), 4);
-      mbar_init(smem_u32(&sh.o_full[x]), 1);
-      mbar_init(smem_u32(&sh.most_full[x]), 4);
+      mbar_init(smem_u32(&sh.most_full[x]), 8);
     }
-    mbar_init(smem_u32(&sh.sum_full), 4);
+    mbar_init(smem_u32(&sh.p_full), 8);
+    mbar_init(smem_u32(&sh.o_full), 1);
+    mbar_init(smem_u32(&sh.sum_full), 8);
     mbar_init_fence();
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
@@ -437,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       id[2] = page_of(mine);
       head[2] = mine.at.head;
       bool handed = false;
+#pragma unroll 1
       for (int k = 0; k < step_tiles && left > 0 && ok; ++k, --left) {
         const int j = step * step_tiles + k;
 #pragma unroll
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int g = 2 * H * j + i, x = g % SLOTS;
           const bool in_slot = my_tile == k && my_half == i % H && id[0] >= 0;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, in_slot)) * page_bytes;
-          ok = ok && mbar_wait_nocall(smem_u32(&sh.empty[x]), ((g / SLOTS) & 1) ^ 1, ctx, ST_KV_EMPTY, g);
+          ok = ok && mbar_wait(smem_u32(&sh.empty[x]), ((g / SLOTS) & 1) ^ 1, ctx, ST_KV_EMPTY, g);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const uint32_t bar = smem_u32(&sh.full[x]);
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     constexpr uint64_t kVDesc = D == 128 ? smem_desc_sw128(16, 1024) : smem_desc_sw64(0, 512);
     constexpr uint64_t kPDesc = smem_desc_plain(128, kHalf * 16);
     auto wait_all = [&](uint64_t* bar, uint32_t parity, unsigned int code, int detail) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait_nocall(smem_u32(bar), parity, ctx, code, detail));
+      return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, ctx, code, detail));
     };
     bool ok = true;
     int item = 0;                    // items begun
@@ -505,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
     };
     if (c.left > 0) begin(0, true);
+#pragma unroll 1
     for (int j = 0; c.left > 0 && ok; ++j) {
       const bool ends = c.last_tile();
       c.advance(p, 1);
@@ -512,236 +518,273 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (ends) ++item;
         begin(j + 1, ends);
       }
-      ok = ok && wait_all(&sh.p_full[j & 1], (j >> 1) & 1, ST_KV_P, j);
+      ok = ok && wait_all(&sh.p_full, j & 1, ST_KV_P, j);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const int g = 2 * H * j + H + h, x = g % SLOTS;
         ok = ok && wait_all(&sh.full[x], (g / SLOTS) & 1, ST_KV_V, j);
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t vb = smem_u32(sh.ring[x]), pb = smem_u32(sh.p[j & 1][h]);
+        const uint32_t vb = smem_u32(sh.ring[x]), pb = smem_u32(sh.p[h]);
 #pragma unroll
         for (int kk = 0; kk < kHalf / 32; ++kk)    // 32 tokens: four groups of eight rows
           if (elected)
-            mma_f8_ss(tmem + S::kTmemO + (j & 1) * N, with_address(kVDesc, vb + kk * 32 * D),
+            mma_f8_ss(tmem + S::kTmemO, with_address(kVDesc, vb + kk * 32 * D),
                       with_address(kPDesc, pb + kk * 4 * 128), kIdescPv, h != 0 || kk != 0);
         if (elected) mma_commit(smem_u32(&sh.empty[x]));
       }
       if (!ok) break;
-      if (elected) mma_commit(smem_u32(&sh.o_full[j & 1]));
+      if (elected) mma_commit(smem_u32(&sh.o_full));
       __syncwarp();
     }
   } else {
-    // ---- softmax and sums: a token of the tile, then a column of the head ----
+    // ---- softmax and sums: a token of the tile, then a column of the head and half of the rows ----
+    constexpr int RH = RP / 2;
     const int quarter = warp & 3;                 // the tensor-memory lanes this warp may touch
-    const int me = quarter * 32 + lane;
+    const int half = (warp - kSoftmaxWarp) >> 2;  // of the tile's tokens, later of the rows
+    const int me = quarter * 32 + lane, tid = half * 128 + me;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int step_shift = p.page_shift - 3;      // 32 pages are 2^step_shift tiles
     bool ok = true;
 
     Queries<T, D, RP, PARTS> queries;
-    if (c.left > 0) {
-      queries.load(p, c, me);
-      queries.stage(p, c, me, sh.q[0], sh.q_factor[0], sh.q_at[0]);
+    auto stage = [&](const Cursor& at, int of) {
+      stage_queries<T, D, RP, PARTS>(p, queries.raw, at.seq.len - p.nq, at.at.row_tile, tid, sh.q[of & 1],
+                                     sh.q_factor[of & 1], sh.q_at[of & 1], sh.q_out[of % 3]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[0]));
-      named_barrier_sync(1, 128);    // the rows' factors and positions are written
+      if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[of & 1]));
+    };
+    if (c.left > 0) {
+      queries.load(p, c, tid);
+      stage(c, 0);
+      named_barrier_sync(1, 256);    // the rows' factors and positions are written
     }
 
-    int item = 0;
-    bool first_part = true;                        // the item that the share begins with
-    float acc[RP], l[RP], m[RP], now[RP];          // m: log2 units
+    // An item is finished behind the first maxima of the next one, where its last product has long
+    // been there and so have the other warps' row sums.
+    T* last_out = nullptr;
+    int last_part = 0;
+    bool last_direct = false;
+    float acc[RH], now[RH];          // of this half's rows and this thread's column
+    float l[RP], m[RP];              // of this thread's tokens; the rows' references, log2 units
 #pragma unroll
     for (int r = 0; r < RP; ++r) {
-      acc[r] = l[r] = now[r] = 0.0f;
+      l[r] = 0.0f;
       m[r] = -INFINITY;
     }
-    // the product of tile j joins the sums with the factors that its own step left in `now`
-    auto add_product = [&](int j) {
-      ok = ok && mbar_wait_nocall(smem_u32(&sh.o_full[j & 1]), (j >> 1) & 1, ctx, ST_KV_O, j);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      tc_fence_after_sync();
-      uint32_t raw[N];
 #pragma unroll
-      for (int n = 0; n < N; n += 16)
-        tmem_ld_32x32(tmem + lane_base + S::kTmemO + (j & 1) * N + n, *reinterpret_cast<uint32_t (*)[16]>(&raw[n]));
-      tmem_ld_wait(raw);
-#pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
-#pragma unroll
-        for (int part = PARTS - 2; part >= 0; --part)
-          v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
-        acc[r] = fmaf(v, now[r], acc[r]);
-      }
-    };
-    const int step_shift = p.page_shift - 2 - (H - 1);       // 32 pages are 2^step_shift tiles
-    for (int j = 0; c.left > 0 && ok; ++item) {
-      // one item, as much of it as the share has
-      const int to_end = c.seq.count - c.at.tile;
-      const int n = min(to_end, c.left);
+    for (int i = 0; i < RH; ++i) acc[i] = now[i] = 0.0f;
+    auto mine = [&](const float (&v)[RP], int i) { return half ? v[RH + i] : v[i]; };
+
+    for (int item = 0, j = 0; ok; ++item) {
+      // one item, as much of it as the share has; or none any more, and the last one's end
+      const bool more = c.left > 0;
+      if (!more && item == 0) break;
+      const int to_end = more ? c.seq.count - c.at.tile : 0;
+      const int n = more ? min(to_end, c.left) : 1;
       // the next item's queries are loaded now and staged behind this one's first tile
-      const bool stage_next = c.left > to_end;
+      const bool stage_next = more && c.left > to_end;
       Cursor next = c;
       if (stage_next) {
         next.advance(p, to_end);
-        queries.load(p, next, me);
+        queries.load(p, next, tid);
       }
-      float factor[RP];
-#pragma unroll
-      for (int r = 0; r < RP; ++r) factor[r] = sh.q_factor[item & 1][r];
-
-      for (int k = 0; k < n && ok; ++k, ++j) {
+#pragma unroll 1
+      for (int k = 0; k < n && ok; ++k) {
         const int x = j & 1;
-        const int t0 = tile_start(p, c.seq, c.at.tile + k);
-        constexpr int kTokens = kHalf * H;
-        // every query sees the whole tile: no masks but whether the page is there
-        const bool clean = t0 + kTokens <= c.seq.limit && t0 + kTokens - 1 <= c.seq.len - p.nq &&
-                           (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTokens <= p.sinks);
-        const int step = j >> step_shift;
-        ok = mbar_wait_nocall(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j) &&
-             mbar_wait_nocall(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        float s[H][RP], inv_vs[H];
-        bool there[H];
-        {
+        const int t0 = tile_start(p, c.seq, c.at.tile + k), token = t0 + tid;
+        float s[RP], inv_vs = 0.0f;
+        bool there = true;
+        if (more) {
+          const int step = j >> step_shift;
+          ok = mbar_wait(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j) &&
+               mbar_wait(smem_u32(&sh.s_full[x]), (j >> 1) & 1, ctx, ST_KV_S, j);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after_sync();
-          uint32_t raw[H][N];
+          uint32_t raw[N];
 #pragma unroll
-          for (int h = 0; h < H; ++h)
+          for (int i = 0; i < N; i += 16)
+            tmem_ld_32x32(tmem + lane_base + (x * H + half) * N + i, *reinterpret_cast<uint32_t (*)[16]>(&raw[i]));
+          // every query sees the whole tile: no masks but whether the page is there
+          const bool clean = t0 + kTile <= c.seq.limit && t0 + kTile - 1 <= c.seq.len - p.nq &&
+                             (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTile <= p.sinks);
+          const float4 scale = sh.scale[step & 3][((j << (8 - p.page_shift)) + (tid >> p.page_shift)) & 31];
+          inv_vs = scale.z;
+          // seen by some query, and its page is there
+          there = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
+          float factor[RP];
 #pragma unroll
-            for (int i = 0; i < N; i += 16)
-              tmem_ld_32x32(tmem + lane_base + (x * H + h) * N + i, *reinterpret_cast<uint32_t (*)[16]>(&raw[h][i]));
-          tmem_ld_wait(raw[0]);
-          if constexpr (H == 2) tmem_ld_wait(raw[H - 1]);
+          for (int r = 0; r < RP; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&sh.q_factor[item & 1][r]);
+            factor[r] = f.x;
+            factor[r + 1] = f.y;
+            factor[r + 2] = f.z;
+            factor[r + 3] = f.w;
+          }
+          tmem_ld_wait(raw);
 #pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const int token = t0 + h * kHalf + me;
-            const int entry = (((j * H + h) << (7 - p.page_shift)) + (me >> p.page_shift)) & 31;
-            const float4 scale = sh.scale[step & 3][entry];
-            inv_vs[h] = scale.z;
-            // seen by some query, and its page is there
-            there[h] = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
+          for (int r = 0; r < RP; ++r) {
+            float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
+#pragma unroll
+            for (int part = PARTS - 2; part >= 0; --part)
+              v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
+            // a row that only pads has a product of zero and is as good as any: nobody reads it
+            s[r] = fmaf(v, factor[r] * scale.x, scale.y);
+          }
+          if (!there) {
+#pragma unroll
+            for (int r = 0; r < RP; ++r) s[r] = -INFINITY;
+          }
+          if (!clean) {                          // tokens that some rows do not see
+            const int* at = sh.q_at[item & 1];
 #pragma unroll
             for (int r = 0; r < RP; ++r) {
-              float v = __uint_as_float(raw[h][(PARTS - 1) * RP + r]);
-#pragma unroll
-              for (int part = PARTS - 2; part >= 0; --part)
-                v = fmaf(v, 0.0625f, __uint_as_float(raw[h][part * RP + r]));
-              // a row that only pads has a product of zero and is as good as any: nobody reads it
-              s[h][r] = fmaf(v, factor[r] * scale.x, scale.y);
-            }
-            if (!there[h]) {
-#pragma unroll
-              for (int r = 0; r < RP; ++r) s[h][r] = -INFINITY;
-            }
-            if (!clean) {                          // tokens that some rows do not see
-              const int* at = sh.q_at[item & 1];
-#pragma unroll
-              for (int r = 0; r < RP; ++r) {
-                const bool seen = token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks);
-                if (!seen) s[h][r] = -INFINITY;
-              }
+              const bool seen = token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks);
+              if (!seen) s[r] = -INFINITY;
             }
           }
           float w[RP];
 #pragma unroll
-          for (int r = 0; r < RP; ++r) w[r] = warp_max(H == 2 ? fmaxf(s[0][r], s[H - 1][r]) : s[0][r]);
+          for (int r = 0; r < RP; ++r) w[r] = warp_max(s[r]);
           if (lane == 0) {
 #pragma unroll
             for (int r = 0; r < RP; r += 4)
-              *reinterpret_cast<float4*>(&sh.most[x][quarter][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
+              *reinterpret_cast<float4*>(&sh.most[x][warp - kSoftmaxWarp][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
             mbar_arrive(smem_u32(&sh.most_full[x]));
           }
         }
-        // the tile before joins the sums while the warps' maxima get together
-        if (k > 0) add_product(j - 1);
-        ok = ok && mbar_wait_nocall(smem_u32(&sh.most_full[x]), (j >> 1) & 1, ctx, ST_KV_MOST, j);
+        // while the warps' maxima get together, the product of the tile before joins the sums with
+        // the factors that its own step left in `now`
+        if (k + item > 0) {
+          ok = mbar_wait(smem_u32(&sh.o_full), (j - 1) & 1, ctx, ST_KV_O, j);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after_sync();
+          uint32_t raw[PARTS][RH];
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            tmem_ld_few(tmem + lane_base + S::kTmemO + part * RP + half * RH, raw[part]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) keep_behind(raw[part]);
+#pragma unroll
+          for (int i = 0; i < RH; ++i) {
+            float v = __uint_as_float(raw[PARTS - 1][i]);
+#pragma unroll
+            for (int part = PARTS - 2; part >= 0; --part) v = fmaf(v, 0.0625f, __uint_as_float(raw[part][i]));
+            acc[i] = fmaf(v, now[i], acc[i]);
+          }
+          if (k == 0) {                          // of the item before: its end
+            const int of = item - 1;
+            ok = mbar_wait(smem_u32(&sh.sum_full), of & 1, ctx, ST_KV_SUM, of);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < RH; ++i) {
+              const int r = half * RH + i;
+              float sum = 0.0f;
+#pragma unroll
+              for (int w = 0; w < 8; ++w) sum += sh.sum[of & 1][w][r];
+              if (last_direct) {
+                const int64_t at = sh.q_out[of % 3][r];
+                if (me < D && at >= 0)
+                  last_out[at] = Elem<T>::from_f32(sum > 0.0f ? __fdividef(acc[i], sum) : acc[i] * 0.0f);   // nothing seen: 0
+              } else {
+                if (me < D) p.parts[(last_part + r) * D + me] = acc[i];
+                if (me == 0) p.marks[last_part + r] = make_float2(mine(m, i), sum);
+              }
+              acc[i] = 0.0f;
+            }
+#pragma unroll
+            for (int r = 0; r < RP; ++r) {
+              l[r] = 0.0f;
+              m[r] = -INFINITY;
+            }
+          }
+        }
+        if (!more) break;
+        ok = mbar_wait(smem_u32(&sh.most_full[x]), (j >> 1) & 1, ctx, ST_KV_MOST, j);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         float mt[RP];      // the reference the tile's probabilities are relative to
 #pragma unroll
         for (int r = 0; r < RP; r += 4) {
-          float4 w[4];
+          float4 w[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
-          mt[r] = fmaxf(max3(w[0].x, w[1].x, w[2].x), w[3].x) - kProbLog2;
-          mt[r + 1] = fmaxf(max3(w[0].y, w[1].y, w[2].y), w[3].y) - kProbLog2;
-          mt[r + 2] = fmaxf(max3(w[0].z, w[1].z, w[2].z), w[3].z) - kProbLog2;
-          mt[r + 3] = fmaxf(max3(w[0].w, w[1].w, w[2].w), w[3].w) - kProbLog2;
+          for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
+          auto most_of = [&](auto get) {
+            return fmaxf(max3(max3(get(w[0]), get(w[1]), get(w[2])), get(w[3]), get(w[4])), max3(get(w[5]), get(w[6]), get(w[7]))) -
+                   kProbLog2;
+          };
+          mt[r] = most_of([](const float4& v) { return v.x; });
+          mt[r + 1] = most_of([](const float4& v) { return v.y; });
+          mt[r + 2] = most_of([](const float4& v) { return v.z; });
+          mt[r + 3] = most_of([](const float4& v) { return v.w; });
         }
         // probabilities (0 where the row sees nothing of the tile), rounded to fp16, in parts
-        float lt[RP];                              // this thread's part of the tile's row sums
+        uint32_t bytes[PARTS][RP / 4];
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          uint32_t bytes[PARTS][RP / 4];
+        for (int r = 0; r < RP; ++r) s[r] = exp2_approx(s[r] - (mt[r] == -INFINITY ? 0.0f : mt[r]));
 #pragma unroll
-          for (int r = 0; r < RP; r += 2) {
-            float pr[2];
+        for (int r = 0; r < RP; r += 2) {
+          __half2 pair = __floats2half2_rn(s[r], s[r + 1]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              pr[i] = exp2_approx(s[h][r + i] - (mt[r + i] == -INFINITY ? 0.0f : mt[r + i]));
-              lt[r + i] = h == 0 ? pr[i] * inv_vs[0] : fmaf(pr[i], inv_vs[h], lt[r + i]);
-            }
-            __half2 pair = __floats2half2_rn(pr[0], pr[1]);
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-              const uint32_t q = split2(pair);
-              if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
-            }
+          for (int part = 0; part < PARTS; ++part) {
+            const uint32_t q = split2(pair);
+            if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
           }
-          // the token's row of P: N bytes, 16 at a time
+        }
+        // the token's row of P: N bytes, 16 at a time
 #pragma unroll
-          for (int i = 0; i < N; i += 16) {
-            uint32_t w[4];
+        for (int i = 0; i < N; i += 16) {
+          uint32_t w[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const int at = (i + 4 * b) / RP, r = (i + 4 * b) % RP;
-              w[b] = at < PARTS ? bytes[at < PARTS ? at : 0][r / 4] : 0u;
-            }
-            st_shared_v4(smem_u32(sh.p[x][h]) + (i / 16) * (kHalf * 16) + me * 16, w[0], w[1], w[2], w[3]);
+          for (int b = 0; b < 4; ++b) {
+            const int at = (i + 4 * b) / RP, r = (i + 4 * b) % RP;
+            w[b] = at < PARTS ? bytes[at < PARTS ? at : 0][r / 4] : 0u;
           }
-          if (__any_sync(0xffffffffu, !there[h])) {
-            const int g = 2 * H * j + H + h;
-            ok = ok && mbar_wait_nocall(smem_u32(&sh.full[g % SLOTS]), (g / SLOTS) & 1, ctx, ST_KV_ZERO, j);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!there[h]) {
-#pragma unroll
-              for (int i = 0; i < D; i += 16)     // neighbours start at different banks
-                st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + ((i + me * 16) & (D - 1))]), 0, 0, 0, 0);
-            }
+          st_shared_v4(smem_u32(sh.p[half]) + (i / 16) * (kHalf * 16) + me * 16, w[0], w[1], w[2], w[3]);
+        }
+        if (__any_sync(0xffffffffu, !there)) {
+          const int g = 2 * H * j + H + half;
+          ok = mbar_wait(smem_u32(&sh.full[g % SLOTS]), (g / SLOTS) & 1, ctx, ST_KV_ZERO, j);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!there) {
+#pragma unroll 1
+            for (int i = 0; i < D; i += 16)     // neighbours start at different banks
+              st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + ((i + me * 16) & (D - 1))]), 0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[x]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
 
-        if (stage_next && k == 0) {
-          const int y = (item + 1) & 1;
-          queries.stage(p, next, me, sh.q[y], sh.q_factor[y], sh.q_at[y]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[y]));
-        }
+        if (stage_next && k == 0) stage(next, item + 1);
 
         // the sums move to the larger of the two references
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float top = fmaxf(m[r], mt[r]);
-          const float ref = top == -INFINITY ? 0.0f : top;
-          const float old = exp2_approx(m[r] - ref), to = exp2_approx(mt[r] - ref);
-          m[r] = top;
-          l[r] = fmaf(lt[r], to, l[r] * old);
-          acc[r] *= old;
-          now[r] = to;
+        for (int i = 0; i < RH; ++i) {
+          float old[2], to[2];                     // of row i and of its fellow in the other half
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = h * RH + i;
+            const float top = fmaxf(m[r], mt[r]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            old[h] = exp2_approx(m[r] - ref);
+            to[h] = exp2_approx(mt[r] - ref);
+            m[r] = top;
+            l[r] = fmaf(s[r] * inv_vs, to[h], l[r] * old[h]);
+          }
+          acc[i] *= half ? old[1] : old[0];
+          now[i] = half ? to[1] : to[0];
         }
+        ++j;
       }
-      if (ok) add_product(j - 1);
-      if (!ok) break;
-      // the row sums over the 128 tokens' threads
+      if (!ok || !more) break;
+      // the row sums over the tokens' threads, on their way
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
 #pragma unroll
@@ -750,33 +793,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane == 0) {
 #pragma unroll
         for (int r = 0; r < RP; r += 4)
-          *reinterpret_cast<float4*>(&sh.sum[quarter][r]) = make_float4(l[r], l[r + 1], l[r + 2], l[r + 3]);
+          *reinterpret_cast<float4*>(&sh.sum[item & 1][warp - kSoftmaxWarp][r]) = make_float4(l[r], l[r + 1], l[r + 2], l[r + 3]);
         mbar_arrive(smem_u32(&sh.sum_full));
       }
-      ok = mbar_wait_nocall(smem_u32(&sh.sum_full), item & 1, ctx, ST_KV_SUM, item);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const int row0 = c.at.row_tile * RP;
-      const bool direct = c.at.tile == 0 && n == to_end;
-      const int part = (2 * blockIdx.x + (first_part ? 0 : 1)) * RP;
-#pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        const float sum = (sh.sum[0][r] + sh.sum[1][r]) + (sh.sum[2][r] + sh.sum[3][r]);
-        const int row = row0 + r;
-        if (direct) {
-          if (me < D && row < p.rows) {
-            T* dst = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + row / p.group * p.o_token_stride +
-                     (c.at.head * p.group + row % p.group) * p.o_head_stride + me;
-            *dst = Elem<T>::from_f32(sum > 0.0f ? acc[r] / sum : acc[r] * 0.0f);   // nothing seen: 0
-          }
-        } else {
-          if (me < D) p.parts[(part + r) * D + me] = acc[r];
-          if (me == 0) p.marks[part + r] = make_float2(m[r], sum);
-        }
-        acc[r] = l[r] = 0.0f;
-        m[r] = -INFINITY;
-      }
-      first_part = false;
+      last_out = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + (int64_t)c.at.head * p.group * p.o_head_stride + me;
+      last_direct = c.at.tile == 0 && n == to_end;
+      last_part = (2 * blockIdx.x + (item == 0 ? 0 : 1)) * RP;    // the share's first or second part
       c = next;
       if (!stage_next) c.left = 0;
     }
@@ -908,8 +930,8 @@ int launch_kv(KvAttnParams p, const CUtensorMap& mk, const CUtensorMap& mv, cuda
   kern<<<p.shares, kThreads, smem, stream>>>(mk, mv, p);
   if (int rc = cuda_check(cudaGetLastError(), "kv attention launch")) return rc;
   // no sequence of the table can be long enough to be cut
-  const int64_t most = ((int64_t)p.max_pages << p.page_shift) + (1 << p.tile_shift) - 1;
-  if ((most >> p.tile_shift) <= kWholeItems) return 0;
+  const int64_t most = ((int64_t)p.max_pages << p.page_shift) + (1 << kTileShift) - 1;
+  if ((most >> kTileShift) <= kWholeItems) return 0;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)device_info().sm_count);
   config.blockDim = dim3(kJoinThreads);
@@ -1024,7 +1046,6 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   p.max_pages = (int)max_pages;
   p.window = (int)window;
   p.sinks = (int)sinks;
-  p.tile_shift = rp <= 8 ? 8 : 7;
   p.shares = shares_of();
   p.marks = reinterpret_cast<float2*>(p.parts + 2ll * p.shares * rp * cache->head_dim);
   p.q_aligned = at16(q) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;

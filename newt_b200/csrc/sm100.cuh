@@ -333,20 +333,36 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
       tmem_st_32x32(taddr + q * 32, *reinterpret_cast<const uint32_t (*)[32]>(&r[q * 32]));
   }
 }
+// The same for 2, 4 and 8 columns.
+__device__ __forceinline__ void tmem_ld_few(uint32_t taddr, uint32_t (&r)[2]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_few(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_few(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// The same, and the registers the loads were to fill pass through it: whatever is computed from
-// them cannot be moved in front of the wait.
+// Registers that a load was to fill: whatever is computed from them cannot be moved in front of this,
+// which stands behind the wait.
+template <int N>
+__device__ __forceinline__ void keep_behind(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]));
+}
 template <int N>
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
-  static_assert(N % 8 == 0, "eight registers at a time");
   tmem_ld_wait();
-#pragma unroll
-  for (int i = 0; i < N; i += 8)
-    asm volatile(""
-                 : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]),
-                   "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+  keep_behind(r);
 }
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
