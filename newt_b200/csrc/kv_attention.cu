@@ -49,8 +49,7 @@ constexpr int kSmemPerCta = 106 * 1024;
 constexpr int kThreads = 320;            // producer, issuer, eight softmax warps
 constexpr int kSoftmaxWarp = 2;
 constexpr int kJoinThreads = 256;
-constexpr int kMinShare = 1;             // tiles
-constexpr int kWholeItems = 3;           // tiles
+constexpr int kJoinTiles = 3;
 constexpr int kMaxShares = 320;          // two CTAs on each of 148 SMs
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastScale = 8.67361738e-19f;   // 2^-60
@@ -154,16 +153,17 @@ struct WorkList {
   }
   __device__ int tiles() const { return total * per_seq; }
 
-  // Shares of whole items where all are short (a cut would cost more than it evens out: below),
-  // of tiles otherwise.
-  __device__ bool whole_items() const { return largest <= kWholeItems; }
+  // Shares of whole items, or of tiles?  Joining the parts of cut items costs about as much as
+  // kJoinTiles tiles: whole items where the longest share of them is no longer than that.
+  __device__ int tile_share(const KvAttnParams& p) const { return (tiles() + p.shares - 1) / p.shares; }
+  __device__ bool whole_items(const KvAttnParams& p) const {
+    const long long items = (p.batch * per_seq + p.shares - 1) / p.shares;
+    return items * largest <= tile_share(p) + kJoinTiles;
+  }
 
   // first tile of share c, from 0 to tiles(); the same c in all lanes
   __device__ int share_start(const KvAttnParams& p, int c) const {
-    if (!whole_items()) {
-      const int share = max((tiles() + p.shares - 1) / p.shares, kMinShare);
-      return (int)min((long long)c * share, (long long)tiles());
-    }
+    if (!whole_items(p)) return (int)min((long long)c * tile_share(p), (long long)tiles());
     const int items = p.batch * per_seq;
     const int i = (int)((long long)items * c / p.shares);
     if (i >= items) return tiles();
@@ -236,7 +236,7 @@ struct Shape {
   static constexpr int kPBytes = kN * kHalf;
   // ring of a tile's K halves, its V halves, the next tile's ...: what two CTAs per SM, and the
   // joining kernel beside them, leave room for
-  static constexpr int kRoom = (kSmemPerCta - 5120 - 2 * kPBytes - 2 * kQBytes) / kSlotBytes;
+  static constexpr int kRoom = (kSmemPerCta - 3072 - 320 * RP - 2 * kPBytes - 2 * kQBytes) / kSlotBytes;
   static constexpr int kSlots = kRoom < 12 ? kRoom : 12;
   static constexpr int kTmemO = 4 * kN;                           // behind the scores of two tiles
   static constexpr int kTmemCols = 5 * kN <= 128 ? 128 : 256;
@@ -256,6 +256,7 @@ struct Shared {
   int64_t q_out[3][RP];
   float most[2][8][RP];                        // the warps' maxima, alternating by tile
   float sum[2][8][RP];                         // the warps' row sums, alternating by item
+  float4 step[8][RP];                          // a warp's own: a row's reference, what the sums and the tile are scaled by
   uint64_t full[S::kSlots], empty[S::kSlots], scale_full[4];
   uint64_t q_full[2], s_full[2], most_full[2], p_full, o_full, sum_full;
   uint32_t tmem_slot, abort_flag;
@@ -567,15 +568,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     int last_part = 0;
     bool last_direct = false;
     float acc[RH], now[RH];          // of this half's rows and this thread's column
-    float l[RP], m[RP];              // of this thread's tokens; the rows' references, log2 units
+    float l[RP];                     // of this thread's tokens
+    float m = -INFINITY;             // the reference of row lane % RP, log2 units
 #pragma unroll
-    for (int r = 0; r < RP; ++r) {
-      l[r] = 0.0f;
-      m[r] = -INFINITY;
-    }
+    for (int r = 0; r < RP; ++r) l[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < RH; ++i) acc[i] = now[i] = 0.0f;
-    auto mine = [&](const float (&v)[RP], int i) { return half ? v[RH + i] : v[i]; };
 
     for (int item = 0, j = 0; ok; ++item) {
       // one item, as much of it as the share has; or none any more, and the last one's end
@@ -693,40 +691,43 @@ __global__ void __launch_bounds__(kThreads, 2)
                   last_out[at] = Elem<T>::from_f32(sum > 0.0f ? __fdividef(acc[i], sum) : acc[i] * 0.0f);   // nothing seen: 0
               } else {
                 if (me < D) p.parts[(last_part + r) * D + me] = acc[i];
-                if (me == 0) p.marks[last_part + r] = make_float2(mine(m, i), sum);
+                if (quarter == 0 && lane == r) p.marks[last_part + r] = make_float2(m, sum);
               }
               acc[i] = 0.0f;
             }
 #pragma unroll
-            for (int r = 0; r < RP; ++r) {
-              l[r] = 0.0f;
-              m[r] = -INFINITY;
-            }
+            for (int r = 0; r < RP; ++r) l[r] = 0.0f;
+            m = -INFINITY;
           }
         }
         if (!more) break;
         ok = mbar_wait(smem_u32(&sh.most_full[x]), (j >> 1) & 1, ctx, ST_KV_MOST, j);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        float mt[RP];      // the reference the tile's probabilities are relative to
+        // Lane by lane a row each: the reference its probabilities in this tile are relative to, and
+        // what brings the sums so far and the tile to the larger of that and the one before.
+        {
+          const int r = lane % RP;
+          float top = sh.most[x][lane / RP][r];
 #pragma unroll
-        for (int r = 0; r < RP; r += 4) {
-          float4 w[8];
+          for (int i = 32 / RP; i < 8; i += 32 / RP) top = fmaxf(top, sh.most[x][lane / RP + i][r]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const float4*>(&sh.most[x][i][r]);
-          auto most_of = [&](auto get) {
-            return fmaxf(max3(max3(get(w[0]), get(w[1]), get(w[2])), get(w[3]), get(w[4])), max3(get(w[5]), get(w[6]), get(w[7]))) -
-                   kProbLog2;
-          };
-          mt[r] = most_of([](const float4& v) { return v.x; });
-          mt[r + 1] = most_of([](const float4& v) { return v.y; });
-          mt[r + 2] = most_of([](const float4& v) { return v.z; });
-          mt[r + 3] = most_of([](const float4& v) { return v.w; });
+          for (int o = RP; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float mt = top - kProbLog2, both = fmaxf(m, mt), ref = both == -INFINITY ? 0.0f : both;
+          if (lane < RP)
+            sh.step[warp - kSoftmaxWarp][r] = make_float4(mt == -INFINITY ? 0.0f : mt, exp2_approx(m - ref), exp2_approx(mt - ref), 0.0f);
+          m = both;
+          __syncwarp();
         }
+        const float4* row_step = sh.step[warp - kSoftmaxWarp];
         // probabilities (0 where the row sees nothing of the tile), rounded to fp16, in parts
         uint32_t bytes[PARTS][RP / 4];
 #pragma unroll
-        for (int r = 0; r < RP; ++r) s[r] = exp2_approx(s[r] - (mt[r] == -INFINITY ? 0.0f : mt[r]));
+        for (int r = 0; r < RP; ++r) {
+          const float4 f = row_step[r];
+          s[r] = exp2_approx(s[r] - f.x);
+          l[r] = fmaf(s[r] * inv_vs, f.z, l[r] * f.y);
+        }
 #pragma unroll
         for (int r = 0; r < RP; r += 2) {
           __half2 pair = __floats2half2_rn(s[r], s[r + 1]);
@@ -764,23 +765,13 @@ __global__ void __launch_bounds__(kThreads, 2)
 
         if (stage_next && k == 0) stage(next, item + 1);
 
-        // the sums move to the larger of the two references
 #pragma unroll
         for (int i = 0; i < RH; ++i) {
-          float old[2], to[2];                     // of row i and of its fellow in the other half
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = h * RH + i;
-            const float top = fmaxf(m[r], mt[r]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            old[h] = exp2_approx(m[r] - ref);
-            to[h] = exp2_approx(mt[r] - ref);
-            m[r] = top;
-            l[r] = fmaf(s[r] * inv_vs, to[h], l[r] * old[h]);
-          }
-          acc[i] *= half ? old[1] : old[0];
-          now[i] = half ? to[1] : to[0];
+          const float4 f = row_step[half * RH + i];
+          acc[i] *= f.y;
+          now[i] = f.z;
         }
+        __syncwarp();                            // before the next tile's steps are written
         ++j;
       }
       if (!ok || !more) break;
@@ -831,7 +822,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
   const WorkList list(p);
   const int share = list.share_start(p, 1);            // all but the last are as long as the first
   int count = 0;
-  if (!list.whole_items()) {
+  if (!list.whole_items(p)) {
     // in the order of the boundaries, so that every block has the same list
     for (int c0 = 0; c0 < p.shares - 1; c0 += kJoinThreads) {
       const int c = c0 + tid;
@@ -855,7 +846,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int units = count * RP;
-  const bool by_block = units <= 2 * (int)gridDim.x;   // the same everywhere
+  const bool by_block = units <= (int)gridDim.x;       // the same everywhere
   const int step = by_block ? kWarps : 1, mine = by_block ? warp : 0;
   for (int u = by_block ? blockIdx.x : blockIdx.x * kWarps + warp; u < units;
        u += by_block ? gridDim.x : gridDim.x * kWarps) {
@@ -931,9 +922,9 @@ int launch_kv(KvAttnParams p, const CUtensorMap& mk, const CUtensorMap& mv, cuda
   if (int rc = cuda_check(cudaGetLastError(), "kv attention launch")) return rc;
   // no sequence of the table can be long enough to be cut
   const int64_t most = ((int64_t)p.max_pages << p.page_shift) + (1 << kTileShift) - 1;
-  if ((most >> kTileShift) <= kWholeItems) return 0;
+  if ((most >> kTileShift) <= kJoinTiles) return 0;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)device_info().sm_count);
+  config.gridDim = dim3(4u * (unsigned)device_info().sm_count);
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   cudaLaunchAttribute attr;
