@@ -817,7 +817,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
   __shared__ Place places[kMaxShares];     // of the boundaries that are the first inside their item
   __shared__ short found[kMaxShares];      // which boundaries those are
   __shared__ int in_warps[kWarps];
-  __shared__ float column[kWarps][D], weight[kWarps];
+  __shared__ float column[kWarps][D];
+  __shared__ float2 marks[kWarps][kMaxShares];   // a warp's own: its item's parts
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const WorkList list(p);
   const int share = list.share_start(p, 1);            // all but the last are as long as the first
@@ -847,7 +848,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int units = count * RP;
   const bool by_block = units <= (int)gridDim.x;       // the same everywhere
-  const int step = by_block ? kWarps : 1, mine = by_block ? warp : 0;
+  const int team = by_block ? kWarps : 1, mine = by_block ? warp : 0;
   for (int u = by_block ? blockIdx.x : blockIdx.x * kWarps + warp; u < units;
        u += by_block ? gridDim.x : gridDim.x * kWarps) {
     const int r = u % RP, first = found[u / RP];
@@ -860,36 +861,61 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
     const int n = (end - 1) / share - first + 1;
     // part i: the first share's first or second part, the first parts of the shares behind it
     auto part = [&](int i) { return (2 * (first + i) + (i == 0 ? skip : 0)) * RP + r; };
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, p.marks[part(i)].x);
-    m = warp_max(m);
-    float acc[kCols], sum = 0.0f;
+    // the first parts' columns are on their way before any weight is known
+    constexpr int kBatch = 8;
+    float q[kBatch][kCols];
+    auto fetch = [&](int base) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = base + b * team;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) q[b][k] = i < n ? p.parts[part(i) * D + lane + k * 32] : 0.0f;
+      }
+    };
+    fetch(mine);
+    // weights: every warp works out all of them for itself
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+      const float2 mark = p.marks[part(i)];
+      marks[warp][i] = mark;
+      top = fmaxf(top, mark.x);
+    }
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int i = lane; i < n; i += 32) {               // this lane's own
+      const float w = exp2_approx(marks[warp][i].x - ref);
+      sum = fmaf(marks[warp][i].y, w, sum);
+      marks[warp][i].x = w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncwarp();
+    float acc[kCols];
 #pragma unroll
     for (int k = 0; k < kCols; ++k) acc[k] = 0.0f;
-#pragma unroll 4
-    for (int i = mine; i < n; i += step) {
-      const float2 mark = p.marks[part(i)];
-      const float* q = p.parts + part(i) * D + lane;
-      const float w = mark.x == -INFINITY ? 0.0f : exp2_approx(mark.x - m);
+    for (int base = mine; base < n; base += kBatch * team) {
+      if (base != mine) fetch(base);
 #pragma unroll
-      for (int k = 0; k < kCols; ++k) acc[k] = fmaf(q[k * 32], w, acc[k]);
-      sum = fmaf(mark.y, w, sum);
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = base + b * team;
+        const float w = i < n ? marks[warp][i].x : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) acc[k] = fmaf(q[b][k], w, acc[k]);
+      }
     }
+    __syncwarp();                                      // before marks are written again
     if (by_block) {
       __syncthreads();                                 // the row before has been read
 #pragma unroll
       for (int k = 0; k < kCols; ++k) column[warp][k * 32 + lane] = acc[k];
-      if (lane == 0) weight[warp] = sum;
       __syncthreads();
       if (warp != 0) continue;
-      sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kCols; ++k) acc[k] = 0.0f;
+      for (int k = 0; k < kCols; ++k) {
+        acc[k] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-#pragma unroll
-        for (int k = 0; k < kCols; ++k) acc[k] += column[i][k * 32 + lane];
-        sum += weight[i];
+        for (int i = 0; i < kWarps; ++i) acc[k] += column[i][k * 32 + lane];
       }
     }
     T* dst = static_cast<T*>(p.out) + at.b * p.o_batch_stride + row / p.group * p.o_token_stride +
