@@ -352,14 +352,15 @@ int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const void* v, i
  * j > position - window (`window` 0: all) or j < sinks.  A query that sees nothing (a sequence
  * shorter than `queries`, an empty one) gives zeros.  Tokens whose page is missing from the table
  * are not seen.  What lies in page rows that no query of the call sees has no effect, NaN included.
- * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 14 (fp16)
+ * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 11 (fp16)
  * significant bits.
  * `workspace`: 16-byte aligned device memory of at least nb200_kv_attention_workspace_bytes(...)
- * bytes, the caller's; nothing in it needs clearing, and it must not be shared by launches that can
- * overlap on the GPU.  The lengths stay on the device, so a captured call replays with new ones.
+ * bytes (0: none is needed, sequences of so few pages are never cut), the caller's; nothing in it
+ * needs clearing, and it must not be shared by launches that can overlap on the GPU.  The lengths stay on the device, so a captured call replays with new ones.
  * Beside nb200_attention_fwd; the reference has no cache. */
 int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cache, int64_t batch,
-                                           int64_t queries, int64_t heads, int dtype);
+                                           int64_t queries, int64_t heads, int64_t max_pages,
+                                           int dtype);
 int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, void* out, int64_t batch,
                        int64_t queries, int64_t heads, int64_t q_batch_stride,
                        int64_t q_token_stride, int64_t q_head_stride, int64_t o_batch_stride,

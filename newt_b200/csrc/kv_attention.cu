@@ -154,11 +154,12 @@ struct WorkList {
   __device__ int tiles() const { return total * per_seq; }
 
   // Shares of whole items, or of tiles?  Joining the parts of cut items costs about as much as
-  // kJoinTiles tiles: whole items where the longest share of them is no longer than that.
+  // kJoinTiles tiles: whole items where the longest share of them is no longer than that, and always
+  // where every item is that short (the host counts on it: can_be_cut).
   __device__ int tile_share(const KvAttnParams& p) const { return (tiles() + p.shares - 1) / p.shares; }
   __device__ bool whole_items(const KvAttnParams& p) const {
     const long long items = (p.batch * per_seq + p.shares - 1) / p.shares;
-    return items * largest <= tile_share(p) + kJoinTiles;
+    return largest <= kJoinTiles || items * largest <= tile_share(p) + kJoinTiles;
   }
 
   // first tile of share c, from 0 to tiles(); the same c in all lanes
@@ -928,6 +929,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
 
 // ---- host ------------------------------------------------------------------------------------------
 
+// Can a sequence of this many pages be long enough for its items to be cut?
+bool can_be_cut(int64_t pages, int64_t page) { return cdiv64(pages * page, kTile) > kJoinTiles; }
+
 int row_tile_of(int64_t rows) {
   int rp = 4;
   while (rp < rows && rp < 16) rp *= 2;
@@ -946,9 +950,7 @@ int launch_kv(KvAttnParams p, const CUtensorMap& mk, const CUtensorMap& mv, cuda
   if (int rc = prepare_kernel((const void*)kern, smem)) return rc;
   kern<<<p.shares, kThreads, smem, stream>>>(mk, mv, p);
   if (int rc = cuda_check(cudaGetLastError(), "kv attention launch")) return rc;
-  // no sequence of the table can be long enough to be cut
-  const int64_t most = ((int64_t)p.max_pages << p.page_shift) + (1 << kTileShift) - 1;
-  if ((most >> kTileShift) <= kJoinTiles) return 0;
+  if (!can_be_cut(p.max_pages, p.page)) return 0;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(4u * (unsigned)device_info().sm_count);
   config.blockDim = dim3(kJoinThreads);
@@ -988,8 +990,10 @@ int encode_pages(CUtensorMap* map, const void* base, const nb200_kv_cache& c, in
 using namespace nb200;
 
 extern "C" int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cache, int64_t batch,
-                                                      int64_t queries, int64_t heads, int dtype) {
+                                                      int64_t queries, int64_t heads,
+                                                      int64_t max_pages, int dtype) {
   if (!cache || cache->heads <= 0 || batch <= 0 || queries <= 0 || heads <= 0) return 0;
+  if (!can_be_cut(max_pages, cache->page_size)) return 0;
   const int rp = row_tile_of(queries * (heads / cache->heads));
   return 2ll * shares_of() * rp * (cache->head_dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }
@@ -1022,8 +1026,8 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   if (!q || !out || !lengths || (max_pages > 0 && !page_table))
     return fail(NB200_E_INVALID, "kv attention: null tensor pointer");
   if (cache->pages == 0) return fail(NB200_E_INVALID, "kv attention: the cache has no pages");
-  const int64_t need = nb200_kv_attention_workspace_bytes(cache, batch, queries, heads, dtype);
-  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+  const int64_t need = nb200_kv_attention_workspace_bytes(cache, batch, queries, heads, max_pages, dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || !at16(workspace)))
     return fail(NB200_E_INVALID, "kv attention: a 16-byte aligned workspace of %lld bytes is needed (given %lld)",
                 (long long)need, (long long)workspace_bytes);
   const bool bf16 = dtype == NB200_BF16;
@@ -1064,7 +1068,7 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   p.window = (int)window;
   p.sinks = (int)sinks;
   p.shares = shares_of();
-  p.marks = reinterpret_cast<float2*>(p.parts + 2ll * p.shares * rp * cache->head_dim);
+  p.marks = need > 0 ? reinterpret_cast<float2*>(p.parts + 2ll * p.shares * rp * cache->head_dim) : nullptr;
   p.q_aligned = at16(q) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   p.scale = scale;
   p.wait_limit_ns = wait_limit_ns();

@@ -25,6 +25,8 @@ import torch
 from .runtime import abi
 
 E4M3 = torch.float8_e4m3fn
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_HALVES = (torch.bfloat16, torch.float16)
 _CODES = {torch.float32: abi.F32, torch.float16: abi.F16, torch.bfloat16: abi.BF16, E4M3: abi.E4M3}
 
 
@@ -88,33 +90,33 @@ def _launch_stream(names, *tensors):
     raise AssertionError("a tensor changed its device")
 
 
-def _shaped(name, t, shape, dtype=None):
+def _refuse(name, t, shape, dtype):
+    """Says what is wrong with a tensor that is not of this shape and type, rows dense."""
     if t.shape != shape:
         raise ValueError(f"'{name}' has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if dtype is not None and t.dtype is not dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"'{name}' is {t.dtype}, expected {dtype}")
+    raise ValueError(f"'{name}' must have unit stride along its last dimension")
 
 
-def _dense_rows(name, t):
+def _rows(name, t, shape, dtype):
     """Rows may lie anywhere, the elements of a row side by side."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"'{name}' must have unit stride along its last dimension")
+    if t.shape != shape or t.dtype is not dtype or (t.stride(-1) != 1 and shape[-1] > 1):
+        _refuse(name, t, shape, dtype)
 
 
-def _contiguous(name, t):
-    if not t.is_contiguous():
-        raise ValueError(f"'{name}' must be contiguous")
+def _vector(name, t, length, dtype):
+    if t.shape != (length,) or t.dtype is not dtype or not t.is_contiguous():
+        _refuse(name, t, (length,), dtype)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _rows_like(x, dtype):
-    """A fresh contiguous tensor of x's shape."""
-    if x.is_contiguous():
-        return torch.empty_like(x, dtype=dtype)
-    return torch.empty(x.shape, dtype=dtype, device=x.device)
+def _fresh(x, dtype):
+    """A contiguous tensor of x's shape (empty_like is the quicker call, but keeps x's strides)."""
+    return torch.empty_like(x, dtype=dtype) if x.is_contiguous() else x.new_empty(x.shape, dtype=dtype)
 
 
 def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=None, scales=None,
@@ -126,77 +128,73 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
     scale = max|y| / 448 over the row (`group` 0; scales [rows, 1]) or over every `group` of 32, 64
     or 128 columns (scales [rows, ceil(n / group)]).  With a residual, h comes back in x's type.
     `out` and `residual_out` may be x and residual themselves."""
-    if x.dim() != 2:
-        raise ValueError(f"'x' must be [rows, n], got {tuple(x.shape)}")
-    rows, n = x.shape
-    dtype = x.dtype
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 2:
+        raise ValueError(f"'x' must be [rows, n], got {tuple(shape)}")
+    rows, n = shape
+    if dtype not in _FLOATS:
+        raise TypeError(f"rmsnorm: {dtype} (fp32, fp16 or bf16)")
     if out_dtype is None:
         out_dtype = dtype
-    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"rmsnorm: {dtype} (fp32, fp16 or bf16)")
-    if out_dtype not in (dtype, E4M3):
+    elif out_dtype is not E4M3 and out_dtype is not dtype:
         raise TypeError(f"rmsnorm: the output is {dtype} or float8_e4m3fn, not {out_dtype}")
-    _shaped("weight", weight, (n,), dtype)
-    _contiguous("weight", weight)
+    _rows("x", x, shape, dtype)
+    _vector("weight", weight, n, dtype)
     if out is None:
-        out = _rows_like(x, out_dtype)
+        out = _fresh(x, out_dtype)
     else:
-        _shaped("out", out, (rows, n), out_dtype)
-        _dense_rows("out", out)
+        _rows("out", out, shape, out_dtype)
+    scale_stride = residual_stride = residual_out_stride = 0
     if out_dtype is E4M3:
         if group not in (0, 32, 64, 128):
             raise ValueError(f"rmsnorm: group {group} (0: one scale per row; 32, 64, 128 columns)")
         columns = -(-n // group) if group else 1
         if scales is None:
-            scales = torch.empty((rows, columns), dtype=torch.float32, device=x.device)
+            scales = x.new_empty((rows, columns), dtype=torch.float32)
+            scale_stride = columns
         else:
-            _shaped("scales", scales, (rows, columns), torch.float32)
-            _dense_rows("scales", scales)
+            _rows("scales", scales, (rows, columns), torch.float32)
+            scale_stride = scales.stride(0)
     elif group or scales is not None:
         raise ValueError("rmsnorm: scales and groups go with an e4m3 output")
     if residual is not None:
-        _shaped("residual", residual, (rows, n), dtype)
-        _dense_rows("residual", residual)
+        _rows("residual", residual, shape, dtype)
+        residual_stride = residual.stride(0)
         if residual_out is None:
-            residual_out = _rows_like(x, dtype)
+            residual_out = _fresh(x, dtype)
         else:
-            _shaped("residual_out", residual_out, (rows, n), dtype)
-            _dense_rows("residual_out", residual_out)
+            _rows("residual_out", residual_out, shape, dtype)
+        residual_out_stride = residual_out.stride(0)
     elif residual_out is not None:
         raise ValueError("rmsnorm: 'residual_out' goes with a residual")
-    _dense_rows("x", x)
     stream = _launch_stream("x weight residual out scales residual_out", x, weight, residual, out,
                             scales, residual_out)
     abi.check(abi.load().nb200_rmsnorm(
         x.data_ptr(), _ptr(residual), weight.data_ptr(), out.data_ptr(), _ptr(residual_out),
-        _ptr(scales), rows, n, x.stride(0), residual.stride(0) if residual is not None else 0,
-        out.stride(0), residual_out.stride(0) if residual_out is not None else 0,
-        scales.stride(0) if scales is not None else 0, group, eps, _CODES[dtype],
-        _CODES[out_dtype], stream))
+        _ptr(scales), rows, n, x.stride(0), residual_stride, out.stride(0), residual_out_stride,
+        scale_stride, group, eps, _CODES[dtype], _CODES[out_dtype], stream))
     return RmsNorm(out, scales, residual_out)
 
 
 def _pack_cache(cache):
     """nb200_kv_cache of a KVCache, after its shapes and types have been looked at."""
     k, v, ks, vs = cache
-    if k.dim() != 4:
-        raise ValueError(f"'cache.k' must be [pages, heads, page_size, head_dim], got {tuple(k.shape)}")
     shape = k.shape
+    if len(shape) != 4:
+        raise ValueError(f"'cache.k' must be [pages, heads, page_size, head_dim], got {tuple(shape)}")
     pages, heads, page, d = shape
     if v.shape != shape:
         raise ValueError(f"'cache.v' has shape {tuple(v.shape)}, 'cache.k' {tuple(shape)}")
     if k.dtype is not E4M3 or v.dtype is not E4M3:
         raise TypeError(f"the cache holds {k.dtype} and {v.dtype}, expected float8_e4m3fn")
-    _shaped("cache.k_scales", ks, (pages, heads), torch.float32)
-    _shaped("cache.v_scales", vs, (pages, heads), torch.float32)
+    of_scales = (pages, heads)
+    _rows("cache.k_scales", ks, of_scales, torch.float32)
+    _rows("cache.v_scales", vs, of_scales, torch.float32)
     kp, kh, kt, ku = k.stride()
     vp, vh, vt, vu = v.stride()
     if ku != 1 or vu != 1:
         raise ValueError("the cache must have unit stride along head_dim")
-    ksp, ksh = ks.stride()
-    vsp, vsh = vs.stride()
-    if heads > 1 and (ksh != 1 or vsh != 1):
-        raise ValueError("the cache's scales must have unit stride over heads")
+    ksp, vsp = ks.stride(0), vs.stride(0)
     if pages <= 1 or heads <= 1:
         # the stride of a dimension of one element is never used: torch may say anything there
         dense = page * d
@@ -210,11 +208,10 @@ def _pack_cache(cache):
 
 
 def _page_table(table, batch):
-    if table.dim() != 2 or table.shape[0] != batch:
-        raise ValueError(f"'page_table' has shape {tuple(table.shape)}, expected ({batch}, pages)")
-    if table.dtype is not torch.int32:
-        raise TypeError(f"'page_table' is {table.dtype}, expected torch.int32")
-    _dense_rows("page_table", table)
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != batch:
+        raise ValueError(f"'page_table' has shape {tuple(shape)}, expected ({batch}, pages)")
+    _rows("page_table", table, shape, torch.int32)
 
 
 def kv_append(cache, k, v, page_table, starts, offsets, max_new):
@@ -229,27 +226,25 @@ def kv_append(cache, k, v, page_table, starts, offsets, max_new):
     or gets a larger one, to which the older tokens are then brought.  Sequences must not share the
     pages they write to.  Tokens whose page the table lacks are not written."""
     packed = _pack_cache(cache)
-    pages, heads, page, d = cache.k.shape
-    if k.dim() != 3 or k.shape[1:] != (heads, d):
-        raise ValueError(f"'k' has shape {tuple(k.shape)}, expected (tokens, {heads}, {d})")
-    _shaped("v", v, k.shape, k.dtype)
-    if k.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"kv_append: {k.dtype} (fp16 or bf16)")
-    _dense_rows("k", k)
-    _dense_rows("v", v)
+    heads, d = cache.k.shape[1], cache.k.shape[3]
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or shape[1] != heads or shape[2] != d:
+        raise ValueError(f"'k' has shape {tuple(shape)}, expected (tokens, {heads}, {d})")
+    if dtype not in _HALVES:
+        raise TypeError(f"kv_append: {dtype} (fp16 or bf16)")
+    _rows("k", k, shape, dtype)
+    _rows("v", v, shape, dtype)
     batch = starts.shape[0]
-    _shaped("starts", starts, (batch,), torch.int32)
-    _shaped("offsets", offsets, (batch + 1,), torch.int32)
-    _contiguous("starts", starts)
-    _contiguous("offsets", offsets)
+    _vector("starts", starts, batch, torch.int32)
+    _vector("offsets", offsets, batch + 1, torch.int32)
     _page_table(page_table, batch)
     stream = _launch_stream(
         "k v page_table starts offsets cache.k cache.v cache.k_scales cache.v_scales", k, v,
         page_table, starts, offsets, cache.k, cache.v, cache.k_scales, cache.v_scales)
     abi.check(abi.load().nb200_kv_append(
-        packed, k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), v.stride(0),
+        packed, k.data_ptr(), v.data_ptr(), shape[0], k.stride(0), k.stride(1), v.stride(0),
         v.stride(1), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-        starts.data_ptr(), offsets.data_ptr(), batch, max_new, _CODES[k.dtype], stream))
+        starts.data_ptr(), offsets.data_ptr(), batch, max_new, _CODES[dtype], stream))
 
 
 def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, out=None):
@@ -261,52 +256,45 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     with `window` > 0 only the last `window` of them and the first `sinks` of the sequence.  A query
     that sees nothing gives zeros.  scale: 1 / sqrt(head_dim) if not given."""
     packed = _pack_cache(cache)
-    if q.dim() != 4:
-        raise ValueError(f"'q' must be [batch, queries, heads, head_dim], got {tuple(q.shape)}")
-    batch, queries, heads, d = q.shape
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 4:
+        raise ValueError(f"'q' must be [batch, queries, heads, head_dim], got {tuple(shape)}")
+    batch, queries, heads, d = shape
     if d != cache.k.shape[3]:
         raise ValueError(f"'q' has head_dim {d}, the cache {cache.k.shape[3]}")
-    dtype = q.dtype
-    if dtype not in (torch.bfloat16, torch.float16):
+    if dtype not in _HALVES:
         raise TypeError(f"kv_attention: {dtype} (fp16 or bf16)")
-    _dense_rows("q", q)
-    _shaped("lengths", lengths, (batch,), torch.int32)
-    _contiguous("lengths", lengths)
+    _rows("q", q, shape, dtype)
+    _vector("lengths", lengths, batch, torch.int32)
     _page_table(page_table, batch)
     if out is None:
-        out = _rows_like(q, dtype)
+        out = _fresh(q, dtype)
     else:
-        _shaped("out", out, q.shape, dtype)
-        _dense_rows("out", out)
+        _rows("out", out, shape, dtype)
     stream = _launch_stream(
         "q page_table lengths out cache.k cache.v cache.k_scales cache.v_scales", q, page_table,
         lengths, out, cache.k, cache.v, cache.k_scales, cache.v_scales)
     lib = abi.load()
-    code = _CODES[dtype]
-    need = lib.nb200_kv_attention_workspace_bytes(packed, batch, queries, heads, code)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+    code, pages = _CODES[dtype], page_table.shape[1]
+    need = lib.nb200_kv_attention_workspace_bytes(packed, batch, queries, heads, pages, code)
+    ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    qb, qt, qh, _ = q.stride()
+    ob, ot, oh, _ = out.stride()
     abi.check(lib.nb200_kv_attention(
-        q.data_ptr(), packed, out.data_ptr(), batch, queries, heads, q.stride(0), q.stride(1),
-        q.stride(2), out.stride(0), out.stride(1), out.stride(2), page_table.data_ptr(),
-        page_table.stride(0), page_table.shape[1], lengths.data_ptr(),
+        q.data_ptr(), packed, out.data_ptr(), batch, queries, heads, qb, qt, qh, ob, ot, oh,
+        page_table.data_ptr(), page_table.stride(0), pages, lengths.data_ptr(),
         d ** -0.5 if scale is None else scale, window, sinks, code, _ptr(ws), need, stream))
     return out
 
 
 def _logits(logits):
-    if logits.dim() != 2:
-        raise ValueError(f"'logits' must be [rows, vocabulary], got {tuple(logits.shape)}")
-    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    shape = logits.shape
+    if len(shape) != 2:
+        raise ValueError(f"'logits' must be [rows, vocabulary], got {tuple(shape)}")
+    if logits.dtype not in _FLOATS:
         raise TypeError(f"'logits' is {logits.dtype} (fp32, fp16 or bf16)")
-    _dense_rows("logits", logits)
-    return logits.shape
-
-
-def _row_values(rows, dtype, **tensors):
-    for name, t in tensors.items():
-        if t is not None:
-            _shaped(name, t, (rows,), dtype)
-            _contiguous(name, t)
+    _rows("logits", logits, shape, logits.dtype)
+    return shape
 
 
 def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
@@ -315,19 +303,18 @@ def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
     their log probabilities, ties to the lower index.  tokens: int64 [rows]; a negative one stands
     for none and scores 0.  Returns TokenLogprobs of fp32 tensors (top_index: int64)."""
     rows, vocab = _logits(logits)
-    _row_values(rows, torch.int64, tokens=tokens)
+    if tokens is not None:
+        _vector("tokens", tokens, rows, torch.int64)
     if not 0 <= top <= 32:
         raise ValueError(f"token_logprobs: {top} alternatives (0 to 32)")
     stream = _launch_stream("logits tokens", logits, tokens)
-    device = logits.device
-    both = torch.empty((3, rows), dtype=torch.float32, device=device)
-    logprob, entropy, lse = both.unbind(0)
+    logprob, entropy, lse = logits.new_empty((3, rows), dtype=torch.float32).unbind(0)
     if tokens is None:
         logprob = None
     best = index = None
     if top:
-        best = torch.empty((rows, top), dtype=torch.float32, device=device)
-        index = torch.empty((rows, top), dtype=torch.int64, device=device)
+        best = logits.new_empty((rows, top), dtype=torch.float32)
+        index = logits.new_empty((rows, top), dtype=torch.int64)
     abi.check(abi.load().nb200_token_logprobs(
         logits.data_ptr(), _ptr(tokens), _ptr(logprob), entropy.data_ptr(), lse.data_ptr(),
         _ptr(best), _ptr(index), rows, vocab, logits.stride(0), top, inv_temperature,
@@ -341,14 +328,18 @@ def token_logprobs_backward(logits, tokens, lse, entropy, grad_logprob=None, gra
     + sum(grad_entropy * entropy), with the lse and entropy that it returned.  `out` may be the
     logits themselves."""
     rows, vocab = _logits(logits)
-    _row_values(rows, torch.int64, tokens=tokens)
-    _row_values(rows, torch.float32, lse=lse, entropy=entropy, grad_logprob=grad_logprob,
-                grad_entropy=grad_entropy)
+    if tokens is not None:
+        _vector("tokens", tokens, rows, torch.int64)
+    _vector("lse", lse, rows, torch.float32)
+    _vector("entropy", entropy, rows, torch.float32)
+    if grad_logprob is not None:
+        _vector("grad_logprob", grad_logprob, rows, torch.float32)
+    if grad_entropy is not None:
+        _vector("grad_entropy", grad_entropy, rows, torch.float32)
     if out is None:
-        out = _rows_like(logits, logits.dtype)
+        out = _fresh(logits, logits.dtype)
     else:
-        _shaped("out", out, (rows, vocab), logits.dtype)
-        _dense_rows("out", out)
+        _rows("out", out, (rows, vocab), logits.dtype)
     stream = _launch_stream("logits tokens lse entropy grad_logprob grad_entropy out", logits, tokens,
                             lse, entropy, grad_logprob, grad_entropy, out)
     abi.check(abi.load().nb200_token_logprobs_bwd(

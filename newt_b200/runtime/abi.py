@@ -94,7 +94,7 @@ SIGNATURES = {
                       [ctypes.c_float, ctypes.c_int, ctypes.c_int, _vp]),
     "nb200_kv_append": (ctypes.c_int, [ctypes.c_char_p, _vp, _vp] + [_i64] * 5 +
                         [_vp, _i64, _i64, _vp, _vp, _i64, _i64, ctypes.c_int, _vp]),
-    "nb200_kv_attention_workspace_bytes": (ctypes.c_int64, [ctypes.c_char_p, _i64, _i64, _i64,
+    "nb200_kv_attention_workspace_bytes": (ctypes.c_int64, [ctypes.c_char_p, _i64, _i64, _i64, _i64,
                                                             ctypes.c_int]),
     "nb200_kv_attention": (ctypes.c_int, [_vp, ctypes.c_char_p, _vp] + [_i64] * 9 +
                            [_vp, _i64, _i64, _vp, ctypes.c_float, _i64, _i64, ctypes.c_int, _vp,

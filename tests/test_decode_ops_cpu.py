@@ -85,6 +85,10 @@ def _grad(logits=P, tokens=P, lse=P, entropy=P, g=P, ge=P, out=P, rows=2, vocab=
     (lambda: _attend(q=None), abi.E_INVALID, "null"),
     (lambda: _attend(lengths=None), abi.E_INVALID, "null"),
     (lambda: _attend(max_pages=1 << 40), abi.E_INVALID, "extent"),
+    (lambda: _attend(max_pages=400, workspace=None), abi.E_INVALID, "workspace"),
+    (lambda: _attend(max_pages=400, size=1000), abi.E_INVALID, "workspace"),
+    (lambda: _attend(max_pages=400, workspace=P + 8), abi.E_INVALID, "workspace"),
+    (lambda: _attend(_cache(pages=0)), abi.E_INVALID, "no pages"),
     (lambda: _score(vocab=0), abi.E_INVALID, "vocabulary"),
     (lambda: _score(top=33, best=P, index=P), abi.E_UNSUPPORTED, "alternatives"),
     (lambda: _score(top=20, vocab=19, best=P, index=P), abi.E_INVALID, "alternatives"),

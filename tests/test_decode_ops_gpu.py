@@ -755,3 +755,18 @@ def test_a_prompt_and_its_decode_steps():
     mine = torch.cat([t.logprob for t in scores]).double()
     picked = log_p[torch.arange(total), torch.arange(total)]
     assert (mine - picked).abs().mean().item() < 0.1
+
+
+def test_attention_of_many_sequences_of_few_tiles():
+    """More sequences than shares of the work, of one to four steps each: shares of whole items, and
+    a table so short that no workspace is asked for."""
+    gen = _gen(63)
+    for longest in (700, 1000):
+        lengths = [1 + (i * 37) % longest for i in range(311)]
+        lengths[5] = longest
+        table, total = _pages(gen, lengths, 64)
+        table = table[:, :-(-longest // 64)].contiguous()
+        cache = _finite_cache(gen, total, 1, 64, 64)
+        q = _randn(gen, 311, 1, 2, 64, dtype=BF16)
+        lengths = _int32(lengths)
+        _check_attention(ops.kv_attention(q, cache, table, lengths), q, cache, table, lengths)
