@@ -5,26 +5,34 @@
 //
 // Forward: one pass over the row, in log2 units: y_j = x_j * (inv_temperature * log2 e).  Every
 // thread keeps a reference R (the largest y so far, rounded), S = sum 2^(y_j - R) and
-// E = sum 2^(y_j - R) (y_j - R); both are rescaled when R moves.  y_j - R is one fused
+// E = sum 2^(y_j - R) (y_j - R); both are rescaled when R grows.  y_j - R is one fused
 // multiply-add, exact but for its rounding, and R is only ever used as the rounded number it is, so
-// nothing is lost by its rounding; two lanes of packed fp32 share an instruction.  What the special
-// function unit does -- one 2^x per element -- takes three quarters of the time HBM does for 16-bit
-// logits, which is why everything else is kept to four or five instructions per element.  Logits
-// are raised to -1e30 at least, where 2^x is 0: -inf would make E a NaN.  log S and E / S give all
-// three results.  Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest value of a
-// wide type, +inf) are done again, from differences to the maximum, by the row's first CTA.
+// nothing is lost by its rounding; two lanes of packed fp32 share an instruction.  Logits are raised to
+// -1e30 at least, where 2^x is 0: -inf would make E a NaN.  log S and E / S give all three results.
+// Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest value of a wide type, +inf) are
+// done again, from differences to the maximum, by the row's first CTA.
+//
+// What bounds it: HBM, and for 16-bit logits the special function unit close behind, whose one 2^x per
+// element takes three quarters of the time HBM does; everything else is kept to four or five
+// instructions per element.  4096 x 50021 in bf16 take 70 us (5.8 TB/s), 2048 x 50021 in fp32 65
+// (6.3 TB/s).  Short rows wait for their first load and
+// their last reduction: 30000 x 3001 in bf16 reach 2 TB/s.
 //
 // Alternatives: an element's key is (order-preserving bits of the value, ~index), so keys differ
-// and ties go to the lowest index.  A CTA keeps a list of candidate keys in shared memory and the
-// key of its k-th largest so far; an element enters the list only above that.  The first threshold
-// comes from the first chunk of the row: in every warp the k-th largest of the 32 lanes' best keys
-// is a lower bound of the k-th largest.  The list has room for a whole chunk of new candidates, so
-// no order of the logits makes it overflow; it is cut back to k keys when it has grown.
+// and ties go to the lowest index.  The pass above is the same with and without them.  Behind it the
+// k-th largest of the threads' own maxima bounds the k-th largest logit from below, and only the k
+// threads whose maxima reach the bound can have seen one of the k largest: their vectors, a few
+// hundred, are read again, and what reaches the bound is sorted in shared memory.  The list has room
+// for a whole step of new candidates and is cut back to k keys when it has grown, so no order of the
+// logits and no ties make it overflow.  4096 x 50021 in fp16 with 5 alternatives take 90 us.  (Keeping
+// the k largest during the pass, with a barrier per chunk for the common threshold: 332 us.)
 //
-// HBM-bound.  A row is shared by a cluster of 1 to 8 CTAs, as many as it takes for few rows to
-// fill the chip; their partial results meet in the first CTA's shared memory, in rank order.
-// Rows of any alignment are read in 16-byte vectors from their first 16-byte boundary on, with
-// the elements before and after them one by one.
+// Few rows are shared by clusters of up to 8 CTAs; their partial results meet in the first CTA's shared
+// memory, in rank order.  Rows of any alignment are read in 16-byte vectors from their first 16-byte
+// boundary on, with the elements before and after them one by one.
+//
+// Gradient: one read and one write of the logits, everything between in registers: 4096 x 50021 in bf16
+// take 121 us (6.8 TB/s), 65 x 32000 in fp32 3.1.
 
 #include "elem.cuh"
 #include "sm100.cuh"
@@ -37,7 +45,7 @@ using namespace sm100;
 constexpr int kThreads = 256;            // of the gradient; the forward pass says its own
 constexpr int kMaxCluster = 8;
 constexpr int kTopMax = 32;
-constexpr int kListKept = 4 * kTopMax;   // candidates that may stay in the list between chunks
+constexpr int kListKept = 4 * kTopMax;   // candidates that may stay in the list between two steps
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -119,16 +127,10 @@ __device__ __forceinline__ void unpack(const Vec<__half>& v, float (&f)[8], floa
   most = fmaxf(most, fmaxf(__low2float(m), __high2float(m)));
 }
 
-// How a CTA reads: `kVectors` 16-byte vectors per thread at a time, a chunk, with the next two chunks
-// under way.  With alternatives a chunk is also what is read between two looks at the candidates.
-// The CTAs per SM are what the registers and 80 KB or so of loads in flight come to.
-template <typename T, bool TOP>
-struct Chunk {
-  static constexpr int kThreads = TOP ? 512 : 256, kWarps = kThreads / 32;
-  static constexpr int kCtas = TOP ? 2 : 4;
-  static constexpr int kVectors = 2;
-  static constexpr int kElems = kThreads * kVectors * Elem<T>::kPerVec;
-};
+// How a CTA of so many threads reads: `kVectors` 16-byte vectors per thread at a time, a chunk, with the
+// next two chunks under way.  The CTAs per SM are what 64 registers per thread come to.
+constexpr int kVectors = 2;
+constexpr int ctas_per_sm(int threads) { return 1024 / threads; }
 
 struct ClusterShared {
   Partial part[kMaxCluster];
@@ -136,7 +138,7 @@ struct ClusterShared {
 };
 
 struct TopState {
-  unsigned long long* list;   // kListKept + a chunk + the elements around the vectors
+  unsigned long long* list;   // kListKept + the elements of kVectors vectors per thread + those around the vectors
   unsigned long long* sorted; // kTopMax
   unsigned long long* warp_best;
   int* count;
@@ -207,22 +209,78 @@ __device__ __forceinline__ bool offer(TopState& t, float v, int index) {
   return at >= kListKept;
 }
 
-// A lower bound of the k-th largest of the chunk from the threads' best keys, less one so that the key
-// itself passes: over the W warps that have elements, the smallest of their ceil(k / W)-th largest.
-// For values in no order it lets through two or three times k.
+// A lower bound of the k-th largest of the threads' values: over the warps whose lanes all have
+// vectors, the smallest of their ceil(k / warps)-th largest.
 template <int THREADS>
-__device__ __forceinline__ void first_threshold(TopState& t, unsigned long long best, int vectors) {
-  const int w = min((vectors + 31) / 32, THREADS / 32);
-  unsigned long long kth = ~0ull;
-  for (int i = 0; i < (t.k + w - 1) / w; ++i) {
-    kth = warp_max_key(best);
-    if (best == kth) best = 0;
+__device__ __forceinline__ float lower_bound(float value, int k, int vectors, float* warp_value) {
+  const int w = max(min(vectors, THREADS) / 32, 1);
+  float kth = -INFINITY;
+  for (int i = 0; i < (k + w - 1) / w; ++i) {
+    kth = warp_max(value);
+    if (value == kth) value = -INFINITY;
   }
-  if ((threadIdx.x & 31) == 0) t.warp_best[threadIdx.x >> 5] = kth;
+  if ((threadIdx.x & 31) == 0) warp_value[threadIdx.x >> 5] = kth;
   __syncthreads();
-  unsigned long long least = ~0ull;
-  for (int i = 0; i < w; ++i) least = t.warp_best[i] < least ? t.warp_best[i] : least;
-  t.threshold = least > 0 ? least - 1 : 0;
+  float least = INFINITY;
+  for (int i = 0; i < w; ++i) least = fminf(least, warp_value[i]);
+  return least;
+}
+
+// The k largest keys of a CTA's part of a row into t.list, from the largest logit of each thread.  The
+// k-th largest of those bounds the CTA's k-th largest logit from below, so that only the vectors of the
+// k threads (more, with ties) that reach the bound are read again, by all threads, and few of their
+// elements pass.  `body`: v1 - v0 vectors, of which thread i had i, i + THREADS, ...; `first` is the
+// row's index of the first element.  `alone`: this thread's elements around the vectors, -1 for none.
+template <typename T, int THREADS>
+__device__ __forceinline__ void gather(TopState& t, const T* x, const T* body, int vectors, int first, float largest,
+                                       const int (&alone)[2], unsigned long long* picks, int* picked) {
+  constexpr int E = Elem<T>::kPerVec, U = kVectors;
+  const int tid = threadIdx.x;
+  float bound = lower_bound<THREADS>(largest, t.k, vectors, reinterpret_cast<float*>(t.warp_best));
+  if (bound <= kLowest) bound = -INFINITY;           // what `largest` says of raised logits is no bound
+  if (largest >= bound) picks[atomicAdd(picked, 1)] = make_key(largest, tid);
+  __syncthreads();
+  int n = *picked;
+  uint32_t least = (uint32_t)(make_key(bound, 0) >> 32);
+  const int per = (vectors + THREADS - 1) / THREADS;
+  constexpr int kStep = THREADS * U;
+  if ((n * per - 1) / kStep > (t.k * per - 1) / kStep) {   // the bound itself saves a step below
+    const unsigned long long mine = tid < n ? picks[tid] : 0ull;
+    const int rank = tid < n ? count_larger(picks, n, mine) : 0;
+    __syncthreads();
+    if (tid < n) picks[rank] = mine;
+    __syncthreads();
+    if (key_value(picks[t.k - 1]) > kLowest) least = (uint32_t)(picks[t.k - 1] >> 32);
+    n = __syncthreads_count(tid < n && (uint32_t)(mine >> 32) >= least);
+  }
+  t.threshold = ((unsigned long long)least << 32) - 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (alone[i] >= 0) offer(t, Elem<T>::to_f32(x[alone[i]]), alone[i]);
+  for (int item = tid; item - tid < n * per; item += kStep) {
+    Vec<T> v[U];
+    int at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = item + u * THREADS;
+      at[u] = i < n * per ? key_index(picks[i % n]) + i / n * THREADS : vectors;
+      if (at[u] < vectors) v[u].raw = ld_once(body + (int64_t)at[u] * E);
+    }
+    bool grown = false;
+    const float reach = key_value(t.threshold + 1);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at[u] >= vectors) continue;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float f = Elem<T>::to_f32(v[u].e[j]);
+        if (!(f < reach)) grown |= offer(t, f, first + at[u] * E + j);   // NaN may pass, with -inf
+      }
+    }
+    if (__syncthreads_or(grown)) compact<THREADS>(t);
+  }
+  __syncthreads();
+  compact<THREADS>(t);
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -286,15 +344,15 @@ __device__ __noinline__ Partial whole_row(const T* x, int vocab, float factor, P
   return total;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas) logprob_kernel(const LogprobParams p) {
-  using C = Chunk<T, TOP>;
-  constexpr int E = Elem<T>::kPerVec, U = C::kVectors, kThreads = C::kThreads, kWarps = C::kWarps;
+template <typename T, bool TOP, int kThreads>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(kThreads)) logprob_kernel(const LogprobParams p) {
+  constexpr int E = Elem<T>::kPerVec, U = kVectors, kWarps = kThreads / 32;
   __shared__ ClusterShared meet;       // filled by the cluster, in the first CTA
   __shared__ Partial warp_part[kWarps];
   __shared__ unsigned long long sorted[kTopMax], warp_best[kWarps];
-  __shared__ int count;
-  extern __shared__ __align__(16) unsigned long long list[];
+  __shared__ int count, picked;
+  extern __shared__ __align__(16) unsigned long long dynamic[];   // with alternatives: keys of threads, candidates
+  unsigned long long *picks = dynamic, *list = dynamic + kThreads + 2;
 
   const int rank = (int)cluster_rank(), ranks = (int)cluster_size();
   const int row = blockIdx.x / ranks;
@@ -321,10 +379,7 @@ __global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas)
   }
 
   TopState top{list, sorted, warp_best, &count, 0ull, p.top};
-  if constexpr (TOP) {
-    if (tid == 0) count = 0;
-    __syncthreads();
-  }
+  if (TOP && tid == 0) count = picked = 0;
 
   float largest = -INFINITY;           // of the logits as they are
   float ref = 0.0f;                    // means something once `largest` does
@@ -380,39 +435,6 @@ __global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas)
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < E; j += 2) take2(f[u][j], f[u][j + 1]);
-    if constexpr (TOP) {
-      // a raised logit is one of the few cases where the row itself is asked again
-      auto value = [&](int u, int j, int index) {
-        return f[u][j] < 0.9f * kLowest ? Elem<T>::to_f32(x[index]) : f[u][j];
-      };
-      bool grown = base == v0;
-      if (base == v0) {
-        unsigned long long best = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int at = base + u * kThreads + tid;
-          if (at < v1) {
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-              const unsigned long long key = make_key(value(u, j, head + at * E + j), head + at * E + j);
-              best = key > best ? key : best;
-            }
-          }
-        }
-        first_threshold<kThreads>(top, best, v1 - v0);
-      }
-      if (!(most < key_value(top.threshold))) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int at = base + u * kThreads + tid;
-          if (at < v1) {
-#pragma unroll
-            for (int j = 0; j < E; ++j) grown |= offer(top, value(u, j, head + at * E + j), head + at * E + j);
-          }
-        }
-      }
-      if (__syncthreads_or(grown)) compact<kThreads>(top);     // the same answer in every thread
-    }
   };
   load(raw[0], v0);
   load(raw[1], v0 + kStep);
@@ -428,14 +450,12 @@ __global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas)
     const float v = Elem<T>::to_f32(x[index]);
     if (v > largest) raise(v);
     take2(raised(v), kLowest);
-    if constexpr (TOP) offer(top, v, index);
   };
-  if (rank == 0 && tid < head) take(tid);
-  if (rank == ranks - 1 && tail + tid < vocab) take(tail + tid);
-  if constexpr (TOP) {
-    __syncthreads();
-    compact<kThreads>(top);
-  }
+  const int alone[2] = {rank == 0 && tid < head ? tid : -1, rank == ranks - 1 && tail + tid < vocab ? tail + tid : -1};
+  if (alone[0] >= 0) take(alone[0]);
+  if (alone[1] >= 0) take(alone[1]);
+  if constexpr (TOP)
+    gather<T, kThreads>(top, x, body + (int64_t)v0 * E, v1 - v0, head + v0 * E, largest, alone, picks, &picked);
 
   // the CTA's sums: relative to the warp's reference, then to the CTA's
   float sa, sb, ea, eb;
@@ -481,7 +501,7 @@ __global__ void __launch_bounds__(Chunk<T, TOP>::kThreads, Chunk<T, TOP>::kCtas)
     if (rank != 0) return;
     total = merge(meet.part, ranks);
     if constexpr (TOP) {
-      // at most kMaxCluster * kTopMax <= kThreads keys; 0 stands for none
+      // at most kMaxCluster * kTopMax keys, no more than threads where there are clusters; 0 stands for none
       const int n = ranks * p.top;
       if (tid < p.top) list[tid] = 0;
       __syncthreads();
@@ -615,23 +635,17 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
 
 // ---- host -----------------------------------------------------------------------------------------
 
-template <typename T, bool TOP>
-int launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
-  auto kern = logprob_kernel<T, TOP>;
-  using C = Chunk<T, TOP>;
-  constexpr int kList = kListKept + C::kElems + 16;
-  const int smem = TOP ? kList * (int)sizeof(unsigned long long) : 0;
+template <typename T, bool TOP, int THREADS>
+int launch_logprobs(const LogprobParams& p, int ranks, cudaStream_t stream) {
+  auto kern = logprob_kernel<T, TOP, THREADS>;
+  // picks, and the list with the elements that one step of the gathering and those around the vectors add
+  constexpr int kKeys = THREADS + 2 + kListKept + (THREADS * kVectors + 2) * Elem<T>::kPerVec;
+  const int smem = TOP ? kKeys * (int)sizeof(unsigned long long) : 0;
   if (TOP)
     if (int rc = prepare_kernel((const void*)kern, smem)) return rc;
-  // CTAs per row: until the rows fill the chip twice over, as long as each has a chunk to read
-  const int sms = device_info().sm_count;
-  int ranks = 1;
-  while (ranks < kMaxCluster && (int64_t)p.rows * ranks * 2 <= 4 * sms &&
-         p.vocab >= ranks * 2 * C::kElems)
-    ranks *= 2;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)p.rows * ranks);
-  config.blockDim = dim3(C::kThreads);
+  config.blockDim = dim3(THREADS);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr;
@@ -642,6 +656,23 @@ int launch_logprobs(const LogprobParams& p, cudaStream_t stream) {
   config.attrs = &attr;
   config.numAttrs = 1;
   return cuda_check(cudaLaunchKernelEx(&config, kern, p), "token logprobs launch");
+}
+
+template <typename T, bool TOP>
+int dispatch_logprobs(const LogprobParams& p, cudaStream_t stream) {
+  // More rows than SMs: a small CTA per row, many of them per SM, so that some stream while others start
+  // or finish their rows (4096 x 50021 bf16: 70 us; CTAs of 256 threads 76, of 64 85; 600 rows: 17.3, with
+  // CTAs of 512 threads 20.6; with 5 alternatives 21 and 30).
+  const int sms = device_info().sm_count;
+  if (p.rows > sms) return launch_logprobs<T, TOP, 128>(p, 1, stream);
+  // Otherwise a large CTA per row, or a cluster of them as long as the rows have no more CTAs than there
+  // are SMs and each CTA has a chunk to read.  A second CTA per SM loses more to the cluster's
+  // barriers than it gains: 100 rows of 50021 take 6.2 us, shared by two CTAs 7.3; with alternatives
+  // 9.6 and 11.9; 16 rows of 129001 in fp32 with 20 take 11.3.
+  constexpr int kChunk = 512 * kVectors * Elem<T>::kPerVec;
+  int ranks = 1;
+  while (ranks < kMaxCluster && p.rows * ranks * 2 <= sms && p.vocab >= ranks * 2 * kChunk) ranks *= 2;
+  return launch_logprobs<T, TOP, 512>(p, ranks, stream);
 }
 
 template <typename T>
@@ -692,12 +723,12 @@ extern "C" int nb200_token_logprobs(const void* logits, const int64_t* tokens, f
                   (int)vocab, (int)top, inv_temperature};
   switch (dtype) {
     case NB200_F32:
-      return top ? launch_logprobs<float, true>(p, stream) : launch_logprobs<float, false>(p, stream);
+      return top ? dispatch_logprobs<float, true>(p, stream) : dispatch_logprobs<float, false>(p, stream);
     case NB200_F16:
-      return top ? launch_logprobs<__half, true>(p, stream) : launch_logprobs<__half, false>(p, stream);
+      return top ? dispatch_logprobs<__half, true>(p, stream) : dispatch_logprobs<__half, false>(p, stream);
     default:
-      return top ? launch_logprobs<__nv_bfloat16, true>(p, stream)
-                 : launch_logprobs<__nv_bfloat16, false>(p, stream);
+      return top ? dispatch_logprobs<__nv_bfloat16, true>(p, stream)
+                 : dispatch_logprobs<__nv_bfloat16, false>(p, stream);
   }
 }
 

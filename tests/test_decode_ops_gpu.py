@@ -546,6 +546,40 @@ def test_token_logprobs_of_masked_logits(dtype):
         assert (grad[2] == 0).all()               # masked as a whole
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("vocab", [3, 100, 1023, 4099, 20011])
+def test_token_logprobs_of_many_rows(vocab, dtype):
+    """More rows than the chip has SMs: each is one small CTA's."""
+    gen = _gen(vocab)
+    x = _randn(gen, 301, vocab, dtype=dtype, scale=3.0)
+    tokens = torch.randint(0, vocab, (301,), generator=gen, device="cuda")
+    for top, inv in ((0, 1.0), (1, 0.7), (min(5, vocab), 1.25), (min(32, vocab), 2.0)):
+        _check_scores(x, tokens, top, inv)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("vocab", [33, 1000, 4099, 20000])
+def test_alternatives_of_any_order(vocab, rows, dtype):
+    """Equal, ordered, sparse and bunched logits: no list overflows and ties go to the lower index."""
+    gen = _gen(vocab + rows)
+    steps = torch.arange(vocab, device="cuda").float() * (20.0 / vocab)
+    sparse = torch.full((vocab,), -math.inf, device="cuda")
+    sparse[::max(1, vocab // 9)] = 1.0
+    bunched = _randn(gen, vocab)
+    bunched[::8] += 50.0
+    not_numbers = _randn(gen, vocab)
+    not_numbers[::7] = math.nan
+    lowest = torch.full((vocab,), torch.finfo(dtype).min, device="cuda")
+    for row in (torch.full((vocab,), 1.5, device="cuda"), steps, -steps, steps.round(), sparse, bunched,
+                not_numbers, lowest, sparse - math.inf):
+        x = row.to(dtype).expand(rows, vocab).contiguous()
+        order = torch.sort(x.float().nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf), dim=1,
+                           descending=True, stable=True)[1]
+        for top in (1, 2, 7, 32):
+            assert torch.equal(ops.token_logprobs(x, top=top).top_index, order[:, :top])
+
+
 def test_token_logprobs_of_rows_without_any_and_of_nan():
     x = torch.full((4, 5000), float("-inf"), device="cuda")
     x[1, 77], x[1, 78] = float("nan"), 1.0
