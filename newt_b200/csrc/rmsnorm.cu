@@ -9,10 +9,14 @@
 // HBM-bound: 16-bit rows with a residual and an e4m3 output move 7 bytes per element for about
 // ten instructions.  A row lives in registers, ITEMS 16-byte vectors of x and of the residual per
 // thread, so both are read once and all of a row's loads are in flight before its first use.
-// `threads` threads share a row (32: a warp per row, eight rows per CTA; more: one row per CTA).
+// `threads` threads share a row (32: a warp per row, eight rows per CTA; more: one row per CTA): as
+// many warps as the row's vectors fill.  8191 x 4096 fp16 with a residual, e4m3 by 128 columns: 39 us
+// (6.0 TB/s); 8 x 4096 bf16: 2.7 us, one row's chain of loads and two reductions.
 // Nothing is prefetched across rows: the loads of the other resident CTAs cover a row's
 // reductions.  The weight is read through L1, where it stays: x and the residual do not allocate
 // there.
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "elem.cuh"
@@ -22,6 +26,8 @@ namespace nb200 {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;
+constexpr int kMaxColumns = 32768;     // 32 values per thread are what 1024 threads have registers for
+constexpr int kMaxShifted = 16384;     // of shifted rows, which take a few registers more
 
 // The scale of values of magnitude up to `most`, and what they are multiplied with: 1 where they are
 // all zero, or so small that the scale is no normal number (they become zeros).  Neither is the
@@ -70,15 +76,44 @@ struct Max {   // of magnitudes: 0 is neutral
   __device__ static float apply(float a, float b) { return fmaxf(a, b); }
 };
 
-// FAST: every row of every tensor starts on a 16-byte boundary (8-byte for the e4m3 output of a
-// 16-bit type) and n is a multiple of the vector: a thread's E columns are neighbours.  Otherwise a
-// warp's 32 * E columns are the same but a thread's lie 32 apart, so that every access of a warp is
-// one run of elements whatever the row's alignment (8191 x 4097 fp16: 162 us with E neighbours read
-// one by one and as many stores of a byte or two, 160 like this: the count of accesses is what is left).
-template <typename T, bool E4M3, int ITEMS, bool FAST, int MAX_THREADS>
+// How a row's columns are spread over its threads.
+//   ALIGNED: every row of every tensor starts on a 16-byte boundary (8-byte or 4-byte for the e4m3
+//     output) and n is a multiple of the vector: a thread's E columns are neighbours.
+//   SHIFTED: the rows start anywhere, but at the same remainder `m` in all tensors but the weight, as rows
+//     of odd length do: vectors from the row's first boundary on, the elements around them one to a thread.
+//     The weight's vectors are put together from two each, the second of which ends inside the row too.
+//     A thread's columns may lie in two groups, so the groups' maxima meet in shared memory.
+//   SINGLE: neither.  A warp's 32 * E columns are the same but a thread's lie 32 apart, so that every access
+//     of a warp is one run of elements.
+// 8191 x 4097 fp16 with a residual, e4m3 by 128: 66 us SHIFTED (issue slots: 64 % busy), 160 SINGLE (five
+// accesses an element); 8191 x 4096 ALIGNED 39.
+enum Spread { ALIGNED, SHIFTED, SINGLE };
+
+// E elements from `off` < E on of the 2 * E in lo and hi.
+template <typename T>
+__device__ __forceinline__ Vec<T> window(const uint4& lo, const uint4& hi, int off) {
+  const int bits = off * (int)sizeof(T) * 8, q = bits >> 5;
+  const uint32_t a[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  uint32_t b[7], c[5];
+#pragma unroll
+  for (int k = 0; k < 7; ++k) b[k] = (q & 1) ? a[k + 1] : a[k];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) c[k] = (q & 2) ? b[k + 2] : b[k];
+  Vec<T> r;
+  r.raw.x = __funnelshift_r(c[0], c[1], bits);
+  r.raw.y = __funnelshift_r(c[1], c[2], bits);
+  r.raw.z = __funnelshift_r(c[2], c[3], bits);
+  r.raw.w = __funnelshift_r(c[3], c[4], bits);
+  return r;
+}
+
+template <typename T, bool E4M3, int ITEMS, int SPREAD, int MAX_THREADS>
 __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
   constexpr int E = Elem<T>::kPerVec;
+  constexpr bool FAST = SPREAD == ALIGNED, WHOLE = SPREAD != SINGLE;
   __shared__ float slots[2][32];
+  // SHIFTED: the groups' maxima, a row's behind the other's (a row of one warp has at most 32 groups)
+  __shared__ uint32_t group_most[SPREAD == SHIFTED && E4M3 ? kMaxShifted / 32 : 1];
   const int warps = p.threads >> 5;
   const int per_cta = blockDim.x / p.threads;
   const int lane = threadIdx.x % p.threads;       // of the row
@@ -89,43 +124,75 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
   }
   if (row >= p.rows) return;     // whole warps, and only where a row is a warp
   const int n = p.n;
+  const int groups = (n + (1 << p.group_shift) - 1) >> p.group_shift;
+  uint32_t* most_of = group_most + threadIdx.x / p.threads * groups;
+  if (SPREAD == SHIFTED && E4M3 && p.group_shift) {
+    for (int g = lane; g < groups; g += p.threads) most_of[g] = 0;   // the row's first reduction is the barrier
+    if (warps == 1) __syncwarp();
+  }
   const T* x = static_cast<const T*>(p.x) + row * p.stride_x;
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.stride_residual : nullptr;
   const T* w = static_cast<const T*>(p.w);
-  const int col0 = FAST ? lane * E : (lane >> 5) * 32 * E + (lane & 31), col_step = p.threads * E;
-  auto column = [&](int i, int j) { return col0 + i * col_step + (FAST ? j : 32 * j); };
+  const int m = SPREAD == SHIFTED ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
+  const int head = m ? E - m : 0;
+  const int end = SPREAD == SHIFTED ? head + max(n - m - head, 0) / E * E : n;     // of the vectors
+  // vectors from m columns before the row on, the first of them left out where m is not 0
+  const int col0 = WHOLE ? lane * E - m : (lane >> 5) * 32 * E + (lane & 31), col_step = p.threads * E;
+  auto column = [&](int i, int j) { return col0 + i * col_step + (WHOLE ? j : 32 * j); };
+  auto whole = [&](int i) { return (unsigned)column(i, 0) < (unsigned)end; };
+  // this thread's element outside of the vectors: at most 2 E - 1 threads of a row have one
+  const int alone = SPREAD != SHIFTED ? n : lane < head ? lane : end - head + lane;
+  const bool has_alone = SPREAD == SHIFTED && lane < n - (end - head);
 
-  // this thread's part of a row; columns past n are 0
-  auto read = [&](const T* from, bool once, Vec<T> (&to)[ITEMS]) {
+  // this thread's part of a row; columns outside of it are 0
+  auto read = [&](const T* from, Vec<T> (&to)[ITEMS]) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      if constexpr (FAST) {
-        to[i].raw = make_uint4(0, 0, 0, 0);
-        if (column(i, 0) < n)
-          to[i].raw = once ? ld_once(from + column(i, 0)) : __ldg(reinterpret_cast<const uint4*>(from + column(i, 0)));
+      to[i].raw = make_uint4(0, 0, 0, 0);
+      if constexpr (WHOLE) {
+        if (whole(i)) to[i].raw = ld_once(from + column(i, 0));
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j)
-          to[i].e[j] = column(i, j) < n ? from[column(i, j)] : Elem<T>::from_f32(0.0f);
+          if (column(i, j) < n) to[i].e[j] = from[column(i, j)];
       }
     }
   };
-  auto write = [&](T* to, const float (&from)[ITEMS * E]) {
+  auto read_weight = [&](Vec<T> (&to)[ITEMS]) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      if constexpr (FAST) {
-        if (column(i, 0) < n) st_once(to + column(i, 0), round_elems<T>(&from[i * E]).raw);
+      to[i].raw = make_uint4(0, 0, 0, 0);
+      if constexpr (WHOLE) {
+        if (!whole(i)) continue;
+        const uint4* at = reinterpret_cast<const uint4*>(w + column(i, 0) - head);
+        to[i].raw = __ldg(at);
+        if (SPREAD == SHIFTED && m) to[i] = window<T>(to[i].raw, __ldg(at + 1), head);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (column(i, j) < n) to[i].e[j] = w[column(i, j)];
+      }
+    }
+  };
+  auto write = [&](T* to, const float (&from)[ITEMS * E], float from_alone) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if constexpr (WHOLE) {
+        if (whole(i)) st_once(to + column(i, 0), round_elems<T>(&from[i * E]).raw);
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j)
           if (column(i, j) < n) to[column(i, j)] = Elem<T>::from_f32(from[i * E + j]);
       }
     }
+    if (has_alone) to[alone] = Elem<T>::from_f32(from_alone);
   };
 
   Vec<T> xv[ITEMS], rv[ITEMS];
-  read(x, true, xv);
-  if (res) read(res, true, rv);
+  read(x, xv);
+  if (res) read(res, rv);
+  float single = has_alone ? Elem<T>::to_f32(x[alone]) : 0.0f;
+  if (res && has_alone) single += Elem<T>::to_f32(res[alone]);
   float v[ITEMS * E];
 #pragma unroll
   for (int k = 0; k < ITEMS * E; ++k) v[k] = Elem<T>::to_f32(xv[k / E].e[k % E]);
@@ -133,20 +200,25 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
 #pragma unroll
     for (int k = 0; k < ITEMS * E; ++k) v[k] += Elem<T>::to_f32(rv[k / E].e[k % E]);
   }
-  float sum = 0.0f;
+  float sum = single * single;
 #pragma unroll
   for (int k = 0; k < ITEMS * E; ++k) sum = fmaf(v[k], v[k], sum);
-  if (p.residual_out) write(static_cast<T*>(p.residual_out) + row * p.stride_residual_out, v);
+  if (p.residual_out) write(static_cast<T*>(p.residual_out) + row * p.stride_residual_out, v, single);
   sum = reduce_row<Add>(sum, slots[0], warps);
   const float rstd = rsqrtf(sum / (float)n + p.eps);
-  read(w, false, xv);
+  read_weight(xv);
+  if (has_alone) single = single * rstd * Elem<T>::to_f32(w[alone]);
 #pragma unroll
   for (int k = 0; k < ITEMS * E; ++k) v[k] = v[k] * rstd * Elem<T>::to_f32(xv[k / E].e[k % E]);
 
   if constexpr (!E4M3) {
-    write(static_cast<T*>(p.out) + row * p.stride_out, v);
+    write(static_cast<T*>(p.out) + row * p.stride_out, v, single);
   } else {
-    float amax[ITEMS][FAST ? 1 : E];      // of a thread's columns: one scale for all of them, or for each
+    // of a thread's columns: one scale for all of them, one for those before column m and one for those
+    // from it on, or one for each
+    constexpr int SCALES = FAST ? 1 : SPREAD == SHIFTED ? 2 : E;
+    float amax[ITEMS][SCALES];
+    float most_alone = 0.0f;                    // of the group of the element outside of the vectors
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       amax[i][0] = 0.0f;
@@ -155,14 +227,15 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
     }
     float* scales = p.scales + row * p.stride_scales;
     if (p.group_shift == 0) {
-      float most = amax[0][0];
+      float most = fmaxf(amax[0][0], fabsf(single));
 #pragma unroll
       for (int i = 1; i < ITEMS; ++i) most = fmaxf(most, amax[i][0]);
       most = reduce_row<Max>(most, slots[1], warps);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int j = 0; j < (FAST ? 1 : E); ++j) amax[i][j] = most;
+        for (int j = 0; j < SCALES; ++j) amax[i][j] = most;
+      most_alone = most;
       if (lane == 0) scales[0] = e4m3_scale(most);
     } else if constexpr (FAST) {
       // a group is 32, 64 or 128 columns: 4 to 32 neighbouring lanes
@@ -173,6 +246,36 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
           amax[i][0] = fmaxf(amax[i][0], __shfl_xor_sync(0xffffffffu, amax[i][0], o));
         const int col = column(i, 0);
         if ((lane & (lanes - 1)) == 0 && col < n) scales[col >> p.group_shift] = e4m3_scale(amax[i][0]);
+      }
+    } else if constexpr (SPREAD == SHIFTED) {
+      // A vector's columns from its m-th on and those before the m-th of the thread behind are E neighbours
+      // from a multiple of E on, in one group; a warp's last thread leaves the thread behind to that
+      // one's warp.
+      const int lanes = (1 << p.group_shift) / E, in_warp = threadIdx.x & 31;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        float before = 0.0f, from = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float a = fabsf(v[i * E + j]);
+          if (j < m) before = fmaxf(before, a); else from = fmaxf(from, a);
+        }
+        const float behind = __shfl_down_sync(0xffffffffu, before, 1);
+        if (in_warp < 31) from = fmaxf(from, behind);
+        for (int o = lanes >> 1; o > 0; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xffffffffu, from, o));
+        const int col = column(i, 0) + m;            // magnitudes are ordered as their bits are
+        if (in_warp == 0 && m && col <= end) atomicMax(&most_of[(col - 1) >> p.group_shift], __float_as_uint(before));
+        if ((in_warp & (lanes - 1)) == 0 && col < n) atomicMax(&most_of[col >> p.group_shift], __float_as_uint(from));
+      }
+      if (has_alone) atomicMax(&most_of[alone >> p.group_shift], __float_as_uint(fmaxf(fabsf(single), 0.0f)));
+      if (warps > 1) __syncthreads(); else __syncwarp();
+      if (has_alone) most_alone = __uint_as_float(most_of[alone >> p.group_shift]);
+      for (int g = lane; g < groups; g += p.threads) scales[g] = e4m3_scale(__uint_as_float(most_of[g]));
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int col = column(i, 0) + m;
+        amax[i][0] = __uint_as_float(most_of[min(max(col - 1, 0) >> p.group_shift, groups - 1)]);
+        amax[i][1] = __uint_as_float(most_of[min(col >> p.group_shift, groups - 1)]);
       }
     } else {
       // a group is one, two or four neighbouring runs of 32 columns
@@ -201,61 +304,79 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
     uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.stride_out;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      if constexpr (FAST) {
-        if (column(i, 0) < n) store_e4m3<E>(out + column(i, 0), &v[i * E], e4m3_factor(amax[i][0]));
+      if constexpr (WHOLE) {
+        if (!whole(i)) continue;
+        const float factor = e4m3_factor(amax[i][0]);
+        if constexpr (SPREAD == SHIFTED) {
+          const float from = e4m3_factor(amax[i][1]);
+#pragma unroll
+          for (int j = 0; j < E; ++j) v[i * E + j] *= j < m ? factor : from;
+        }
+        store_e4m3<E>(out + column(i, 0), &v[i * E], SPREAD == SHIFTED ? 1.0f : factor);
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j)
           if (column(i, j) < n) out[column(i, j)] = (uint8_t)e4m3x2(v[i * E + j] * e4m3_factor(amax[i][j]), 0.0f);
       }
     }
+    if (has_alone) out[alone] = (uint8_t)e4m3x2(single * e4m3_factor(most_alone), 0.0f);
   }
 }
 
 template <typename T, bool E4M3, int ITEMS>
-int launch_rms(const RmsParams& p, bool fast, cudaStream_t stream) {
+int launch_rms(const RmsParams& p, Spread spread, cudaStream_t stream) {
   const int threads = p.threads == 32 ? 256 : p.threads;
   const int64_t grid = cdiv64(p.rows, threads / p.threads);
   auto go = [&](auto kern) {
     kern<<<(int)grid, threads, 0, stream>>>(p);
     return cuda_check(cudaGetLastError(), "rmsnorm launch");
   };
-  // up to 256 threads a CTA may have 255 registers a thread, 1024 have 64
-  if (threads <= 256)
-    return fast ? go(rms_kernel<T, E4M3, ITEMS, true, 256>) : go(rms_kernel<T, E4M3, ITEMS, false, 256>);
-  return fast ? go(rms_kernel<T, E4M3, ITEMS, true, 1024>) : go(rms_kernel<T, E4M3, ITEMS, false, 1024>);
+  // Registers a thread: 64 fit 1024 threads.  Aligned rows do with that (bounds of 256 threads give them 68
+  // and seven CTAs of 128 instead of eight: 39.1 us, not 38.8), shifted ones spill (86: 70 us, 91: 66).
+  auto of = [&](auto spread) {
+    constexpr int S = decltype(spread)::value;
+    constexpr int SMALL = S == ALIGNED ? 512 : 256;
+    return threads <= SMALL ? go(rms_kernel<T, E4M3, ITEMS, S, SMALL>) : go(rms_kernel<T, E4M3, ITEMS, S, 1024>);
+  };
+  if (spread == ALIGNED) return of(std::integral_constant<int, ALIGNED>());
+  if constexpr (ITEMS <= 4)            // what kMaxShifted columns come to
+    if (spread == SHIFTED) return of(std::integral_constant<int, SHIFTED>());
+  return of(std::integral_constant<int, SINGLE>());
 }
 
 template <typename T, bool E4M3>
 int dispatch_rms(RmsParams p, cudaStream_t stream) {
   constexpr int E = Elem<T>::kPerVec;
-  bool fast = p.n % E == 0 && at16(p.x) && at16(p.w) && p.stride_x % E == 0;
-  if (p.residual) fast = fast && at16(p.residual) && p.stride_residual % E == 0;
-  if (p.residual_out) fast = fast && at16(p.residual_out) && p.stride_residual_out % E == 0;
-  if (E4M3) fast = fast && reinterpret_cast<uintptr_t>(p.out) % E == 0 && p.stride_out % E == 0;
-  else fast = fast && at16(p.out) && p.stride_out % E == 0;
+  // whether all rows of a tensor start where x's do, modulo the vector; `bytes` per element
+  auto with_x = [&](const void* t, int64_t stride, int bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t), x = reinterpret_cast<uintptr_t>(p.x);
+    return at % bytes == 0 && (at / bytes - x / sizeof(T)) % E == 0 && (stride - p.stride_x) % E == 0;
+  };
+  bool together = reinterpret_cast<uintptr_t>(p.x) % sizeof(T) == 0 && at16(p.w);
+  if (p.residual) together = together && with_x(p.residual, p.stride_residual, sizeof(T));
+  if (p.residual_out) together = together && with_x(p.residual_out, p.stride_residual_out, sizeof(T));
+  together = together && with_x(p.out, p.stride_out, E4M3 ? 1 : sizeof(T));
+  const bool aligned = p.n % E == 0 && at16(p.x) && p.stride_x % E == 0;
+  const Spread spread = together && aligned ? ALIGNED
+                        : together && p.n <= kMaxShifted ? SHIFTED : SINGLE;
 
-  // 32 values per thread are what 1024 threads have registers for
-  if (p.n > 1024 * 32)
-    return fail(NB200_E_UNSUPPORTED, "rmsnorm: rows of %d elements (at most 32768)", p.n);
-  const int64_t vectors = cdiv64(p.n, E);
+  if (p.n > kMaxColumns)
+    return fail(NB200_E_UNSUPPORTED, "rmsnorm: rows of %d elements (at most %d)", p.n, kMaxColumns);
+  const int64_t vectors = spread == SHIFTED ? (p.n >= E ? p.n / E : 1) : cdiv64(p.n, E);
   int items = 1;
-  p.threads = 32;
   // Few rows: as many threads as there are vectors, the row's latency counts (8 rows of 4096 bf16:
   // 2.7 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
-  // rows of 4096 fp16: 49.7 us with one, 41.5 with two, 40.2 with four).
-  const int most = p.rows >= 2 * device_info().sm_count ? 4 : 1;
-  while ((int64_t)p.threads * items < vectors) {
-    if (items < most) items *= 2;
-    else if (p.threads < 1024) p.threads *= 2;
-    else items *= 2;
-  }
+  // rows of 4096 fp16: 49.7 us with one, 41.5 with two, 40.2 with four; of 4097: 73 with two, 66).
+  const int most = p.rows < 2 * device_info().sm_count ? 1 : 4;
+  while (32 * items < vectors && items < most) items *= 2;
+  while (1024 * items < vectors) items *= 2;
+  p.threads = 32 * (int)cdiv64(vectors, 32 * items);
   switch (items) {
-    case 1: return launch_rms<T, E4M3, 1>(p, fast, stream);
-    case 2: return launch_rms<T, E4M3, 2>(p, fast, stream);
-    case 4: return launch_rms<T, E4M3, 4>(p, fast, stream);
+    case 1: return launch_rms<T, E4M3, 1>(p, spread, stream);
+    case 2: return launch_rms<T, E4M3, 2>(p, spread, stream);
+    case 4: return launch_rms<T, E4M3, 4>(p, spread, stream);
   }
-  if constexpr (E == 4) return launch_rms<T, E4M3, 8>(p, fast, stream);
+  if constexpr (E == 4) return launch_rms<T, E4M3, 8>(p, spread, stream);
   return fail(NB200_E_INVALID, "rmsnorm: no kernel for %d vectors per thread", items);
 }
 

@@ -105,6 +105,37 @@ def test_rmsnorm_of_strided_and_offset_rows():
         assert (room[:, keep.cuda()] == 7.0).all()          # nothing beside the rows was written
 
 
+@pytest.mark.parametrize("out, group", [(None, 0), (E4M3, 0), (E4M3, 32), (E4M3, 64), (E4M3, 128)])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows, n", [(700, 5), (700, 129), (600, 1003), (400, 5122), (300, 16383)])
+def test_rmsnorm_of_many_odd_rows(rows, n, dtype, out, group):
+    """Rows that start at every remainder of 16 bytes, enough of them for several vectors per thread."""
+    gen = _gen(rows + n)
+    x, residual, w = (_randn(gen, *shape, dtype=dtype) for shape in ((rows, n), (rows, n), (n,)))
+    got = ops.rmsnorm(x, w, residual=residual, eps=1e-5, out_dtype=out, group=group)
+    _check_rms(x, w, residual, got, out, group, 1e-5)
+
+
+@pytest.mark.parametrize("first", [1, 4, 7])
+@pytest.mark.parametrize("n", [17, 256, 1001])
+def test_rmsnorm_of_rows_that_start_alike(first, n):
+    """All tensors off by the same remainder, and nothing beside their rows is written."""
+    gen = _gen(first + n)
+    x, residual = (_randn(gen, 9, n + 16, dtype=BF16)[:, first:first + n] for _ in range(2))
+    w = _randn(gen, n, dtype=BF16)
+    rooms = [torch.full((9, n + 16), 7.0, device="cuda", dtype=BF16) for _ in range(2)]
+    codes = torch.full((9, n + 16), 0x55, device="cuda", dtype=torch.uint8)
+    inside = [t[:, first:first + n] for t in rooms]
+    got = ops.rmsnorm(x, w, residual=residual, eps=1e-5, out=inside[0], residual_out=inside[1])
+    _check_rms(x, w, residual, got, None, 0, 1e-5)
+    got = ops.rmsnorm(x, w, residual=residual, eps=1e-5, out_dtype=E4M3, group=32,
+                      out=codes.view(E4M3)[:, first:first + n])
+    _check_rms(x, w, residual, got, E4M3, 32, 1e-5)
+    beside = torch.ones(n + 16, dtype=torch.bool, device="cuda")
+    beside[first:first + n] = False
+    assert (codes[:, beside] == 0x55).all() and all((t[:, beside] == 7.0).all() for t in rooms)
+
+
 @pytest.mark.parametrize("n", [256, 4096, 1003])
 def test_rmsnorm_over_its_own_inputs(n):
     gen = _gen(n)
