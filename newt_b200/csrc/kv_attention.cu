@@ -257,7 +257,7 @@ struct Shared {
   int64_t q_out[3][RP];
   float most[2][8][RP];                        // the warps' maxima, alternating by tile
   float sum[2][8][RP];                         // the warps' row sums, alternating by item
-  float4 step[8][RP];                          // a warp's own: a row's reference, what the sums and the tile are scaled by
+  float step[8][3][RP];                        // a warp's own: a row's reference, negative, and what the sums and the tile are scaled by
   uint64_t full[S::kSlots], empty[S::kSlots], scale_full[4];
   uint64_t q_full[2], s_full[2], most_full[2], p_full, o_full, sum_full;
   uint32_t tmem_slot, abort_flag;
@@ -568,13 +568,29 @@ __global__ void __launch_bounds__(kThreads, 2)
     T* last_out = nullptr;
     int last_part = 0;
     bool last_direct = false;
-    float acc[RH], now[RH];          // of this half's rows and this thread's column
-    float l[RP];                     // of this thread's tokens
+    using Pair = unsigned long long;  // of two rows' numbers
+    Pair acc[RH / 2];                // of this half's rows and this thread's column
+    Pair l[RP / 2];                  // of this thread's tokens
     float m = -INFINITY;             // the reference of row lane % RP, log2 units
 #pragma unroll
-    for (int r = 0; r < RP; ++r) l[r] = 0.0f;
+    for (int r = 0; r < RP / 2; ++r) l[r] = 0;
 #pragma unroll
-    for (int i = 0; i < RH; ++i) acc[i] = now[i] = 0.0f;
+    for (int i = 0; i < RH / 2; ++i) acc[i] = 0;
+    const Pair sixteenth = pack2(0.0625f, 0.0625f);
+    // pairs of RP or RH numbers in shared memory
+    auto pairs_of = [](const float* from, auto& to) {
+      constexpr int n = sizeof(to) / sizeof(to[0]);
+      if constexpr (n % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < n; i += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(from + 2 * i);
+          to[i] = two.x;
+          to[i + 1] = two.y;
+        }
+      } else {
+        to[0] = *reinterpret_cast<const Pair*>(from);
+      }
+    };
 
     for (int item = 0, j = 0; ok; ++item) {
       // one item, as much of it as the share has; or none any more, and the last one's end
@@ -593,7 +609,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int k = 0; k < n && ok; ++k) {
         const int x = j & 1;
         const int t0 = tile_start(p, c.seq, c.at.tile + k), token = t0 + tid;
-        float s[RP], inv_vs = 0.0f;
+        Pair s[RP / 2];
+        float inv_vs = 0.0f;
         bool there = true;
         if (more) {
           const int step = j >> step_shift;
@@ -602,10 +619,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after_sync();
-          uint32_t raw[N];
+          // eight rows' products at a time: more do not fit the registers
+          constexpr int ROWS = RP < 8 ? RP : 8;
+          uint32_t raw[PARTS][ROWS];
+          auto fetch = [&](int first) {
 #pragma unroll
-          for (int i = 0; i < N; i += 16)
-            tmem_ld_32x32(tmem + lane_base + (x * H + half) * N + i, *reinterpret_cast<uint32_t (*)[16]>(&raw[i]));
+            for (int part = 0; part < PARTS; ++part)
+              tmem_ld_few(tmem + lane_base + (x * H + half) * N + part * RP + first, raw[part]);
+          };
+          fetch(0);
           // every query sees the whole tile: no masks but whether the page is there
           const bool clean = t0 + kTile <= c.seq.limit && t0 + kTile - 1 <= c.seq.len - p.nq &&
                              (!p.window || t0 > c.seq.len - 1 - p.window || t0 + kTile <= p.sinks);
@@ -613,49 +635,51 @@ __global__ void __launch_bounds__(kThreads, 2)
           inv_vs = scale.z;
           // seen by some query, and its page is there
           there = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
-          float factor[RP];
+          Pair factor[RP / 2];
+          pairs_of(sh.q_factor[item & 1], factor);
+          const Pair ks = pack2(scale.x, scale.x), log_vs = pack2(scale.y, scale.y);
 #pragma unroll
-          for (int r = 0; r < RP; r += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(&sh.q_factor[item & 1][r]);
-            factor[r] = f.x;
-            factor[r + 1] = f.y;
-            factor[r + 2] = f.z;
-            factor[r + 3] = f.w;
-          }
-          tmem_ld_wait(raw);
+          for (int first = 0; first < RP; first += ROWS) {
+            if (first > 0) fetch(first);
+            tmem_ld_wait();
 #pragma unroll
-          for (int r = 0; r < RP; ++r) {
-            float v = __uint_as_float(raw[(PARTS - 1) * RP + r]);
+            for (int part = 0; part < PARTS; ++part) keep_behind(raw[part]);
+            auto product = [&](int part, int r) { return pack2(__uint_as_float(raw[part][2 * r]), __uint_as_float(raw[part][2 * r + 1])); };
 #pragma unroll
-            for (int part = PARTS - 2; part >= 0; --part)
-              v = fmaf(v, 0.0625f, __uint_as_float(raw[part * RP + r]));
-            // a row that only pads has a product of zero and is as good as any: nobody reads it
-            s[r] = fmaf(v, factor[r] * scale.x, scale.y);
+            for (int r = 0; r < ROWS / 2; ++r) {
+              Pair v = product(PARTS - 1, r);
+#pragma unroll
+              for (int part = PARTS - 2; part >= 0; --part) v = fma2(v, sixteenth, product(part, r));
+              // a row that only pads has a product of zero and is as good as any: nobody reads it
+              s[first / 2 + r] = fma2(v, mul2(factor[first / 2 + r], ks), log_vs);
+            }
           }
           if (!there) {
 #pragma unroll
-            for (int r = 0; r < RP; ++r) s[r] = -INFINITY;
+            for (int r = 0; r < RP / 2; ++r) s[r] = pack2(-INFINITY, -INFINITY);
           }
           if (!clean) {                          // tokens that some rows do not see
             const int* at = sh.q_at[item & 1];
+            auto seen = [&](int r) { return token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks); };
 #pragma unroll
-            for (int r = 0; r < RP; ++r) {
-              const bool seen = token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks);
-              if (!seen) s[r] = -INFINITY;
+            for (int r = 0; r < RP / 2; ++r) {
+              float a, b;
+              unpack2(s[r], a, b);
+              s[r] = pack2(seen(2 * r) ? a : -INFINITY, seen(2 * r + 1) ? b : -INFINITY);
             }
           }
-          float w[RP];
 #pragma unroll
-          for (int r = 0; r < RP; ++r) w[r] = warp_max(s[r]);
-          if (lane == 0) {
-#pragma unroll
-            for (int r = 0; r < RP; r += 4)
-              *reinterpret_cast<float4*>(&sh.most[x][warp - kSoftmaxWarp][r]) = make_float4(w[r], w[r + 1], w[r + 2], w[r + 3]);
-            mbar_arrive(smem_u32(&sh.most_full[x]));
+          for (int r = 0; r < RP; r += 4) {
+            float a, b, c0, d;
+            unpack2(s[r / 2], a, b);
+            unpack2(s[r / 2 + 1], c0, d);
+            const float4 w = make_float4(warp_max(a), warp_max(b), warp_max(c0), warp_max(d));
+            if (lane == 0) *reinterpret_cast<float4*>(&sh.most[x][warp - kSoftmaxWarp][r]) = w;
           }
+          if (lane == 0) mbar_arrive(smem_u32(&sh.most_full[x]));
         }
         // while the warps' maxima get together, the product of the tile before joins the sums with
-        // the factors that its own step left in `now`
+        // the factors of its own step
         if (k + item > 0) {
           ok = mbar_wait(smem_u32(&sh.o_full), (j - 1) & 1, ctx, ST_KV_O, j);
           ok = __all_sync(0xffffffffu, ok);
@@ -668,12 +692,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           tmem_ld_wait();
 #pragma unroll
           for (int part = 0; part < PARTS; ++part) keep_behind(raw[part]);
+          Pair old[RH / 2], fresh[RH / 2];
+          pairs_of(&sh.step[warp - kSoftmaxWarp][1][half * RH], old);
+          pairs_of(&sh.step[warp - kSoftmaxWarp][2][half * RH], fresh);
 #pragma unroll
-          for (int i = 0; i < RH; ++i) {
-            float v = __uint_as_float(raw[PARTS - 1][i]);
+          for (int i = 0; i < RH / 2; ++i) {
+            auto product = [&](int part) { return pack2(__uint_as_float(raw[part][2 * i]), __uint_as_float(raw[part][2 * i + 1])); };
+            Pair v = product(PARTS - 1);
 #pragma unroll
-            for (int part = PARTS - 2; part >= 0; --part) v = fmaf(v, 0.0625f, __uint_as_float(raw[part][i]));
-            acc[i] = fmaf(v, now[i], acc[i]);
+            for (int part = PARTS - 2; part >= 0; --part) v = fma2(v, sixteenth, product(part));
+            acc[i] = fma2(v, fresh[i], mul2(acc[i], old[i]));
           }
           if (k == 0) {                          // of the item before: its end
             const int of = item - 1;
@@ -683,21 +711,25 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int i = 0; i < RH; ++i) {
               const int r = half * RH + i;
+              float even, odd;
+              unpack2(acc[i / 2], even, odd);
+              const float total = i % 2 ? odd : even;
               float sum = 0.0f;
 #pragma unroll
               for (int w = 0; w < 8; ++w) sum += sh.sum[of & 1][w][r];
               if (last_direct) {
                 const int64_t at = sh.q_out[of % 3][r];
                 if (me < D && at >= 0)
-                  last_out[at] = Elem<T>::from_f32(sum > 0.0f ? __fdividef(acc[i], sum) : acc[i] * 0.0f);   // nothing seen: 0
+                  last_out[at] = Elem<T>::from_f32(sum > 0.0f ? __fdividef(total, sum) : total * 0.0f);   // nothing seen: 0
               } else {
-                if (me < D) p.parts[(last_part + r) * D + me] = acc[i];
+                if (me < D) p.parts[(last_part + r) * D + me] = total;
                 if (quarter == 0 && lane == r) p.marks[last_part + r] = make_float2(m, sum);
               }
-              acc[i] = 0.0f;
             }
 #pragma unroll
-            for (int r = 0; r < RP; ++r) l[r] = 0.0f;
+            for (int i = 0; i < RH / 2; ++i) acc[i] = 0;
+#pragma unroll
+            for (int r = 0; r < RP / 2; ++r) l[r] = 0;
             m = -INFINITY;
           }
         }
@@ -715,27 +747,36 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
           for (int o = RP; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const float mt = top - kProbLog2, both = fmaxf(m, mt), ref = both == -INFINITY ? 0.0f : both;
-          if (lane < RP)
-            sh.step[warp - kSoftmaxWarp][r] = make_float4(mt == -INFINITY ? 0.0f : mt, exp2_approx(m - ref), exp2_approx(mt - ref), 0.0f);
+          __syncwarp();                            // everyone has read the last tile's
+          if (lane < RP) {
+            auto& mine = sh.step[warp - kSoftmaxWarp];
+            mine[0][r] = mt == -INFINITY ? 0.0f : -mt;
+            mine[1][r] = exp2_approx(m - ref);
+            mine[2][r] = exp2_approx(mt - ref);
+          }
           m = both;
           __syncwarp();
         }
-        const float4* row_step = sh.step[warp - kSoftmaxWarp];
+        const auto& row_step = sh.step[warp - kSoftmaxWarp];
         // probabilities (0 where the row sees nothing of the tile), rounded to fp16, in parts
         uint32_t bytes[PARTS][RP / 4];
+        Pair less[RP / 2], old[RP / 2], fresh[RP / 2];
+        pairs_of(row_step[0], less);
+        pairs_of(row_step[1], old);
+        pairs_of(row_step[2], fresh);
+        const Pair inv = pack2(inv_vs, inv_vs);
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float4 f = row_step[r];
-          s[r] = exp2_approx(s[r] - f.x);
-          l[r] = fmaf(s[r] * inv_vs, f.z, l[r] * f.y);
-        }
-#pragma unroll
-        for (int r = 0; r < RP; r += 2) {
-          __half2 pair = __floats2half2_rn(s[r], s[r + 1]);
+        for (int r = 0; r < RP / 2; ++r) {
+          float a, b;
+          unpack2(add2(s[r], less[r]), a, b);
+          a = exp2_approx(a);
+          b = exp2_approx(b);
+          l[r] = fma2(mul2(pack2(a, b), inv), fresh[r], mul2(l[r], old[r]));
+          __half2 pair = __floats2half2_rn(a, b);
 #pragma unroll
           for (int part = 0; part < PARTS; ++part) {
             const uint32_t q = split2(pair);
-            if (r % 4 == 0) bytes[part][r / 4] = q; else bytes[part][r / 4] |= q << 16;
+            if (r % 2 == 0) bytes[part][r / 2] = q; else bytes[part][r / 2] |= q << 16;
           }
         }
         // the token's row of P: N bytes, 16 at a time
@@ -766,26 +807,24 @@ __global__ void __launch_bounds__(kThreads, 2)
 
         if (stage_next && k == 0) stage(next, item + 1);
 
-#pragma unroll
-        for (int i = 0; i < RH; ++i) {
-          const float4 f = row_step[half * RH + i];
-          acc[i] *= f.y;
-          now[i] = f.z;
-        }
-        __syncwarp();                            // before the next tile's steps are written
         ++j;
       }
       if (!ok || !more) break;
       // the row sums over the tokens' threads, on their way
+      float sums[RP];
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
+      for (int r = 0; r < RP; r += 2) {
+        unpack2(l[r / 2], sums[r], sums[r + 1]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+        for (int o = 16; o > 0; o >>= 1) {
+          sums[r] += __shfl_xor_sync(0xffffffffu, sums[r], o);
+          sums[r + 1] += __shfl_xor_sync(0xffffffffu, sums[r + 1], o);
+        }
       }
       if (lane == 0) {
 #pragma unroll
         for (int r = 0; r < RP; r += 4)
-          *reinterpret_cast<float4*>(&sh.sum[item & 1][warp - kSoftmaxWarp][r]) = make_float4(l[r], l[r + 1], l[r + 2], l[r + 3]);
+          *reinterpret_cast<float4*>(&sh.sum[item & 1][warp - kSoftmaxWarp][r]) = make_float4(sums[r], sums[r + 1], sums[r + 2], sums[r + 3]);
         mbar_arrive(smem_u32(&sh.sum_full));
       }
       last_out = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + (int64_t)c.at.head * p.group * p.o_head_stride + me;
