@@ -252,9 +252,9 @@ struct Shared {
   float4 scale[4][32];                         // of a step's pages: ks, log2 vs, 1 / vs, 1 if it is there
   float q_factor[2][RP];                       // what takes a row's product to log2 units
   int q_at[2][RP];                             // position of the row's query; -1: no such row
-  // where its output is in its sequence and head; -1: no such row.  Three turns: an item's are read
-  // while the one after the next is staged.
-  int64_t q_out[3][RP];
+  // where its output is in its sequence and head; -1: no such row.  Four turns: an item's are read
+  // by the end of the next one's first maxima, when a warp ahead may be staging two items further.
+  int64_t q_out[4][RP];
   float most[2][8][RP];                        // the warps' maxima, alternating by tile
   float sum[2][8][RP];                         // the warps' row sums, alternating by item
   float step[8][3][RP];                        // a warp's own: a row's reference, negative, and what the sums and the tile are scaled by
@@ -552,15 +552,22 @@ __global__ void __launch_bounds__(kThreads, 2)
     Queries<T, D, RP, PARTS> queries;
     auto stage = [&](const Cursor& at, int of) {
       stage_queries<T, D, RP, PARTS>(p, queries.raw, at.seq.len - p.nq, at.at.row_tile, tid, sh.q[of & 1],
-                                     sh.q_factor[of & 1], sh.q_at[of & 1], sh.q_out[of % 3]);
+                                     sh.q_factor[of & 1], sh.q_at[of & 1], sh.q_out[of & 3]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[of & 1]));
+    };
+    auto load_behind = [&](const Cursor& at) {     // the queries of the item behind this one, if it is ours
+      if (at.left <= at.seq.count - at.at.tile) return;
+      Cursor behind = at;
+      behind.advance(p, at.seq.count - at.at.tile);
+      queries.load(p, behind, tid);
     };
     if (c.left > 0) {
       queries.load(p, c, tid);
       stage(c, 0);
       named_barrier_sync(1, 256);    // the rows' factors and positions are written
+      load_behind(c);
     }
 
     // An item is finished behind the first maxima of the next one, where its last product has long
@@ -598,12 +605,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!more && item == 0) break;
       const int to_end = more ? c.seq.count - c.at.tile : 0;
       const int n = more ? min(to_end, c.left) : 1;
-      // the next item's queries are loaded now and staged behind this one's first tile
+      // The next item's queries are staged before this one's first tile, so that its products follow this
+      // one's without a pause, and the ones behind it are loaded.  Where they go, the item before has
+      // been read from: all warps' maxima of its last tile were there.
       const bool stage_next = more && c.left > to_end;
       Cursor next = c;
       if (stage_next) {
         next.advance(p, to_end);
-        queries.load(p, next, tid);
+        stage(next, item + 1);
+        load_behind(next);
       }
 #pragma unroll 1
       for (int k = 0; k < n && ok; ++k) {
@@ -718,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
               for (int w = 0; w < 8; ++w) sum += sh.sum[of & 1][w][r];
               if (last_direct) {
-                const int64_t at = sh.q_out[of % 3][r];
+                const int64_t at = sh.q_out[of & 3][r];
                 if (me < D && at >= 0)
                   last_out[at] = Elem<T>::from_f32(sum > 0.0f ? __fdividef(total, sum) : total * 0.0f);   // nothing seen: 0
               } else {
@@ -804,8 +814,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
-
-        if (stage_next && k == 0) stage(next, item + 1);
 
         ++j;
       }
