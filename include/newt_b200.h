@@ -301,8 +301,8 @@ int nb200_attention_fwd(const void* q, const void* k, const void* v, void* o,
  * 16/32-bit outputs.  `residual_out` (null: not wanted): h in `dtype`.  One rounding per output.
  * `out` and `residual_out` may be the very tensors x and residual (same base and strides); no
  * other overlap.  Rows of up to 32768 elements, any alignment (16-byte aligned rows of whole vectors
- * are faster).  Beside nb200_layernorm; the reference has no
- * counterpart with a residual or an 8-bit output. */
+ * are faster).  Beside nb200_layernorm; the reference has no counterpart with a residual or an 8-bit
+ * output. */
 int nb200_rmsnorm(const void* x, const void* residual, const void* w, void* out, void* residual_out,
                   float* scales, int64_t rows, int64_t n, int64_t stride_x, int64_t stride_residual,
                   int64_t stride_out, int64_t stride_residual_out, int64_t stride_scales,
@@ -356,7 +356,8 @@ int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const void* v, i
  * significant bits.
  * `workspace`: 16-byte aligned device memory of at least nb200_kv_attention_workspace_bytes(...)
  * bytes (0: none is needed, sequences of so few pages are never cut), the caller's; nothing in it
- * needs clearing, and it must not be shared by launches that can overlap on the GPU.  The lengths stay on the device, so a captured call replays with new ones.
+ * needs clearing, and it must not be shared by launches that can overlap on the GPU (two captured
+ * graphs among them).  The lengths stay on the device, so a captured call replays with new ones.
  * Beside nb200_attention_fwd; the reference has no cache. */
 int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cache, int64_t batch,
                                            int64_t queries, int64_t heads, int64_t max_pages,

@@ -12,15 +12,17 @@
 //   O^T [head_dim  x N]  = V tile (MN-major, as it lies) x P parts [N x 128 tokens]
 // and the other operand, which is small, is split into sums of e4m3 numbers that fill N columns:
 // a bf16 has 8 significant bits and is exactly hi + lo / 16 of two e4m3 (4 bits each, and what the
-// first rounding leaves over fits the second), an fp16 takes three.  So the queries lose nothing,
-// and the probabilities keep 9 or 14 bits.  N = parts * rows, at least 16, was idle anyway.
+// first rounding leaves over fits the second), an fp16 takes three.  So the queries lose nothing; the
+// probabilities are rounded to fp16 and keep 9 bits (two parts) or 11 (three): as many as the output
+// has, one more for bf16.  N = parts * rows, at least 16, was idle anyway.
 //
-// Per tile of 128 tokens a thread owns one token: it reads its N scores from tensor memory, applies
-// both scales and the masks, and takes part in the rows' maxima over the tile (warp reductions and
-// one exchange through shared memory).  Probabilities are relative to the tile's own maximum
-// (of s + log2 vs, so that they fit e4m3 whatever the scales); the tile's product is read back --
-// now a thread owns one of the head's columns -- and joins the running sums in registers with the
-// usual rescaling, in fp32.  P is laid out so that a thread writes its token's N bytes in one piece.
+// Per tile of 256 tokens each of 256 threads owns one token: it reads its N scores from tensor memory,
+// applies both scales and the masks, and takes part in the rows' maxima over the tile (warp reductions
+// and one exchange through shared memory, on a barrier of its own).  Probabilities are relative to the
+// tile's own maximum (of s + log2 vs, so that they fit e4m3 whatever the scales).  While the maxima of
+// one tile get together, the product of the tile before is read back -- now a thread owns one of the
+// head's columns and half of the rows -- and joins the running sums in registers with the usual
+// rescaling, in fp32.  P is laid out so that a thread writes its token's N bytes in one piece.
 //
 // Value rows that no query sees are cleared in shared memory before the product: their weight is
 // zero, but zero times a NaN that was left in a page would not be.
@@ -30,8 +32,16 @@
 // chip.  A share may start and end inside an item; such parts leave their sums in the workspace and
 // a second kernel joins them, in token order.  Lengths are read on the device, so a captured call
 // follows them.
-
-#include <type_traits>
+//
+// What bounds it: HBM where there is enough of it to do (64 sequences of 4 to 8 thousand tokens, 8 key
+// heads of 128 in bf16: 134 us, 6.1 TB/s; the sums of 16 rows a key head in fp16 keep the softmax
+// threads busier than HBM: 31 sequences of 11 to 22 thousand tokens, 28 rows, 90 us, a fifth of HBM's
+// rate, with issue slots half used and the rest spent on the exchange of the maxima); below some 20 us
+// the chain length -> page -> tile -> scores -> probabilities -> sums, 8.3 us for one short sequence.
+// Two CTAs per SM hide one's exchange behind the other's arithmetic.  Measured on the way, the first of
+// these cases: a thread per score without tensor cores 9463 us, tiles of 128 tokens with four softmax
+// warps 191, pages and scales looked up two steps ahead and products joined a tile later 140, tiles of
+// 256 tokens with eight warps 134.
 
 #include "elem.cuh"
 #include "kv_cache.cuh"
@@ -49,7 +59,7 @@ constexpr int kSmemPerCta = 106 * 1024;
 constexpr int kThreads = 320;            // producer, issuer, eight softmax warps
 constexpr int kSoftmaxWarp = 2;
 constexpr int kJoinThreads = 256;
-constexpr int kJoinTiles = 3;
+constexpr int kWholeTiles = 3, kJoinTiles = 2;   // see whole_items
 constexpr int kMaxShares = 320;          // two CTAs on each of 148 SMs
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastScale = 8.67361738e-19f;   // 2^-60
@@ -154,12 +164,14 @@ struct WorkList {
   __device__ int tiles() const { return total * per_seq; }
 
   // Shares of whole items, or of tiles?  Joining the parts of cut items costs about as much as
-  // kJoinTiles tiles: whole items where the longest share of them is no longer than that, and always
-  // where every item is that short (the host counts on it: can_be_cut).
+  // kJoinTiles tiles: whole items where the longest share of them is no longer than that (1 sequence of
+  // 1000 tokens, 8 key heads of 4 tiles: cut 10.7 us, whole 14.0).  Always whole where every item has
+  // up to kWholeTiles: the host then leaves out the joining launch (can_be_cut; 32 sequences of 700
+  // tokens: whole 16.5 us, cut 18.5; 1 of 600: 10.8 and 12.7).
   __device__ int tile_share(const KvAttnParams& p) const { return (tiles() + p.shares - 1) / p.shares; }
   __device__ bool whole_items(const KvAttnParams& p) const {
     const long long items = (p.batch * per_seq + p.shares - 1) / p.shares;
-    return largest <= kJoinTiles || items * largest <= tile_share(p) + kJoinTiles;
+    return largest <= kWholeTiles || items * largest <= tile_share(p) + kJoinTiles;
   }
 
   // first tile of share c, from 0 to tiles(); the same c in all lanes
@@ -977,7 +989,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
 // ---- host ------------------------------------------------------------------------------------------
 
 // Can a sequence of this many pages be long enough for its items to be cut?
-bool can_be_cut(int64_t pages, int64_t page) { return cdiv64(pages * page, kTile) > kJoinTiles; }
+bool can_be_cut(int64_t pages, int64_t page) { return cdiv64(pages * page, kTile) > kWholeTiles; }
 
 int row_tile_of(int64_t rows) {
   int rp = 4;
@@ -1040,7 +1052,7 @@ extern "C" int64_t nb200_kv_attention_workspace_bytes(const nb200_kv_cache* cach
                                                       int64_t queries, int64_t heads,
                                                       int64_t max_pages, int dtype) {
   if (!cache || cache->heads <= 0 || batch <= 0 || queries <= 0 || heads <= 0) return 0;
-  if (!can_be_cut(max_pages, cache->page_size)) return 0;
+  if ((dtype != NB200_F16 && dtype != NB200_BF16) || !can_be_cut(max_pages, cache->page_size)) return 0;
   const int rp = row_tile_of(queries * (heads / cache->heads));
   return 2ll * shares_of() * rp * (cache->head_dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }

@@ -345,12 +345,15 @@ def _check_attention(got, q, cache, table, lengths, scale=None, window=0, sinks=
     d = q.shape[3]
     scale = d ** -0.5 if scale is None else scale
     want, size = _attend_exact(q, cache, table, lengths, scale, window, sinks)
-    # Before the last rounding: a probability has 9 (bf16) or 14 (fp16) significant bits, so it is
-    # off by 2^-9 or 2^-14 of itself; a score is an fp32 sum of d products, off by at most
-    # d 2^-24 sum |q k| scale < 2^-11 for the inputs below, and so is its exponential; a
-    # probability below 2^-22 of its 128 tokens' largest may be lost.  All are relative to the
-    # mean magnitude of the values seen.
-    extra = {BF16: 2.0 ** -9, FP16: 2.0 ** -14}[q.dtype] + 2.0 ** -11 + 2.0 ** -15
+    # Before the last rounding, relative to the mean magnitude of the values seen:
+    # - a probability in [1, 2) times a power of two is rounded to fp16: half a step is 2^-11.  For
+    #   bf16 two e4m3 parts hold it: the first leaves up to half its step, 2^-4, and the second up to
+    #   half the step of a number below 2^-4, which is 2^-9.  For fp16 three parts of 4 bits hold the
+    #   11 bits exactly.
+    # - a score is an fp32 sum of d products, off by at most d 2^-24 sum |q k| scale < 2^-11 for the
+    #   inputs below, and so is its exponential;
+    # - a probability below 2^-22 of its 256 tokens' largest may be lost: 256 of them are 2^-14.
+    extra = {BF16: 2.0 ** -9 + 2.0 ** -11, FP16: 2.0 ** -11}[q.dtype] + 2.0 ** -11 + 2.0 ** -14
     off = (got.double() - want).abs() - (HALF[q.dtype] * want.abs() + extra * size + TINY[q.dtype])
     assert not torch.isnan(off).any()
     assert off.max().item() <= 0.0, off.max().item()
