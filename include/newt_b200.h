@@ -352,6 +352,7 @@ int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const void* v, i
  * j > position - window (`window` 0: all) or j < sinks.  A query that sees nothing (a sequence
  * shorter than `queries`, an empty one) gives zeros.  Tokens whose page is missing from the table
  * are not seen.  What lies in page rows that no query of the call sees has no effect, NaN included.
+ * `out` must not overlap q.
  * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 11 (fp16)
  * significant bits.
  * `workspace`: 16-byte aligned device memory of at least nb200_kv_attention_workspace_bytes(...)

@@ -265,8 +265,10 @@ extern "C" int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const
   if (tokens == 0 || batch == 0 || max_new == 0 || max_pages == 0 || cache->pages == 0) return 0;
   if (!k || !v || !page_table || !starts || !offsets)
     return fail(NB200_E_INVALID, "kv append: null tensor pointer");
-  // a run of max_new tokens touches at most this many pages
-  const int64_t slots = (max_new + cache->page_size - 2) / cache->page_size + 1;
+  if (max_new > tokens) max_new = tokens;
+  // a run of max_new tokens touches at most this many pages, of max_pages that there are
+  int64_t slots = (max_new + cache->page_size - 2) / cache->page_size + 1;
+  if (slots > max_pages) slots = max_pages;
   if (batch * slots > INT32_MAX || cache->heads * 2 > 65535)
     return fail(NB200_E_UNSUPPORTED, "kv append: %lld sequences of up to %lld pages, %lld heads", (long long)batch,
                 (long long)slots, (long long)cache->heads);

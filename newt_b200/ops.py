@@ -105,6 +105,13 @@ def _rows(name, t, shape, dtype):
         _refuse(name, t, shape, dtype)
 
 
+def _written(name, t, shape, dtype):
+    """The same for a tensor that a kernel writes: no two elements in one place."""
+    _rows(name, t, shape, dtype)
+    if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(shape, t.stride())):
+        raise ValueError(f"'{name}' has elements that share their memory (strides {t.stride()})")
+
+
 def _vector(name, t, length, dtype):
     if t.shape != (length,) or t.dtype is not dtype or not t.is_contiguous():
         _refuse(name, t, (length,), dtype)
@@ -143,7 +150,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
     if out is None:
         out = _fresh(x, out_dtype)
     else:
-        _rows("out", out, shape, out_dtype)
+        _written("out", out, shape, out_dtype)
     scale_stride = residual_stride = residual_out_stride = 0
     if out_dtype is E4M3:
         if group not in (0, 32, 64, 128):
@@ -153,7 +160,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
             scales = x.new_empty((rows, columns), dtype=torch.float32)
             scale_stride = columns
         else:
-            _rows("scales", scales, (rows, columns), torch.float32)
+            _written("scales", scales, (rows, columns), torch.float32)
             scale_stride = scales.stride(0)
     elif group or scales is not None:
         raise ValueError("rmsnorm: scales and groups go with an e4m3 output")
@@ -163,7 +170,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
         if residual_out is None:
             residual_out = _fresh(x, dtype)
         else:
-            _rows("residual_out", residual_out, shape, dtype)
+            _written("residual_out", residual_out, shape, dtype)
         residual_out_stride = residual_out.stride(0)
     elif residual_out is not None:
         raise ValueError("rmsnorm: 'residual_out' goes with a residual")
@@ -254,7 +261,7 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     lengths: int32 [batch], the tokens of each sequence in the cache, the new ones among them: query
     i of sequence b stands at position lengths[b] - queries + i and sees the tokens up to its own,
     with `window` > 0 only the last `window` of them and the first `sinks` of the sequence.  A query
-    that sees nothing gives zeros.  scale: 1 / sqrt(head_dim) if not given."""
+    that sees nothing gives zeros.  scale: 1 / sqrt(head_dim) if not given.  `out` must not be q."""
     packed = _pack_cache(cache)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 4:
@@ -270,7 +277,7 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     if out is None:
         out = _fresh(q, dtype)
     else:
-        _rows("out", out, shape, dtype)
+        _written("out", out, shape, dtype)
     stream = _launch_stream(
         "q page_table lengths out cache.k cache.v cache.k_scales cache.v_scales", q, page_table,
         lengths, out, cache.k, cache.v, cache.k_scales, cache.v_scales)
@@ -339,7 +346,7 @@ def token_logprobs_backward(logits, tokens, lse, entropy, grad_logprob=None, gra
     if out is None:
         out = _fresh(logits, logits.dtype)
     else:
-        _rows("out", out, (rows, vocab), logits.dtype)
+        _written("out", out, (rows, vocab), logits.dtype)
     stream = _launch_stream("logits tokens lse entropy grad_logprob grad_entropy out", logits, tokens,
                             lse, entropy, grad_logprob, grad_entropy, out)
     abi.check(abi.load().nb200_token_logprobs_bwd(

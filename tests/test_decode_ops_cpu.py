@@ -25,7 +25,7 @@ def _append(cache=None, k=P, v=P, tokens=4, table=P, max_pages=4, starts=P, offs
                                       max_pages, starts, offsets, batch, max_new, dtype, None)
 
 
-def _attend(cache=None, q=P, out=P, batch=2, queries=1, heads=4, table=P, max_pages=4, lengths=P,
+def _attend(cache=None, q=P, out=2 * P, batch=2, queries=1, heads=4, table=P, max_pages=4, lengths=P,
             scale=0.125, window=0, sinks=0, dtype=abi.BF16, workspace=P, size=1 << 40):
     return abi.load().nb200_kv_attention(q, cache or _cache(), out, batch, queries, heads, 256, 256,
                                          64, 256, 256, 64, table, 4, max_pages, lengths, scale,
@@ -84,6 +84,7 @@ def _grad(logits=P, tokens=P, lse=P, entropy=P, g=P, ge=P, out=P, rows=2, vocab=
     (lambda: _attend(scale=float("inf")), abi.E_INVALID, "scale"),
     (lambda: _attend(q=None), abi.E_INVALID, "null"),
     (lambda: _attend(lengths=None), abi.E_INVALID, "null"),
+    (lambda: _attend(out=P), abi.E_INVALID, "must not be q"),
     (lambda: _attend(max_pages=1 << 40), abi.E_INVALID, "extent"),
     (lambda: _attend(max_pages=400, workspace=None), abi.E_INVALID, "workspace"),
     (lambda: _attend(max_pages=400, size=1000), abi.E_INVALID, "workspace"),
@@ -154,6 +155,13 @@ def test_python_refuses_tensors_that_are_not_on_the_gpu():
     (ValueError, "stride", lambda x, w, c, kv, t, n, o, q: ops.rmsnorm(torch.zeros(64, 4).t(), w)),
     (ValueError, "residual", lambda x, w, c, kv, t, n, o, q: ops.rmsnorm(x, w, residual_out=x)),
     (ValueError, "shape", lambda x, w, c, kv, t, n, o, q: ops.rmsnorm(x, w, residual=x[:2])),
+    (ValueError, "share", lambda x, w, c, kv, t, n, o, q: ops.rmsnorm(x, w, out=w.expand(4, 64))),
+    (ValueError, "share", lambda x, w, c, kv, t, n, o, q: ops.rmsnorm(
+        x, w, residual=x, residual_out=w.expand(4, 64))),
+    (ValueError, "share", lambda x, w, c, kv, t, n, o, q: ops.kv_attention(
+        q, c, t, n, out=q[:1].expand(2, 1, 4, 64))),
+    (ValueError, "share", lambda x, w, c, kv, t, n, o, q: ops.token_logprobs_backward(
+        x, None, w[:4], w[:4], out=w.expand(4, 64))),
     (ValueError, "'k'", lambda x, w, c, kv, t, n, o, q: ops.kv_append(c, kv[:, :1], kv, t, n, o, 1)),
     (TypeError, "kv_append", lambda x, w, c, kv, t, n, o, q: ops.kv_append(c, kv.float(), kv.float(),
                                                                           t, n, o, 1)),

@@ -780,6 +780,55 @@ def test_the_operators_in_a_graph_and_on_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(after, _step(*args)))
 
 
+def test_two_steps_at_once():
+    """The same operators on two streams, nothing but their inputs in common, with sequences long
+    enough that the attention's parts are joined."""
+    gen = _gen(131)
+    lengths = [5000, 1, 2300]
+    table, total = _pages(gen, [n + 1 for n in lengths], 16)
+    x = _randn(gen, 3, 1003, dtype=BF16)
+    w = _randn(gen, 1003, dtype=BF16)
+    k, v = _randn(gen, 3, 2, 64, dtype=BF16), _randn(gen, 3, 2, 64, dtype=BF16)
+    q = _randn(gen, 3, 1, 8, 64, dtype=BF16)
+    logits = _randn(gen, 3, 50021, dtype=BF16)
+    offsets, tokens, at = _int32([0, 1, 2, 3]), torch.tensor([1, 2, 3], device="cuda"), _int32(lengths)
+    first = _finite_cache(gen, total, 2, 16, 64)
+    caches = [ops.KVCache(*(t.clone() for t in first)) for _ in range(3)]
+    args = lambda i: (at, table, caches[i], x, k, v, q, logits, w, offsets, tokens)
+    want = _step(*args(2))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(20):                          # the append may be repeated
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = _step(*args(i))
+    torch.cuda.synchronize()
+    for outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_calls_with_nothing_to_do():
+    gen = _gen(17)
+    cache = _finite_cache(gen, 4, 2, 16, 64)
+    before = [t.clone() for t in cache]
+    q = _randn(gen, 2, 3, 4, 64, dtype=FP16)
+    none = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    table = _int32([[0, 1], [2, 3]])
+    # no table, no tokens: nothing is seen
+    assert (ops.kv_attention(q, cache, none, _int32([40, 0])) == 0).all()
+    assert (ops.kv_attention(q, cache, table, _int32([0, -3])) == 0).all()
+    assert ops.kv_attention(q[:0], cache, table[:0], _int32([])).shape == (0, 3, 4, 64)
+    k = _randn(gen, 5, 2, 64, dtype=FP16)
+    ops.kv_append(cache, k, k, none, _int32([0, 0]), _int32([0, 2, 5]), 3)
+    ops.kv_append(cache, k, k, table, _int32([0, 0]), _int32([0, 0, 0]), 3)
+    ops.kv_append(cache, k[:0], k[:0], table, _int32([0, 0]), _int32([0, 0, 0]), 3)
+    for t, was in zip(cache, before):
+        assert torch.equal(*((a.view(torch.uint8) if a.dtype == E4M3 else a) for a in (t, was)))
+    # a bound on the new tokens that is far too large costs nothing and changes nothing
+    _check_append(cache, k, k, table, _int32([0, 3]), _int32([0, 2, 5]), 2 ** 31 - 1)
+
+
 def test_a_prompt_and_its_decode_steps():
     """One layer of a decoder, prompt first and then token by token, on the framework's own
     product and the operators here, against the whole sequence at once in 64 bits."""
