@@ -621,8 +621,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       // one's without a pause, and the ones behind it are loaded.  Where they go, the item before has
       // been read from: all warps' maxima of its last tile were there.
       const bool stage_next = more && c.left > to_end;
-      Cursor next = c;
       if (stage_next) {
+        Cursor next = c;                 // worked out again at the item's end: it is not worth its registers
         next.advance(p, to_end);
         stage(next, item + 1);
         load_behind(next);
@@ -850,8 +850,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       last_out = static_cast<T*>(p.out) + c.at.b * p.o_batch_stride + (int64_t)c.at.head * p.group * p.o_head_stride + me;
       last_direct = c.at.tile == 0 && n == to_end;
       last_part = (2 * blockIdx.x + (item == 0 ? 0 : 1)) * RP;    // the share's first or second part
-      c = next;
-      if (!stage_next) c.left = 0;
+      if (stage_next) c.advance(p, to_end);
+      else c.left = 0;
     }
   }
 
