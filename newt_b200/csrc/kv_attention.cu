@@ -69,6 +69,22 @@ enum : unsigned int {
   ST_KV_Q = 32, ST_KV_K, ST_KV_V, ST_KV_EMPTY, ST_KV_SCALES, ST_KV_S, ST_KV_P, ST_KV_O, ST_KV_ZERO, ST_KV_MOST, ST_KV_SUM
 };
 
+// Division of 0 <= n < 2^31 by a d that the host knows: with 2^(s-1) < d <= 2^s and m = floor(2^(31+s) / d) + 1,
+// m d is 2^(31+s) and up to d more, which adds less than 1 / d to n m / 2^(31+s): it is n / d rounded
+// down.  A division by a number in a register is some thirty instructions, and a block begins with
+// half a dozen of them one behind the other.
+struct Divisor {
+  uint32_t m, shift;
+  Divisor() = default;
+  explicit Divisor(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    m = (uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1);
+    shift = 31 + s;
+  }
+  __device__ int divide(int n) const { return (int)(((unsigned long long)(uint32_t)n * m) >> shift); }
+};
+
 struct KvAttnParams {
   const void* q;
   void* out;
@@ -84,6 +100,9 @@ struct KvAttnParams {
   int rows, row_tiles;                   // nq * group, and how many pieces of RP rows
   int pages, page, page_shift, max_pages, window, sinks;
   int shares, q_aligned;
+  int per_seq, stretch;                  // items of a sequence; sequences that a lane of a work list counts
+  int share_items, longer_shares;        // whole items: how many a share has, and how many shares have one more
+  Divisor by_shares, by_per_seq, by_row_tiles, by_stretch;
   float scale;
   unsigned long long wait_limit_ns;
   unsigned int* status;
@@ -133,14 +152,11 @@ struct Place {
 // The work list as one warp sees it: lane i knows how many tiles a stretch of the sequences has and
 // how many come before it.  All lanes take part in every call.
 struct WorkList {
-  int stretch, before, sum;   // of this lane's stretch, for one (key head, row tile)
+  int before, sum;            // of this lane's stretch, for one (key head, row tile)
   int total, largest;         // of all: tiles of one (key head, row tile), most of one sequence
-  int per_seq;
 
   __device__ WorkList(const KvAttnParams& p) {
-    const int lane = threadIdx.x & 31;
-    per_seq = p.row_tiles * p.kv_heads;
-    stretch = (p.batch + 31) / 32;
+    const int lane = threadIdx.x & 31, stretch = p.stretch;
     sum = largest = 0;
 #pragma unroll 1
     for (int i = 0; i < stretch; ++i) {
@@ -161,51 +177,65 @@ struct WorkList {
     total = __shfl_sync(0xffffffffu, run, 31);
     largest = __reduce_max_sync(0xffffffffu, largest);
   }
-  __device__ int tiles() const { return total * per_seq; }
+  __device__ int tiles(const KvAttnParams& p) const { return total * p.per_seq; }
 
   // Shares of whole items, or of tiles?  Joining the parts of cut items costs about as much as
   // kJoinTiles tiles: whole items where the longest share of them is no longer than that (1 sequence of
   // 1000 tokens, 8 key heads of 4 tiles: cut 10.7 us, whole 14.0).  Always whole where every item has
   // up to kWholeTiles: the host then leaves out the joining launch (can_be_cut; 32 sequences of 700
   // tokens: whole 16.5 us, cut 18.5; 1 of 600: 10.8 and 12.7).
-  __device__ int tile_share(const KvAttnParams& p) const { return (tiles() + p.shares - 1) / p.shares; }
+  __device__ int tile_share(const KvAttnParams& p) const { return p.by_shares.divide(tiles(p) + p.shares - 1); }
   __device__ bool whole_items(const KvAttnParams& p) const {
-    const long long items = (p.batch * per_seq + p.shares - 1) / p.shares;
+    const long long items = p.share_items + (p.longer_shares > 0);
     return largest <= kWholeTiles || items * largest <= tile_share(p) + kJoinTiles;
+  }
+
+  // tiles of the sequences before b and of b, of one (key head, row tile); the same b in all lanes
+  __device__ int before_sequence(const KvAttnParams& p, int b, int* count) const {
+    const int owner = p.by_stretch.divide(b);
+    int at = __shfl_sync(0xffffffffu, before, owner);
+    if (p.stretch == 1) {
+      *count = __shfl_sync(0xffffffffu, sum, owner);
+      return at;
+    }
+#pragma unroll 1
+    for (int k = owner * p.stretch; k < b; ++k) at += make_seq(p, __ldg(p.lengths + k)).count;
+    *count = make_seq(p, __ldg(p.lengths + b)).count;
+    return at;
   }
 
   // first tile of share c, from 0 to tiles(); the same c in all lanes
   __device__ int share_start(const KvAttnParams& p, int c) const {
-    if (!whole_items(p)) return (int)min((long long)c * tile_share(p), (long long)tiles());
-    const int items = p.batch * per_seq;
-    const int i = (int)((long long)items * c / p.shares);
-    if (i >= items) return tiles();
-    const int b = i / per_seq, owner = b / stretch;
-    int at = __shfl_sync(0xffffffffu, before, owner);
-#pragma unroll 1
-    for (int k = owner * stretch; k < b; ++k) at += make_seq(p, __ldg(p.lengths + k)).count;
-    return at * per_seq + (i - b * per_seq) * make_seq(p, __ldg(p.lengths + b)).count;
+    if (!whole_items(p)) return (int)min((long long)c * tile_share(p), (long long)tiles(p));
+    const int i = c * p.share_items + min(c, p.longer_shares), b = p.by_per_seq.divide(i);
+    if (b >= p.batch) return tiles(p);
+    int count;
+    const int at = before_sequence(p, b, &count);
+    return at * p.per_seq + (i - b * p.per_seq) * count;
   }
 
   // The place of a tile, 0 <= flat < tiles(), a tile of its own for every lane if need be.
   __device__ Place locate(const KvAttnParams& p, int flat) const {
-    const int q = flat / per_seq;            // at * per_seq <= flat  <=>  at <= flat / per_seq
+    const int q = p.by_per_seq.divide(flat);   // at * per_seq <= flat  <=>  at <= flat / per_seq
     int owner = 0;
 #pragma unroll
     for (int step = 16; step > 0; step >>= 1)
       if (__shfl_sync(0xffffffffu, before, owner + step) <= q) owner += step;
     int at = __shfl_sync(0xffffffffu, before, owner);
-    int b = owner * stretch;
-    int count = make_seq(p, __ldg(p.lengths + b)).count;
-#pragma unroll 1
-    while (q >= at + count) {
-      at += count;
-      ++b;
+    int b = owner * p.stretch;
+    int count = __shfl_sync(0xffffffffu, sum, owner);
+    if (p.stretch > 1) {
       count = make_seq(p, __ldg(p.lengths + b)).count;
+#pragma unroll 1
+      while (q >= at + count) {
+        at += count;
+        ++b;
+        count = make_seq(p, __ldg(p.lengths + b)).count;
+      }
     }
-    flat -= at * per_seq;
-    const int item = flat / count;
-    return Place{b, item / p.row_tiles, item % p.row_tiles, flat % count};
+    flat -= at * p.per_seq;
+    const int item = flat / count, head = p.by_row_tiles.divide(item);
+    return Place{b, head, item - head * p.row_tiles, flat - item * count};
   }
 };
 
@@ -439,21 +469,18 @@ __global__ void __launch_bounds__(kThreads, 2)
       k_scale = page >= 0 ? __ldg(p.k_scales + page * p.k_scale_stride + of_head) : 0.0f;
       v_scale = page >= 0 ? __ldg(p.v_scales + page * p.v_scale_stride + of_head) : 1.0f;
     };
-    if (c.left > 0) mine.advance(p, my_tile);
+    auto next_step = [&](int& page, int& of_head) {
+      if (mine.left > 0) mine.advance(p, step_tiles);
+      page = page_of(mine);
+      of_head = mine.at.head;
+    };
+    if (c.left > 0 && my_tile > 0) mine.advance(p, my_tile);
     id[0] = page_of(mine);
     head[0] = mine.at.head;
-    if (mine.left > 0) mine.advance(p, step_tiles);
-    id[1] = page_of(mine);
-    head[1] = mine.at.head;
     fetch_scales(id[0], head[0], ks[0], vs[0]);
     bool ok = true;
     int left = c.left;
     for (int step = 0; left > 0 && ok; ++step) {
-      // the next step's scales and the one after's pages are under way while this one is issued
-      fetch_scales(id[1], head[1], ks[1], vs[1]);
-      if (mine.left > 0) mine.advance(p, step_tiles);
-      id[2] = page_of(mine);
-      head[2] = mine.at.head;
       bool handed = false;
 #pragma unroll 1
       for (int k = 0; k < step_tiles && left > 0 && ok; ++k, --left) {
@@ -480,6 +507,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&sh.scale_full[step & 3]));
           handed = true;
+          // the next step's scales and the one after's pages are under way while this one is issued
+          if (step == 0) next_step(id[1], head[1]);
+          fetch_scales(id[1], head[1], ks[1], vs[1]);
+          next_step(id[2], head[2]);
         }
       }
       id[0] = id[1];
@@ -887,7 +918,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttnParam
     // in the order of the boundaries, so that every block has the same list
     for (int c0 = 0; c0 < p.shares - 1; c0 += kJoinThreads) {
       const int c = c0 + tid;
-      const int flat = (int)min((c + 1ll) * share, (long long)list.tiles() - 1);
+      const int flat = (int)min((c + 1ll) * share, (long long)list.tiles(p) - 1);
       const Place w = list.locate(p, flat);
       const bool mine = c < p.shares - 1 && flat == (c + 1ll) * share && w.tile > 0 && (flat - w.tile) / share == c;
       const uint32_t in_warp = __ballot_sync(0xffffffffu, mine);
@@ -1116,6 +1147,8 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   p.rows = (int)queries * p.group;
   const int rp = row_tile_of(p.rows);
   p.row_tiles = (p.rows + rp - 1) / rp;
+  p.per_seq = p.row_tiles * p.kv_heads;
+  p.stretch = (p.batch + 31) / 32;
   // the work list is counted in 32 bits
   const int64_t most_tiles = cdiv64(max_pages * cache->page_size, kHalf) + 1;
   if ((double)most_tiles * batch * p.row_tiles * p.kv_heads > 2e9)
@@ -1128,6 +1161,12 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
   p.window = (int)window;
   p.sinks = (int)sinks;
   p.shares = shares_of();
+  p.share_items = p.batch * p.per_seq / p.shares;
+  p.longer_shares = p.batch * p.per_seq % p.shares;
+  p.by_shares = Divisor(p.shares);
+  p.by_per_seq = Divisor(p.per_seq);
+  p.by_row_tiles = Divisor(p.row_tiles);
+  p.by_stretch = Divisor(p.stretch);
   p.marks = need > 0 ? reinterpret_cast<float2*>(p.parts + 2ll * p.shares * rp * cache->head_dim) : nullptr;
   p.q_aligned = at16(q) && q_batch_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
   p.scale = scale;
