@@ -433,15 +433,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   __syncwarp();
   if (warp == 1) tmem_alloc(smem_u32(&sh.tmem_slot), S::kTmemCols);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = sh.tmem_slot;
   // every warp finds the share's place for itself
   const WorkList list(p);
   const int from = list.share_start(p, blockIdx.x), to = list.share_start(p, blockIdx.x + 1);
   Cursor c;
   c.start(p, to > from ? list.locate(p, from) : Place{0, 0, 0, 0}, to - from);
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = sh.tmem_slot;
 
   if (warp == 0) {
     // ---- producer ----
