@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -39,6 +40,13 @@ class Golden:
         if a.dtype == np.uint16:
             t = torch.from_numpy(a.view(np.int16).copy()).view(torch.bfloat16)
         return t
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _no_garbage_of_other_modules():
+    """A test that skips half way leaves its tensors in a reference cycle with the exception.  They go
+    before the next module begins, so that what a test reads of the allocator is its own doing."""
+    gc.collect()
 
 
 @pytest.fixture(scope="session")
