@@ -34,14 +34,16 @@
 // follows them.
 //
 // What bounds it: HBM where there is enough of it to do (64 sequences of 4 to 8 thousand tokens, 8 key
-// heads of 128 in bf16: 134 us, 6.1 TB/s; the sums of 16 rows a key head in fp16 keep the softmax
-// threads busier than HBM: 31 sequences of 11 to 22 thousand tokens, 28 rows, 90 us, a fifth of HBM's
+// heads of 128 in bf16: 132 us, 6.1 TB/s; the sums of 16 rows a key head in fp16 keep the softmax
+// threads busier than HBM: 31 sequences of 11 to 22 thousand tokens, 28 rows, 87 us, a quarter of HBM's
 // rate, with issue slots half used and the rest spent on the exchange of the maxima); below some 20 us
-// the chain length -> page -> tile -> scores -> probabilities -> sums, 8.3 us for one short sequence.
+// the chain length -> page -> tile -> scores -> probabilities -> sums, 6.5 us for one sequence of 100 tokens.
+// Some 1.5 of them pass until a block knows its share, 1.5 until its first page is asked for and 1 to 2
+// until that is there, which is why the first copies leave before anything else is looked up.
 // Two CTAs per SM hide one's exchange behind the other's arithmetic.  Measured on the way, the first of
 // these cases: a thread per score without tensor cores 9463 us, tiles of 128 tokens with four softmax
 // warps 191, pages and scales looked up two steps ahead and products joined a tile later 140, tiles of
-// 256 tokens with eight warps 134.
+// 256 tokens with eight warps 134, a shorter start 132.
 
 #include "elem.cuh"
 #include "kv_cache.cuh"
@@ -181,9 +183,9 @@ struct WorkList {
 
   // Shares of whole items, or of tiles?  Joining the parts of cut items costs about as much as
   // kJoinTiles tiles: whole items where the longest share of them is no longer than that (1 sequence of
-  // 1000 tokens, 8 key heads of 4 tiles: cut 10.7 us, whole 14.0).  Always whole where every item has
-  // up to kWholeTiles: the host then leaves out the joining launch (can_be_cut; 32 sequences of 700
-  // tokens: whole 16.5 us, cut 18.5; 1 of 600: 10.8 and 12.7).
+  // 1000 tokens, 8 key heads of 4 tiles: cut 9.6 us, whole 11.1; 16 of them: whole 14.4, cut 15.5).
+  // Always whole where every item has up to kWholeTiles: the host then leaves out the joining launch
+  // (can_be_cut; 4 sequences of 700 tokens: whole 9.7 us, cut 10.9).
   __device__ int tile_share(const KvAttnParams& p) const { return p.by_shares.divide(tiles(p) + p.shares - 1); }
   __device__ bool whole_items(const KvAttnParams& p) const {
     const long long items = p.share_items + (p.longer_shares > 0);
