@@ -281,7 +281,7 @@ struct Shape {
   static constexpr int kPBytes = kN * kHalf;
   // ring of a tile's K halves, its V halves, the next tile's ...: what two CTAs per SM, and the
   // joining kernel beside them, leave room for
-  static constexpr int kRoom = (kSmemPerCta - 3072 - 320 * RP - 2 * kPBytes - 2 * kQBytes) / kSlotBytes;
+  static constexpr int kRoom = (kSmemPerCta - 3 * 1024 - 320 * RP - 2 * kPBytes - 2 * kQBytes) / kSlotBytes;
   static constexpr int kSlots = kRoom < 12 ? kRoom : 12;
   static constexpr int kTmemO = 4 * kN;                           // behind the scores of two tiles
   static constexpr int kTmemCols = 5 * kN <= 128 ? 128 : 256;
