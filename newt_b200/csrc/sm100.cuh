@@ -359,11 +359,6 @@ __device__ __forceinline__ void keep_behind(uint32_t (&r)[N]) {
 #pragma unroll
   for (int i = 0; i < N; i += 2) asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]));
 }
-template <int N>
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
-  tmem_ld_wait();
-  keep_behind(r);
-}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
