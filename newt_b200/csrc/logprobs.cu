@@ -660,19 +660,24 @@ int launch_logprobs(const LogprobParams& p, int ranks, cudaStream_t stream) {
 
 template <typename T, bool TOP>
 int dispatch_logprobs(const LogprobParams& p, cudaStream_t stream) {
-  // More rows than SMs: a small CTA per row, many of them per SM, so that some stream while others start
-  // or finish their rows (4096 x 50021 bf16: 70 us; CTAs of 256 threads 76, of 64 85; 600 rows: 17.3, with
-  // CTAs of 512 threads 20.6; with 5 alternatives 21 and 30).
   const int sms = device_info().sm_count;
-  if (p.rows > sms) return launch_logprobs<T, TOP, 128>(p, 1, stream);
-  // Otherwise a large CTA per row, or a cluster of them as long as the rows have no more CTAs than there
-  // are SMs and each CTA has a chunk to read.  A second CTA per SM loses more to the cluster's
-  // barriers than it gains: 100 rows of 50021 take 6.2 us, shared by two CTAs 7.3; with alternatives
-  // 9.6 and 11.9; 16 rows of 129001 in fp32 with 20 take 11.3.
+  // what a CTA should have to read, if a row is to have another one
   constexpr int kChunk = 512 * kVectors * Elem<T>::kPerVec;
   int ranks = 1;
-  while (ranks < kMaxCluster && p.rows * ranks * 2 <= sms && p.vocab >= ranks * 2 * kChunk) ranks *= 2;
-  return launch_logprobs<T, TOP, 512>(p, ranks, stream);
+  if (p.rows <= sms || (p.rows <= 2 * sms && p.vocab >= 2 * kChunk)) {
+    // Large CTAs, and clusters of them as long as the rows have no more CTAs than there are SMs: a second
+    // one per SM loses more to the cluster's barriers than it gains (100 rows of 50021 take 6.2 us, shared
+    // by two CTAs 7.3; with alternatives 9.6 and 11.9; 16 rows of 129001 in fp32 with 20 take 11.3).  Up to
+    // twice as many rows as SMs, where they are long: 290 rows of 129001 17.1 us, small CTAs 26.2 (with
+    // 20 alternatives 22 and 44); of 8003 with 5 alternatives 9.6, small CTAs 7.4.
+    while (ranks < kMaxCluster && p.rows * ranks * 2 <= sms && p.vocab >= ranks * 2 * kChunk) ranks *= 2;
+    return launch_logprobs<T, TOP, 512>(p, ranks, stream);
+  }
+  // Small CTAs, many of them per SM, so that some stream while others start or finish their rows
+  // (4096 x 50021 bf16: 70 us; CTAs of 256 threads 76, of 64 85; 600 rows: 17.3, CTAs of 512 threads 20.6).
+  // Two to a long row while all of them fit the chip (300 rows of 129001: 21.3 us, one to a row 26.4).
+  if (p.rows * 2 <= ctas_per_sm(128) * sms && p.vocab >= 2 * kChunk) ranks = 2;
+  return launch_logprobs<T, TOP, 128>(p, ranks, stream);
 }
 
 template <typename T>

@@ -591,8 +591,19 @@ def test_token_logprobs_of_many_rows(vocab, dtype):
         _check_scores(x, tokens, top, inv)
 
 
+@pytest.mark.parametrize("rows, vocab, dtype", [(150, 30011, BF16), (296, 16384, FP16), (297, 20005, BF16),
+                                               (500, 17003, FP16), (593, 16390, BF16), (400, 9001, FP32)])
+def test_token_logprobs_of_rows_that_share_the_chip(rows, vocab, dtype):
+    """Around once, twice and four times as many rows as SMs, long enough for two small CTAs each."""
+    gen = _gen(rows)
+    x = _randn(gen, rows, vocab, dtype=dtype, scale=3.0)
+    tokens = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    for top in (0, 5, 32):
+        _check_scores(x, tokens, top, 1.0)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
-@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("rows", [3, 200, 400])
 @pytest.mark.parametrize("vocab", [33, 1000, 4099, 20000])
 def test_alternatives_of_any_order(vocab, rows, dtype):
     """Equal, ordered, sparse and bunched logits: no list overflows and ties go to the lower index."""
