@@ -14,7 +14,7 @@
 // HBM-bound: 3 bytes per element; a decode step is bound by its latency (lengths, then the page,
 // then the data).  Small owners with many loads in flight are what counts: a CTA of 256 threads
 // with four vectors each and a loop over heads that fetched the next head ahead measured 21.4 us
-// where this form takes 15.4 (13004 tokens of 8 heads of 128, pages of 64).
+// where this form takes 16 (13004 tokens of 8 heads of 128, pages of 64).
 
 #include "elem.cuh"
 #include "kv_cache.cuh"
