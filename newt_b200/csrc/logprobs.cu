@@ -9,8 +9,9 @@
 // multiply-add, exact but for its rounding, and R is only ever used as the rounded number it is, so
 // nothing is lost by its rounding; two lanes of packed fp32 share an instruction.  Logits are raised to
 // -1e30 at least, where 2^x is 0: -inf would make E a NaN.  log S and E / S give all three results.
-// Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest value of a wide type, +inf) are
-// done again, from differences to the maximum, by the row's first CTA.
+// Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest value of a wide type, +inf), or so
+// large in log2 units that its rounding is more than a factor of two (beyond +-2^24), are done again, from
+// differences to the maximum, by the row's first CTA.
 //
 // What bounds it: HBM, and for 16-bit logits the special function unit close behind, whose one 2^x per
 // element takes three quarters of the time HBM does; everything else is kept to four or five
@@ -80,6 +81,7 @@ struct Partial {
   float m, r, s, e;
 };
 constexpr float kLowest = -1e30f, kNone = -3e38f, kWide = 1e29f;
+constexpr float kFar = 16777216.0f;      // in log2 units: from here on a reference's rounding may be more than a half
 
 // sums relative to 2^to from sums relative to 2^from, from <= to (or both sums 0)
 __device__ __forceinline__ void rescale(float from, float to, float& s, float& e) {
@@ -387,7 +389,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kThreads)) logprob_kerne
   const unsigned long long factor2 = pack2(factor, factor);
   auto raise = [&](float most) {       // the reference moves up to y of `most`
     largest = most;
-    const float to = fmaxf(fmaxf(most, kLowest) * factor, kLowest);   // never below a raised logit's
+    // never so far down that its rounding would matter: what is there has no weight, or its row is done again
+    const float to = fmaxf(most * factor, -2.0f * kFar);
     const float d = fminf(fmaxf(ref - to, -1000.0f), 0.0f);
     const float f = exp2_approx(d);
     const unsigned long long f2 = pack2(f, f);
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kThreads)) logprob_kerne
     }
   }
   float behind = fmaf(total.m, factor, -total.r);    // what rounding took from the reference
-  if (!(fabsf(total.m) < kWide && fabsf(total.m * factor) < kWide)) {   // the same in every thread
+  if (!(fabsf(total.m) < kWide && fabsf(total.m * factor) < kFar)) {   // the same in every thread
     __syncthreads();                                 // warp_part has been read
     total = whole_row<T, kThreads>(x, vocab, factor, warp_part);
     behind = 0.0f;
