@@ -8,10 +8,10 @@
 // E = sum 2^(y_j - R) (y_j - R); both are rescaled when R grows.  y_j - R is one fused
 // multiply-add, exact but for its rounding, and R is only ever used as the rounded number it is, so
 // nothing is lost by its rounding; two lanes of packed fp32 share an instruction.  Logits are raised to
-// -1e30 at least, where 2^x is 0: -inf would make E a NaN.  log S and E / S give all three results.
-// Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest value of a wide type, +inf), or so
-// large in log2 units that its rounding is more than a factor of two (beyond +-2^24), are done again, from
-// differences to the maximum, by the row's first CTA.
+// `low`, -1e30 or what keeps y within -1e38: 2^y is 0 there, and -inf would make E a NaN.  log S and
+// E / S give all three results.  Rows whose largest logit is beyond +-1e29 (all -inf, all at the lowest
+// value of a wide type, +inf), or so large in log2 units that its rounding is more than a factor of two
+// (beyond +-2^24), are done again, from differences to the maximum, by the row's first CTA.
 //
 // What bounds it: HBM, and for 16-bit logits the special function unit close behind, whose one 2^x per
 // element takes three quarters of the time HBM does; everything else is kept to four or five
@@ -61,6 +61,7 @@ struct LogprobParams {
   int64_t stride;
   int rows, vocab, top;
   float inv_temperature;
+  float low;                // what logits are raised to, from inv_temperature
 };
 
 // Larger key = larger value, then lower index.  -0 counts as 0, NaN as the lowest value.
@@ -91,40 +92,40 @@ __device__ __forceinline__ void rescale(float from, float to, float& s, float& e
   s *= f;
 }
 
-__device__ __forceinline__ float raised(float v) {   // NaN stays
+__device__ __forceinline__ float raised(float v, float low) {   // NaN stays
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(kLowest));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(low));
   return r;
 }
-// What a 16-byte vector holds, raised to kLowest, and the largest of it.  NaN is kept among the values
+// What a 16-byte vector holds, raised to `low`, and the largest of it.  NaN is kept among the values
 // and passed over by the maximum.
-__device__ __forceinline__ void unpack(const Vec<float>& v, float (&f)[4], float& most) {
+__device__ __forceinline__ void unpack(const Vec<float>& v, float low, float (&f)[4], float& most) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    f[j] = raised(v.e[j]);
+    f[j] = raised(v.e[j], low);
     most = fmaxf(most, f[j]);
   }
 }
-__device__ __forceinline__ void unpack(const Vec<__nv_bfloat16>& v, float (&f)[8], float& most) {
+__device__ __forceinline__ void unpack(const Vec<__nv_bfloat16>& v, float low, float (&f)[8], float& most) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v.raw);
-  const __nv_bfloat162 low = __float2bfloat162_rn(kLowest);
+  const __nv_bfloat162 low2 = __float2bfloat162_rn(low);
   __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const __nv_bfloat162 x = __hmax2_nan(h[j], low);
+    const __nv_bfloat162 x = __hmax2_nan(h[j], low2);
     f[2 * j] = __low2float(x);
     f[2 * j + 1] = __high2float(x);
   }
   most = fmaxf(most, fmaxf(__low2float(m), __high2float(m)));
 }
-__device__ __forceinline__ void unpack(const Vec<__half>& v, float (&f)[8], float& most) {
+__device__ __forceinline__ void unpack(const Vec<__half>& v, float low, float (&f)[8], float& most) {
   const __half2* h = reinterpret_cast<const __half2*>(&v.raw);
   const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float2 x = __half22float2(h[j]);
-    f[2 * j] = raised(x.x);
-    f[2 * j + 1] = raised(x.y);
+    f[2 * j] = raised(x.x, low);
+    f[2 * j + 1] = raised(x.y, low);
   }
   most = fmaxf(most, fmaxf(__low2float(m), __high2float(m)));
 }
@@ -235,11 +236,11 @@ __device__ __forceinline__ float lower_bound(float value, int k, int vectors, fl
 // row's index of the first element.  `alone`: this thread's elements around the vectors, -1 for none.
 template <typename T, int THREADS>
 __device__ __forceinline__ void gather(TopState& t, const T* x, const T* body, int vectors, int first, float largest,
-                                       const int (&alone)[2], unsigned long long* picks, int* picked) {
+                                       const int (&alone)[2], unsigned long long* picks, int* picked, float low) {
   constexpr int E = Elem<T>::kPerVec, U = kVectors;
   const int tid = threadIdx.x;
   float bound = lower_bound<THREADS>(largest, t.k, vectors, reinterpret_cast<float*>(t.warp_best));
-  if (bound <= kLowest) bound = -INFINITY;           // what `largest` says of raised logits is no bound
+  if (bound <= low) bound = -INFINITY;           // what `largest` says of raised logits is no bound
   if (largest >= bound) picks[atomicAdd(picked, 1)] = make_key(largest, tid);
   __syncthreads();
   int n = *picked;
@@ -252,7 +253,7 @@ __device__ __forceinline__ void gather(TopState& t, const T* x, const T* body, i
     __syncthreads();
     if (tid < n) picks[rank] = mine;
     __syncthreads();
-    if (key_value(picks[t.k - 1]) > kLowest) least = (uint32_t)(picks[t.k - 1] >> 32);
+    if (key_value(picks[t.k - 1]) > low) least = (uint32_t)(picks[t.k - 1] >> 32);
     n = __syncthreads_count(tid < n && (uint32_t)(mine >> 32) >= least);
   }
   t.threshold = ((unsigned long long)least << 32) - 1;
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kThreads)) logprob_kerne
   const int tid = threadIdx.x;
   const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
   const int vocab = p.vocab;
-  const float factor = p.inv_temperature * kLog2e;
+  const float factor = p.inv_temperature * kLog2e, low = p.low;
   if (ranks > 1) cluster_arrive();     // waited for before the first CTA's memory is written
 
   // [0, head) one by one, then `vectors` vectors, then [tail, vocab) one by one
@@ -426,10 +427,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kThreads)) logprob_kerne
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (full || base + u * kThreads + tid < v1) {
-        unpack(from[u], f[u], most);
+        unpack(from[u], low, f[u], most);
       } else {
 #pragma unroll
-        for (int j = 0; j < E; ++j) f[u][j] = kLowest;
+        for (int j = 0; j < E; ++j) f[u][j] = low;
       }
     }
     load(from, base + 2 * kStep);
@@ -452,13 +453,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(kThreads)) logprob_kerne
   auto take = [&](int index) {
     const float v = Elem<T>::to_f32(x[index]);
     if (v > largest) raise(v);
-    take2(raised(v), kLowest);
+    take2(raised(v, low), low);
   };
   const int alone[2] = {rank == 0 && tid < head ? tid : -1, rank == ranks - 1 && tail + tid < vocab ? tail + tid : -1};
   if (alone[0] >= 0) take(alone[0]);
   if (alone[1] >= 0) take(alone[1]);
   if constexpr (TOP)
-    gather<T, kThreads>(top, x, body + (int64_t)v0 * E, v1 - v0, head + v0 * E, largest, alone, picks, &picked);
+    gather<T, kThreads>(top, x, body + (int64_t)v0 * E, v1 - v0, head + v0 * E, largest, alone, picks, &picked, low);
 
   // the CTA's sums: relative to the warp's reference, then to the CTA's
   float sa, sb, ea, eb;
@@ -728,7 +729,7 @@ extern "C" int nb200_token_logprobs(const void* logits, const int64_t* tokens, f
   if (!logits || (logprob && !tokens) || (top > 0 && (!top_logprob || !top_index)))
     return fail(NB200_E_INVALID, "token logprobs: null tensor pointer");
   LogprobParams p{logits, tokens, logprob, entropy, lse, top_logprob, top_index, stride, (int)rows,
-                  (int)vocab, (int)top, inv_temperature};
+                  (int)vocab, (int)top, inv_temperature, fmaxf(kLowest, -1e38f / (inv_temperature * kLog2e))};
   switch (dtype) {
     case NB200_F32:
       return top ? dispatch_logprobs<float, true>(p, stream) : dispatch_logprobs<float, false>(p, stream);

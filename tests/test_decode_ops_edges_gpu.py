@@ -36,7 +36,7 @@ def _agree(got, want, relative, floor):
 
 # ---- log probabilities -------------------------------------------------------------------------
 
-@pytest.mark.parametrize("inv", [1e-20, 1e-3, 0.1, 0.25, 0.5, 0.7, 0.9, 1.3, 1.7, 1e3, 1e6])
+@pytest.mark.parametrize("inv", [1e-20, 1e-3, 0.1, 0.25, 0.5, 0.7, 0.9, 1.3, 1.7, 1e3, 1e6, 1e9, 1e20])
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("rows, vocab, top", [(3, 1003, 5), (301, 1003, 5), (2, 40009, 0), (650, 33, 32)])
 def test_token_logprobs_at_far_temperatures(rows, vocab, top, dtype, inv):
