@@ -390,7 +390,7 @@ int nb200_token_logprobs(const void* logits, const int64_t* tokens, float* logpr
  *   grad_logits = inv_temperature * (g ([j = token] - p) - gH p (log p + entropy))
  * with g = grad_logprob and gH = grad_entropy (either may be null: 0).  A row whose token is
  * negative or beyond the vocabulary has no part from g; a row masked as a whole (lse below -1e30)
- * has gradient 0.
+ * has gradient 0.  log p = z - lse is as exact as an fp32 lse allows, 2^-24 of |lse|, and never above 0.
  * grad_logits has the logits' type, one rounding; it may be the logits themselves. */
 int nb200_token_logprobs_bwd(const void* logits, const int64_t* tokens, const float* lse,
                              const float* entropy, const float* grad_logprob,

@@ -559,6 +559,12 @@ struct GradParams {
 
 constexpr int kGradVectors = 4;   // per thread
 
+__device__ __forceinline__ float at_most_zero(float v) {   // NaN stays
+  float r;
+  asm("min.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // One CTA per stretch of a row: 16-byte vectors counted from the row's first 16-byte boundary, the
 // elements around them by the first CTA of the row.
 template <typename T>
@@ -589,10 +595,11 @@ __global__ void __launch_bounds__(kThreads) logprob_grad_kernel(const GradParams
   const unsigned long long inv2 = pack2(p.inv_temperature, p.inv_temperature), lse2 = pack2(-lse, -lse);
   const unsigned long long log2e2 = pack2(kLog2e, kLog2e), slope2 = pack2(slope, slope), offset2 = pack2(offset, offset);
   auto grad2 = [&](float& a, float& b) {             // two logits become their gradients
-    const unsigned long long z2 = fma2(pack2(a, b), inv2, lse2);       // log p
     float za, zb, ya, yb;
-    unpack2(z2, za, zb);
-    unpack2(mul2(z2, log2e2), ya, yb);
+    unpack2(fma2(pack2(a, b), inv2, lse2), za, zb);                    // log p
+    za = at_most_zero(za);                           // where lse's own rounding would make it more
+    zb = at_most_zero(zb);
+    unpack2(mul2(pack2(za, zb), log2e2), ya, yb);
     const unsigned long long c2 = pack2(fmaxf(za, -1000.0f), fmaxf(zb, -1000.0f));   // 0 times -inf is none of ours
     unpack2(mul2(pack2(exp2_approx(ya), exp2_approx(yb)), fma2(slope2, c2, offset2)), a, b);
   };

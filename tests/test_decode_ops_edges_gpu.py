@@ -59,3 +59,54 @@ def test_token_logprobs_at_far_temperatures(rows, vocab, top, dtype, inv):
         assert torch.equal(got.top_index, order)
         # beyond fp32's range: -inf
         _agree(got.top_logprob, log_p.gather(1, order).float(), 2.0 ** -21, 2.0 ** -18)
+
+
+@pytest.mark.parametrize("inv", [1e-20, 1e-3, 10.0, 100.0, 1e3, 1e6, 1e9, 1e20])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows, vocab", [(3, 1003), (301, 257)])
+def test_token_logprobs_backward_at_far_temperatures(rows, vocab, dtype, inv):
+    """No probability above 1, however coarse the row's lse has become."""
+    gen = _gen(rows * 5 + vocab)
+    x = _randn(gen, rows, vocab, dtype=dtype, scale=3.0)
+    x[:, vocab - 7:] = -math.inf
+    tokens = torch.randint(0, vocab - 7, (rows,), generator=gen, device="cuda")
+    g, ge = _randn(gen, rows), _randn(gen, rows, scale=0.3)
+    f = ops.token_logprobs(x, tokens, inv_temperature=inv)
+    got = ops.token_logprobs_backward(x, tokens, f.lse, f.entropy, g, ge, inv_temperature=inv).double()
+    exactly = torch.tensor(inv, dtype=FP32).double().item()
+    _, entropy, lse, log_p = _score_exact(x, tokens, exactly)
+    p = log_p.exp()
+    hit = torch.zeros_like(p).scatter_(1, tokens[:, None], 1.0)
+    inner = torch.where(p > 0, log_p, 0.0) + entropy[:, None]
+    want = exactly * (g.double()[:, None] * (hit - p) - ge.double()[:, None] * p * inner)
+    # lse and the product of a logit and 1/T are off by 2^-24 of themselves: with d = 2^-21 |lse| more
+    # or less in the exponent p lies between p e^-d and min(1, p e^d), and p |log p| up to 1/e + d p
+    d = (2.0 ** -21 * lse.abs() + 2.0 ** -18)[:, None]
+    high = torch.minimum((log_p + d).exp(), torch.ones_like(p))
+    off_p = torch.maximum(high - p, p * -torch.expm1(-d))
+    part = ge.abs().double()[:, None] * (high * (d + 2.0 ** -18) + off_p * (inner.abs().clamp(max=1000) + d.clamp(max=1000)))
+    # values off by less than a step of a type's smallest normal number may be anything below it
+    bound = exactly * (g.abs().double()[:, None] * (off_p + 2.0 ** -22) + part) + HALF[dtype] * want.abs() + exactly * 2.0 ** -20 + 1e-38
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= bound).all()
+    most = exactly * (2 * g.abs() + ge.abs() * (1 + entropy)).double()[:, None] * 1.01
+    assert (got.abs() <= most).all()
+
+
+def test_token_logprobs_backward_of_large_logits():
+    """Logits whose lse rounds by several units: no probability comes out above 1."""
+    x = torch.full((4, 1000), 1e8, device="cuda")
+    x[1] = -1e8
+    x[2] = 3e9
+    x[3, ::2] = -3e9
+    tokens = torch.tensor([3, 4, 5, 6], device="cuda")
+    f = ops.token_logprobs(x, tokens, inv_temperature=0.7)
+    one = torch.ones(4, device="cuda")
+    got = ops.token_logprobs_backward(x, tokens, f.lse, f.entropy, one, inv_temperature=0.7)
+    assert got.abs().max() <= 1.0
+    got = ops.token_logprobs_backward(x, tokens, f.lse, f.entropy, None, one, inv_temperature=0.7)
+    assert got.abs().max() <= 1 + math.log(1000)
+    x[0, 0] = math.nan                            # still the row's whole
+    f = ops.token_logprobs(x, tokens, inv_temperature=0.7)
+    got = ops.token_logprobs_backward(x, tokens, f.lse, f.entropy, one, one, inv_temperature=0.7)
+    assert torch.isnan(got[0]).all() and torch.isfinite(got[1:]).all()
