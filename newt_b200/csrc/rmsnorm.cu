@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "elem.cuh"
+#include "shifted_row.cuh"
 #include "sm100.cuh"
 
 namespace nb200 {
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
   constexpr int E = Elem<T>::kPerVec;
   constexpr bool FAST = SPREAD == ALIGNED, WHOLE = SPREAD != SINGLE;
   __shared__ float slots[2][32];
-  // SHIFTED: the groups' maxima, a row's behind the other's (a row of one warp has at most 32 groups)
+  // SHIFTED: the groups' maxima, a row's behind the other's (eight rows of one warp have at most 33 groups each)
   __shared__ uint32_t group_most[SPREAD == SHIFTED && E4M3 ? kMaxShifted / 32 : 1];
   const int warps = p.threads >> 5;
   const int per_cta = blockDim.x / p.threads;
@@ -134,15 +135,15 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
   const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.stride_residual : nullptr;
   const T* w = static_cast<const T*>(p.w);
   const int m = SPREAD == SHIFTED ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
-  const int head = m ? E - m : 0;
-  const int end = SPREAD == SHIFTED ? head + max(n - m - head, 0) / E * E : n;     // of the vectors
+  const ShiftedRow at(n, m, E);
+  const int head = at.head, end = SPREAD == SHIFTED ? at.end : n;     // of the vectors
   // vectors from m columns before the row on, the first of them left out where m is not 0
   const int col0 = WHOLE ? lane * E - m : (lane >> 5) * 32 * E + (lane & 31), col_step = p.threads * E;
   auto column = [&](int i, int j) { return col0 + i * col_step + (WHOLE ? j : 32 * j); };
   auto whole = [&](int i) { return (unsigned)column(i, 0) < (unsigned)end; };
   // this thread's element outside of the vectors: at most 2 E - 1 threads of a row have one
-  const int alone = SPREAD != SHIFTED ? n : lane < head ? lane : end - head + lane;
-  const bool has_alone = SPREAD == SHIFTED && lane < n - (end - head);
+  const int alone = SPREAD != SHIFTED ? n : at.single(lane);
+  const bool has_alone = SPREAD == SHIFTED && lane < at.singles();
 
   // this thread's part of a row; columns outside of it are 0
   auto read = [&](const T* from, Vec<T> (&to)[ITEMS]) {
@@ -164,9 +165,9 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
       to[i].raw = make_uint4(0, 0, 0, 0);
       if constexpr (WHOLE) {
         if (!whole(i)) continue;
-        const uint4* at = reinterpret_cast<const uint4*>(w + column(i, 0) - head);
-        to[i].raw = __ldg(at);
-        if (SPREAD == SHIFTED && m) to[i] = window<T>(to[i].raw, __ldg(at + 1), head);
+        const uint4* from = reinterpret_cast<const uint4*>(w + column(i, 0) - head);
+        to[i].raw = __ldg(from);
+        if (SPREAD == SHIFTED && m) to[i] = window<T>(to[i].raw, __ldg(from + 1), head);
       } else {
 #pragma unroll
         for (int j = 0; j < E; ++j)
@@ -263,9 +264,10 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
         const float behind = __shfl_down_sync(0xffffffffu, before, 1);
         if (in_warp < 31) from = fmaxf(from, behind);
         for (int o = lanes >> 1; o > 0; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xffffffffu, from, o));
-        const int col = column(i, 0) + m;            // magnitudes are ordered as their bits are
-        if (in_warp == 0 && m && col <= end) atomicMax(&most_of[(col - 1) >> p.group_shift], __float_as_uint(before));
-        if ((in_warp & (lanes - 1)) == 0 && col < n) atomicMax(&most_of[col >> p.group_shift], __float_as_uint(from));
+        // magnitudes are ordered as their bits are
+        const int group_before = at.group_before(column(i, 0), p.group_shift), group_from = at.group_from(column(i, 0), p.group_shift);
+        if (in_warp == 0 && group_before >= 0) atomicMax(&most_of[group_before], __float_as_uint(before));
+        if ((in_warp & (lanes - 1)) == 0 && group_from >= 0) atomicMax(&most_of[group_from], __float_as_uint(from));
       }
       if (has_alone) atomicMax(&most_of[alone >> p.group_shift], __float_as_uint(fmaxf(fabsf(single), 0.0f)));
       if (warps > 1) __syncthreads(); else __syncwarp();

@@ -1,0 +1,62 @@
+"""What the decode step's operators do at their edges, as far as that can be seen without a GPU:
+index arithmetic compiled for the host, and refusals."""
+
+import os
+import subprocess
+
+import newt_b200
+
+CSRC = os.path.join(os.path.dirname(newt_b200.__file__), "csrc")
+
+COLUMNS = r"""
+#include <cstdio>
+#include <vector>
+#include "shifted_row.cuh"
+using nb200::ShiftedRow;
+
+#define CHECK(what) if (!(what)) { std::printf("n=%d m=%d E=%d shift=%d: %s\n", n, m, E, shift, #what); return 1; }
+
+int check(int n, int m, int E, int shift, int threads) {
+  const ShiftedRow row(n, m, E);
+  const int groups = (n + (1 << shift) - 1) >> shift;
+  std::vector<int> seen(n);
+  CHECK(row.singles() >= 0 && row.singles() < 2 * E);
+  for (int i = 0; i < row.singles(); ++i) {
+    CHECK(row.single(i) >= 0 && row.single(i) < n);
+    ++seen[row.single(i)];
+  }
+  for (int column = -m; column < n + threads * E; column += E) {
+    const int before = row.group_before(column, shift), from = row.group_from(column, shift);
+    CHECK(before >= -1 && before < groups && from >= -1 && from < groups);
+    CHECK((before >= 0) == (m && row.whole(column)));       // nothing from a vector that is left out
+    if (!row.whole(column)) continue;
+    CHECK(column % E == (E - m) % E && column + E <= n);
+    CHECK(m == 0 || column - row.head + 2 * E <= n);        // the weight's second vector
+    for (int j = 0; j < E; ++j) {
+      ++seen[column + j];
+      CHECK(((column + j) >> shift) == (j < m ? before : from));
+    }
+  }
+  for (int c = 0; c < n; ++c) CHECK(seen[c] == 1);
+  return 0;
+}
+
+int main() {
+  for (int E = 4; E <= 8; E += 4)
+    for (int m = 0; m < E; ++m)
+      for (int shift = 5; shift <= 7; ++shift)
+        for (int n = 1; n <= 700; ++n)
+          if (check(n, m, E, shift, 32)) return 1;
+  return 0;
+}
+"""
+
+
+def test_columns_of_shifted_rows_and_their_groups(tmp_path):
+    """Every column of a row that starts off a vector boundary is taken once, and no group outside of the
+    row's is touched."""
+    source, program = tmp_path / "columns.cpp", tmp_path / "columns"
+    source.write_text(COLUMNS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", CSRC, str(source), "-o", str(program)], check=True)
+    done = subprocess.run([str(program)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
