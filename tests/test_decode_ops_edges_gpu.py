@@ -110,3 +110,27 @@ def test_token_logprobs_backward_of_large_logits():
     f = ops.token_logprobs(x, tokens, inv_temperature=0.7)
     got = ops.token_logprobs_backward(x, tokens, f.lse, f.entropy, one, one, inv_temperature=0.7)
     assert torch.isnan(got[0]).all() and torch.isfinite(got[1:]).all()
+
+
+# ---- rmsnorm -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("n", [64, 257, 4096, 16389])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_rmsnorm_of_weights_at_the_end_of_their_type(dtype, n, group):
+    """Outputs above 2^126: the 8-bit numbers are those over the scale, not zeros."""
+    gen = _gen(n + group)
+    x = 0.5 + torch.rand(5, n, generator=gen, device="cuda")
+    x = (x * torch.sign(_randn(gen, 5, n))).to(dtype)
+    for size in (2.0 ** 125, 2.0 ** 126, 1.4 * 2.0 ** 126, 2.0 ** 126.9):
+        w = torch.full((n,), size, device="cuda").to(dtype)
+        got = ops.rmsnorm(x, w, eps=1e-5, out_dtype=ops.E4M3, group=group)
+        h = x.double()
+        y = h / (h.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+        assert y.abs().max() < torch.finfo(FP32).max
+        width = group or n
+        scales = torch.stack([part.abs().amax(1) / 448 for part in y.split(width, 1)], 1)
+        # the mean's sum, the root and the products: below 2^-17 in all; half a step of e4m3 is 2^-4
+        _agree(got.scales, scales, 2.0 ** -17, 0.0)
+        q = y / scales.repeat_interleave(width, 1)[:, :n]
+        _agree(got.out.float(), q, 2.0 ** -4 + 2.0 ** -15, 2.0 ** -10 * 1.001)
