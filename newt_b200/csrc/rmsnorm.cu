@@ -365,7 +365,7 @@ int dispatch_rms(RmsParams p, cudaStream_t stream) {
 
   if (p.n > kMaxColumns)
     return fail(NB200_E_UNSUPPORTED, "rmsnorm: rows of %d elements (at most %d)", p.n, kMaxColumns);
-  const int64_t vectors = spread == SHIFTED ? (p.n >= E ? p.n / E : 1) : cdiv64(p.n, E);
+  const int64_t vectors = spread == SHIFTED ? (p.n >= E ? p.n / E : 1) : cdiv64(p.n > 0 ? p.n : 1, E);
   int items = 1;
   // Few rows: as many threads as there are vectors, the row's latency counts (8 rows of 4096 bf16:
   // 2.7 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
@@ -411,8 +411,9 @@ extern "C" int nb200_rmsnorm(const void* x, const void* residual, const void* w,
   if (!e4m3 && group != 0)
     return fail(NB200_E_INVALID, "rmsnorm: a group of columns goes with an e4m3 output");
   if (!(eps >= 0.0f)) return fail(NB200_E_INVALID, "rmsnorm: eps must not be negative");
-  if (rows == 0 || n == 0) return 0;
-  if (!x || !w || !out || (e4m3 && !scales)) return fail(NB200_E_INVALID, "rmsnorm: null tensor pointer");
+  if (rows == 0 || (n == 0 && !(e4m3 && group == 0))) return 0;     // rows without columns still have a scale each
+  if ((n > 0 && (!x || !w || !out)) || (e4m3 && !scales))
+    return fail(NB200_E_INVALID, "rmsnorm: null tensor pointer");
   RmsParams p;
   p.x = x;
   p.residual = residual;

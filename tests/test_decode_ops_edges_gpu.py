@@ -134,3 +134,12 @@ def test_rmsnorm_of_weights_at_the_end_of_their_type(dtype, n, group):
         _agree(got.scales, scales, 2.0 ** -17, 0.0)
         q = y / scales.repeat_interleave(width, 1)[:, :n]
         _agree(got.out.float(), q, 2.0 ** -4 + 2.0 ** -15, 2.0 ** -10 * 1.001)
+
+
+def test_rmsnorm_of_rows_without_columns():
+    x, w = torch.zeros(3, 0, device="cuda", dtype=BF16), torch.zeros(0, device="cuda", dtype=BF16)
+    scales = torch.full((3, 1), 7.0, device="cuda")
+    got = ops.rmsnorm(x, w, out_dtype=ops.E4M3, scales=scales)
+    assert got.out.shape == (3, 0) and (scales == 1).all()          # the scale of nothing
+    assert ops.rmsnorm(x, w, out_dtype=ops.E4M3, group=32).scales.shape == (3, 0)
+    assert ops.rmsnorm(x, w).out.shape == (3, 0)
