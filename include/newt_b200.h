@@ -351,7 +351,7 @@ int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const void* v, i
  * stands at position lengths[b] - queries + i and sees the tokens j up to its own position with
  * j > position - window (`window` 0: all) or j < sinks.  A query that sees nothing (a sequence
  * shorter than `queries`, an empty one) gives zeros.  Tokens whose page is missing from the table
- * are not seen.  What lies in page rows that no query of the call sees has no effect, NaN included.
+ * are not seen.  What lies in page rows that a query does not see has no effect on it, NaN included.
  * `out` must not overlap q.
  * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 11 (fp16)
  * significant bits.

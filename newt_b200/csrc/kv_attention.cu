@@ -25,7 +25,9 @@
 // rescaling, in fp32.  P is laid out so that a thread writes its token's N bytes in one piece.
 //
 // Value rows that no query sees are cleared in shared memory before the product: their weight is
-// zero, but zero times a NaN that was left in a page would not be.
+// zero, but zero times a NaN that was left in a page would not be.  Of rows that some queries of the
+// call see and others do not, NaN bytes are cleared and noted for the rows that see them
+// (set_nan_aside): nothing reaches a query that it must not see.
 //
 // Work: all (sequence, row tile, key head) items in order, each a run of visible tiles (those of
 // the first tokens, then those of the window), cut into equal shares for a grid that fills the
@@ -302,6 +304,7 @@ struct Shared {
   float most[2][8][RP];                        // the warps' maxima, alternating by tile
   float sum[2][8][RP];                         // the warps' row sums, alternating by item
   float step[8][3][RP];                        // a warp's own: a row's reference, negative, and what the sums and the tile are scaled by
+  uint32_t nan[2][RP][D / 32];                 // columns in which a row has seen NaN set aside, alternating by item
   uint64_t full[S::kSlots], empty[S::kSlots], scale_full[4];
   uint64_t q_full[2], s_full[2], most_full[2], p_full, o_full, sum_full;
   uint32_t tmem_slot, abort_flag;
@@ -402,6 +405,44 @@ __device__ __noinline__ void stage_queries(const KvAttnParams& p, Vec<T> raw, in
   }
 }
 
+// A token that some rows of the item see and others do not: NaN in its value row, `row` of the tile in
+// shared memory, becomes 0, as zero times NaN would reach the rows that do not see it; `noted` keeps the
+// columns for those that do.  Out of line: it runs at the ends of a window, for several query tokens
+// (32 sequences with a window of 2048 and four of them: 26.1 us, without 25.6).
+template <int D, int RP>
+__device__ __noinline__ void set_nan_aside(const KvAttnParams& p, uint8_t* tile, int row, int token, const int* at,
+                                           uint32_t (*noted)[D / 32]) {
+  auto nan_bytes = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };   // 0x7f and 0xff
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < D; i += 16) {                // neighbours start at different banks
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + row * D + ((i + row * 16) & (D - 1)));
+    any |= nan_bytes(v.x) | nan_bytes(v.y) | nan_bytes(v.z) | nan_bytes(v.w);
+  }
+  if (any == 0) return;
+#pragma unroll 1
+  for (int i = 0; i < D; i += 16) {
+    // where the swizzle of its row length has put these 16 columns
+    const int chunk = (i / 16) ^ (D == 128 ? (row & 7) : ((row >> 1) & 3));
+    uint32_t* words = reinterpret_cast<uint32_t*>(tile + row * D + chunk * 16);
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = words[k];
+      const uint32_t nan = nan_bytes(w);
+      if (nan == 0) continue;
+      words[k] = w & ~((nan >> 7) * 0xffu);
+      uint32_t columns = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) columns |= (nan >> (8 * b + 7) & 1u) << b;
+      const int first = i + 4 * k;
+#pragma unroll 1
+      for (int r = 0; r < RP; ++r)
+        if (token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks))
+          atomicOr(&noted[r][first / 32], columns << (first % 32));
+    }
+  }
+}
+
 template <typename T, int D, int RP, int PARTS>
 __global__ void __launch_bounds__(kThreads, 2)
     kv_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -414,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const WaitCtx ctx{&sh.abort_flag, p.status, p.wait_limit_ns};
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel may get ready
+  for (int i = threadIdx.x; i < 2 * RP * (D / 32); i += kThreads) (&sh.nan[0][0][0])[i] = 0;
   if (threadIdx.x == 0) {
     sh.abort_flag = 0;
     for (int x = 0; x < SLOTS; ++x) {
@@ -666,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int t0 = tile_start(p, c.seq, c.at.tile + k), token = t0 + tid;
         Pair s[RP / 2];
         float inv_vs = 0.0f;
-        bool there = true;
+        bool plain = true;                         // seen by every row of the item, as far as is known without looking closer
         if (more) {
           const int step = j >> step_shift;
           ok = mbar_wait(smem_u32(&sh.scale_full[step & 3]), (step >> 2) & 1, ctx, ST_KV_SCALES, j) &&
@@ -689,7 +731,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float4 scale = sh.scale[step & 3][((j << (8 - p.page_shift)) + (tid >> p.page_shift)) & 31];
           inv_vs = scale.z;
           // seen by some query, and its page is there
-          there = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
+          const bool there = scale.w != 0.0f && (clean || seen_by_any(c.seq, token));
+          plain = there;
           Pair factor[RP / 2];
           pairs_of(sh.q_factor[item & 1], factor);
           const Pair ks = pack2(scale.x, scale.x), log_vs = pack2(scale.y, scale.y);
@@ -722,6 +765,10 @@ __global__ void __launch_bounds__(kThreads, 2)
               unpack2(s[r], a, b);
               s[r] = pack2(seen(2 * r) ? a : -INFINITY, seen(2 * r + 1) ? b : -INFINITY);
             }
+            // the item's rows are those of neighbouring positions, the first row's the lowest; one query
+            // token's rows see the same
+            const int low = at[0], high = c.seq.len - 1;
+            if (p.nq > 1) plain = there && token <= low && (!p.window || token > high - p.window || token < p.sinks);
           }
 #pragma unroll
           for (int r = 0; r < RP; r += 4) {
@@ -768,7 +815,15 @@ __global__ void __launch_bounds__(kThreads, 2)
               const int r = half * RH + i;
               float even, odd;
               unpack2(acc[i / 2], even, odd);
-              const float total = i % 2 ? odd : even;
+              float total = i % 2 ? odd : even;
+              if (quarter * 32 < D) {            // this warp's own word
+                const uint32_t nan = sh.nan[of & 1][r][quarter];
+                if (nan) {
+                  if (nan >> lane & 1) total = NAN;
+                  __syncwarp();
+                  if (lane == 0) sh.nan[of & 1][r][quarter] = 0;   // for the item after the next one
+                }
+              }
               float sum = 0.0f;
 #pragma unroll
               for (int w = 0; w < 8; ++w) sum += sh.sum[of & 1][w][r];
@@ -845,14 +900,18 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           st_shared_v4(smem_u32(sh.p[half]) + (i / 16) * (kHalf * 16) + me * 16, w[0], w[1], w[2], w[3]);
         }
-        if (__any_sync(0xffffffffu, !there)) {
+        if (__any_sync(0xffffffffu, !plain)) {
           const int g = 2 * H * j + H + half;
           ok = mbar_wait(smem_u32(&sh.full[g % SLOTS]), (g / SLOTS) & 1, ctx, ST_KV_ZERO, j);
           ok = __all_sync(0xffffffffu, ok);
+          const bool there = sh.scale[(j >> step_shift) & 3][((j << (8 - p.page_shift)) + (tid >> p.page_shift)) & 31].w != 0.0f &&
+                             seen_by_any(c.seq, token);
           if (!there) {
 #pragma unroll 1
             for (int i = 0; i < D; i += 16)     // neighbours start at different banks
               st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + ((i + me * 16) & (D - 1))]), 0, 0, 0, 0);
+          } else if (!plain && ok) {
+            set_nan_aside<D, RP>(p, sh.ring[g % SLOTS], me, token, sh.q_at[item & 1], sh.nan[item & 1]);
           }
         }
         fence_proxy_async_smem();

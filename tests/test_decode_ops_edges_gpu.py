@@ -9,7 +9,8 @@ import torch
 
 from newt_b200 import ops
 from newt_b200.runtime import abi
-from test_decode_ops_gpu import BF16, FP16, FP32, HALF, _gen, _randn, _score_exact
+from test_decode_ops_gpu import (BF16, FP16, FP32, HALF, _attend_exact, _finite_cache, _gen, _int32, _pages, _randn,
+                                 _score_exact)
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +144,82 @@ def test_rmsnorm_of_rows_without_columns():
     assert got.out.shape == (3, 0) and (scales == 1).all()          # the scale of nothing
     assert ops.rmsnorm(x, w, out_dtype=ops.E4M3, group=32).scales.shape == (3, 0)
     assert ops.rmsnorm(x, w).out.shape == (3, 0)
+
+
+# ---- attention over the cache ------------------------------------------------------------------
+
+def _check_some_nan(got, q, cache, table, lengths, window, sinks):
+    """NaN where the definition has NaN and nowhere else; the others as close as they have to be."""
+    want, _ = _attend_exact(q, cache, table, lengths, q.shape[3] ** -0.5, window, sinks)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    nan = torch.isnan(want)
+    clean = cache._replace(**{name: torch.where(torch.isnan(t.float()), 0, t.view(torch.uint8)).view(ops.E4M3)
+                              for name, t in (("k", cache.k), ("v", cache.v))})
+    assert nan.any() and not nan.all()
+    # the same values without NaN: what does not depend on them agrees
+    other, size = _attend_exact(q, clean, table, lengths, q.shape[3] ** -0.5, window, sinks)
+    assert torch.equal(other[~nan], want[~nan])
+    extra = {BF16: 2.0 ** -9 + 2.0 ** -11, FP16: 2.0 ** -11}[q.dtype] + 2.0 ** -11 + 2.0 ** -14
+    off = (got.double() - other).abs() - (HALF[q.dtype] * other.abs() + extra * size + 2.0 ** -25)
+    assert off[~nan].max() <= 0
+
+
+@pytest.mark.parametrize("window, sinks", [(0, 0), (40, 3), (5, 0), (300, 1)])
+@pytest.mark.parametrize("page, d, heads, kv_heads, nq, dtype", [
+    (16, 64, 2, 2, 4, FP16), (16, 128, 4, 2, 2, BF16), (64, 128, 7, 1, 3, BF16), (32, 64, 8, 1, 5, FP16),
+    (128, 128, 8, 2, 8, FP16), (64, 64, 3, 3, 4, BF16)])
+def test_attention_keeps_nan_from_queries_that_do_not_see_it(page, d, heads, kv_heads, nq, dtype, window, sinks):
+    """Value rows with NaN in some columns, seen by some of the call's queries: behind the others' own
+    position, or before their window.  Sequences shorter than the queries among them."""
+    gen = _gen(page + d + nq + window)
+    lengths = [nq + 1, max(nq - 1, 1), 129, 257, 300, 777, 64]
+    table, total = _pages(gen, lengths, page)
+    cache = _finite_cache(gen, total, kv_heads, page, d)
+    for b, n in enumerate(lengths):
+        tokens = [n - 1, n - 2] if b % 2 else [n - 1]
+        if window and n > nq + window:
+            tokens.append(n - nq - window + 1)             # the first query's oldest
+        for t in tokens:
+            codes = cache.v.view(torch.uint8)[table[b, t // page].item(), b % kv_heads, t % page]
+            codes[torch.tensor([3, 17, d - 1, 32 + b], device="cuda")] = torch.tensor(
+                [0x7F, 0xFF, 0x7F, 0xFF], dtype=torch.uint8, device="cuda")
+    q = _randn(gen, len(lengths), nq, heads, d, dtype=dtype)
+    lengths = _int32(lengths)
+    got = ops.kv_attention(q, cache, table, lengths, window=window, sinks=sinks)
+    _check_some_nan(got, q, cache, table, lengths, window, sinks)
+    cache.k.view(torch.uint8)[table[4, (lengths[4].item() - 1) // page].item(), 0, (lengths[4].item() - 1) % page, 5] = 0x7F
+    got = ops.kv_attention(q, cache, table, lengths, window=window, sinks=sinks)
+    _check_some_nan(got, q, cache, table, lengths, window, sinks)
+    for _ in range(2):                                     # and again: nothing of it stays
+        again = ops.kv_attention(q, cache, table, lengths, window=window, sinks=sinks)
+        assert torch.equal(again.view(torch.int16), got.view(torch.int16))
+
+
+def test_attention_keeps_nan_from_one_item_to_the_next():
+    """Many short items one after another in a share, every third with NaN in its last value row."""
+    gen = _gen(77)
+    lengths = [5 + (i * 13) % 200 for i in range(300)]
+    table, total = _pages(gen, lengths, 16)
+    cache = _finite_cache(gen, total, 3, 16, 64)
+    for b in range(0, 300, 3):
+        t = lengths[b] - 1
+        cache.v.view(torch.uint8)[table[b, t // 16].item(), b % 2, t % 16, b % 64] = 0x7F
+    q = _randn(gen, 300, 2, 6, 64, dtype=BF16)
+    lengths = _int32(lengths)
+    got = ops.kv_attention(q, cache, table, lengths)
+    _check_some_nan(got, q, cache, table, lengths, 0, 0)
+
+
+def test_attention_of_more_rows_than_a_tile_keeps_nan_where_it_is_seen():
+    """Row tiles of 16 rows, some of which none of a token's queries is in; parts of cut items."""
+    gen = _gen(78)
+    lengths = [3000, 41]
+    table, total = _pages(gen, lengths, 32)
+    cache = _finite_cache(gen, total, 1, 32, 128)
+    for b, t in ((0, 2990), (0, 2999), (0, 1000), (1, 33)):
+        cache.v.view(torch.uint8)[table[b, t // 32].item(), 0, t % 32, 7 + t % 100] = 0xFF
+    q = _randn(gen, 2, 20, 4, 128, dtype=BF16)
+    lengths = _int32(lengths)
+    for window, sinks in ((0, 0), (30, 2), (1995, 0)):
+        got = ops.kv_attention(q, cache, table, lengths, window=window, sinks=sinks)
+        _check_some_nan(got, q, cache, table, lengths, window, sinks)
