@@ -353,8 +353,9 @@ int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const void* v, i
  * shorter than `queries`, an empty one) gives zeros.  Tokens whose page is missing from the table
  * are not seen.  What lies in page rows that a query does not see has no effect on it, NaN included.
  * `out` must not overlap q.
- * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 11 (fp16)
- * significant bits.
+ * fp32 scores and sums; the probabilities enter the second product with 9 (bf16) or 14 (fp16)
+ * significant bits, the queries' elements exactly down to 2^-14 of the largest of their token and head
+ * and with an error of 2^-22 (bf16) or 2^-26 (fp16) of that below.
  * `workspace`: 16-byte aligned device memory of at least nb200_kv_attention_workspace_bytes(...)
  * bytes (0: none is needed, sequences of so few pages are never cut), the caller's; nothing in it
  * needs clearing, and it must not be shared by launches that can overlap on the GPU (two captured

@@ -12,9 +12,14 @@
 //   O^T [head_dim  x N]  = V tile (MN-major, as it lies) x P parts [N x 128 tokens]
 // and the other operand, which is small, is split into sums of e4m3 numbers that fill N columns:
 // a bf16 has 8 significant bits and is exactly hi + lo / 16 of two e4m3 (4 bits each, and what the
-// first rounding leaves over fits the second), an fp16 takes three.  So the queries lose nothing; the
-// probabilities are rounded to fp16 and keep 9 bits (two parts) or 11 (three): as many as the output
-// has, one more for bf16.  N = parts * rows, at least 16, was idle anyway.
+// first rounding leaves over fits the second), an fp16 takes three.  A row of queries has one exponent,
+// so that much is true of elements down to 2^-14 of the row's largest (bf16; fp16 2^-15); of smaller
+// ones e4m3's smallest step leaves an error of 2^-22 of the largest (fp16 2^-26).  Probabilities
+// keep 9 bits (two parts) or 14 (three): one more than a bf16 output has, three more than an fp16 one
+// (11 with the first part taken from fp16 too: 31 sequences, 28 rows in fp16, 93.7 us, with 14 94.4).
+// The sums of a row take them unrounded: a token whose value scale is far below its tile's
+// largest rounds to nothing in the product, but weighs no less.  N = parts * rows, at least 16, was idle
+// anyway.
 //
 // Per tile of 256 tokens each of 256 threads owns one token: it reads its N scores from tensor memory,
 // applies both scales and the masks, and takes part in the rows' maxima over the tile (warp reductions
@@ -868,7 +873,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           __syncwarp();
         }
         const auto& row_step = sh.step[warp - kSoftmaxWarp];
-        // probabilities (0 where the row sees nothing of the tile), rounded to fp16, in parts
+        // probabilities (0 where the row sees nothing of the tile) in parts
         uint32_t bytes[PARTS][RP / 4];
         Pair less[RP / 2], old[RP / 2], fresh[RP / 2];
         pairs_of(row_step[0], less);
@@ -882,10 +887,12 @@ __global__ void __launch_bounds__(kThreads, 2)
           a = exp2_approx(a);
           b = exp2_approx(b);
           l[r] = fma2(mul2(pack2(a, b), inv), fresh[r], mul2(l[r], old[r]));
+          uint32_t first = 0;
+          if (PARTS > 2) first = split2(a, b);     // what is left of it has 11 bits of its own in fp16
           __half2 pair = __floats2half2_rn(a, b);
 #pragma unroll
           for (int part = 0; part < PARTS; ++part) {
-            const uint32_t q = split2(pair);
+            const uint32_t q = PARTS > 2 && part == 0 ? first : split2(pair);
             if (r % 2 == 0) bytes[part][r / 2] = q; else bytes[part][r / 2] |= q << 16;
           }
         }

@@ -223,3 +223,47 @@ def test_attention_of_more_rows_than_a_tile_keeps_nan_where_it_is_seen():
     for window, sinks in ((0, 0), (30, 2), (1995, 0)):
         got = ops.kv_attention(q, cache, table, lengths, window=window, sinks=sinks)
         _check_some_nan(got, q, cache, table, lengths, window, sinks)
+
+
+@pytest.mark.parametrize("d, heads, nq", [(64, 4, 1), (128, 8, 1), (64, 8, 2)])
+def test_attention_weighs_fp16_queries_to_14_bits(d, heads, nq):
+    """Values of both signs that nearly cancel, so that the output's own rounding is small and what is
+    left are the probabilities' bits."""
+    gen = _gen(d + heads)
+    lengths = [2, 3, 4, 5, 6, 8, 10, 17] * 8
+    table, total = _pages(gen, lengths, 16)
+    cache = _finite_cache(gen, total, 1, 16, d)
+    v = cache.v.view(torch.uint8)
+    v[:, :, 1::2] = v[:, :, 0::2] ^ 0x80
+    q = _randn(gen, len(lengths), nq, heads, d, dtype=FP16, scale=0.05)
+    lengths = _int32(lengths)
+    got = ops.kv_attention(q, cache, table, lengths)
+    want, size = _attend_exact(q, cache, table, lengths, d ** -0.5, 0, 0)
+    # three e4m3 parts: the first leaves up to half its step, 2^-4, the second up to half the step of
+    # a number below 2^-4, 2^-9, the third 2^-14, of a probability in [1, 2); scores of a few units in
+    # fp32 and their exponentials are below 2^-16
+    off = (got.double() - want).abs() - (HALF[FP16] * want.abs() + (2.0 ** -14 + 2.0 ** -16) * size + 2.0 ** -25)
+    assert off.max() <= 0, off.max()
+
+
+@pytest.mark.parametrize("dtype, parts", [(BF16, 2), (FP16, 3)])
+def test_attention_of_queries_far_apart_in_size(dtype, parts):
+    """Elements far below their row's largest enter with the bits that e4m3's smallest steps leave them."""
+    gen = _gen(83)
+    table, total = _pages(gen, [90, 300], 32)
+    cache = _finite_cache(gen, total, 1, 32, 64)
+    lengths = _int32([90, 300])
+    for low in range(10, 25, 2):
+        q = _randn(gen, 2, 1, 4, 64, dtype=FP32) * 2.0 ** -low
+        q[..., 5] = 1.0
+        q = (q * 8).to(dtype)
+        cache.k.view(torch.uint8)[..., 5] = 0                     # the largest element meets nothing
+        got = ops.kv_attention(q, cache, table, lengths, scale=2.0 ** low / 64)
+        want, size = _attend_exact(q, cache, table, lengths, 2.0 ** low / 64, 0, 0)
+        # half a step of the last part: 2^-10 16^-(parts - 1) where the row's largest is at least 224; so
+        # much of 8 / 224 per element, times the keys' magnitudes (below 2^5 2^-5) and the scale: what a
+        # score may be off by, and with it a probability's logarithm
+        score = 2.0 ** -10 * 16.0 ** (1 - parts) * 8 / 224 * 64 * 2.0 ** low / 64
+        extra = {2: 2.0 ** -9, 3: 2.0 ** -11}[parts] + 2.0 ** -11 + 2.0 ** -14 + math.expm1(2 * score)
+        off = (got.double() - want).abs() - (HALF[dtype] * want.abs() + extra * size + 2.0 ** -25)
+        assert off.max() <= 0, (low, off.max())
