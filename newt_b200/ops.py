@@ -14,8 +14,11 @@ Each is one entry point of libnewt_b200.so (include/newt_b200.h holds the exact 
 torch's current stream.  Like the operator API's launcher they refuse tensors that are not on the
 current CUDA device.  Outputs that are not given, and the workspace of `kv_attention`, are fresh
 tensors of torch's caching allocator on the current stream, so calls on different streams share
-nothing.  None of them records anything for autograd; `token_logprobs` has its gradient as a
-function of its own.
+nothing.
+
+`token_logprobs` of logits that require a gradient is recorded for autograd; its gradient is also
+there as a function of its own.  The others have no backward pass: where gradients are enabled they
+refuse tensors that require one.
 """
 
 from typing import NamedTuple, Optional
@@ -117,6 +120,15 @@ def _vector(name, t, length, dtype):
         _refuse(name, t, (length,), dtype)
 
 
+def _no_backward(names, *tensors):
+    """Refuses what would lose a gradient without a word."""
+    if torch.is_grad_enabled():
+        for name, t in zip(names.split(), tensors):
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"tensor '{name}' requires a gradient, but this operator has no backward "
+                                   "pass; call it under torch.no_grad() or give it a detached tensor")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -134,7 +146,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
     `out_dtype` None: out = y in x's type.  torch.float8_e4m3fn: out = y / scale in 8 bits with
     scale = max|y| / 448 over the row (`group` 0; scales [rows, 1]) or over every `group` of 32, 64
     or 128 columns (scales [rows, ceil(n / group)]).  With a residual, h comes back in x's type.
-    `out` and `residual_out` may be x and residual themselves."""
+    `out` and `residual_out` may be x and residual themselves.  It has no backward pass."""
     shape, dtype = x.shape, x.dtype
     if len(shape) != 2:
         raise ValueError(f"'x' must be [rows, n], got {tuple(shape)}")
@@ -147,6 +159,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
         raise TypeError(f"rmsnorm: the output is {dtype} or float8_e4m3fn, not {out_dtype}")
     _rows("x", x, shape, dtype)
     _vector("weight", weight, n, dtype)
+    _no_backward("x weight residual out scales residual_out", x, weight, residual, out, scales, residual_out)
     if out is None:
         out = _fresh(x, out_dtype)
     else:
@@ -231,7 +244,8 @@ def kv_append(cache, k, v, page_table, starts, offsets, max_new):
 
     Scales are powers of two, one per page and head; a page that holds older tokens keeps its scale
     or gets a larger one, to which the older tokens are then brought.  Sequences must not share the
-    pages they write to.  Tokens whose page the table lacks are not written."""
+    pages they write to.  Tokens whose page the table lacks are not written.  It has no backward
+    pass."""
     packed = _pack_cache(cache)
     heads, d = cache.k.shape[1], cache.k.shape[3]
     shape, dtype = k.shape, k.dtype
@@ -245,6 +259,7 @@ def kv_append(cache, k, v, page_table, starts, offsets, max_new):
     _vector("starts", starts, batch, torch.int32)
     _vector("offsets", offsets, batch + 1, torch.int32)
     _page_table(page_table, batch)
+    _no_backward("k v cache.k_scales cache.v_scales", k, v, cache.k_scales, cache.v_scales)
     stream = _launch_stream(
         "k v page_table starts offsets cache.k cache.v cache.k_scales cache.v_scales", k, v,
         page_table, starts, offsets, cache.k, cache.v, cache.k_scales, cache.v_scales)
@@ -261,7 +276,8 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     lengths: int32 [batch], the tokens of each sequence in the cache, the new ones among them: query
     i of sequence b stands at position lengths[b] - queries + i and sees the tokens up to its own,
     with `window` > 0 only the last `window` of them and the first `sinks` of the sequence.  A query
-    that sees nothing gives zeros.  scale: 1 / sqrt(head_dim) if not given.  `out` must not be q."""
+    that sees nothing gives zeros.  scale: 1 / sqrt(head_dim) if not given.  `out` must not be q.  It has
+    no backward pass."""
     packed = _pack_cache(cache)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 4:
@@ -274,6 +290,7 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     _rows("q", q, shape, dtype)
     _vector("lengths", lengths, batch, torch.int32)
     _page_table(page_table, batch)
+    _no_backward("q cache.k_scales cache.v_scales out", q, cache.k_scales, cache.v_scales, out)
     if out is None:
         out = _fresh(q, dtype)
     else:
@@ -304,18 +321,14 @@ def _logits(logits):
     return shape
 
 
-def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
-    """Log probabilities of one given token per row of [rows, vocabulary] logits (fp32, fp16 or
-    bf16), each row's entropy and log-sum-exp, and its `top` (up to 32) largest alternatives with
-    their log probabilities, ties to the lower index.  tokens: int64 [rows]; a negative one stands
-    for none and scores 0.  Returns TokenLogprobs of fp32 tensors (top_index: int64)."""
-    rows, vocab = _logits(logits)
-    if tokens is not None:
-        _vector("tokens", tokens, rows, torch.int64)
-    if not 0 <= top <= 32:
-        raise ValueError(f"token_logprobs: {top} alternatives (0 to 32)")
+def _score(logits, tokens, top, inv_temperature, apart):
+    """TokenLogprobs of checked arguments; `apart`: no two results in one tensor."""
+    rows, vocab = logits.shape
     stream = _launch_stream("logits tokens", logits, tokens)
-    logprob, entropy, lse = logits.new_empty((3, rows), dtype=torch.float32).unbind(0)
+    if apart:
+        logprob, entropy, lse = (logits.new_empty(rows, dtype=torch.float32) for _ in range(3))
+    else:
+        logprob, entropy, lse = logits.new_empty((3, rows), dtype=torch.float32).unbind(0)
     if tokens is None:
         logprob = None
     best = index = None
@@ -329,11 +342,55 @@ def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
     return TokenLogprobs(logprob, entropy, lse, best, index)
 
 
+class _RecordedScore(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, inv_temperature):
+        got = _score(logits, tokens, top, inv_temperature, True)
+        ctx.save_for_backward(logits, tokens, got.lse, got.entropy)
+        ctx.inv_temperature = inv_temperature
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(got.top_index)
+        return tuple(got)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logprob, grad_entropy, grad_lse, grad_top, _):
+        if grad_lse is not None or grad_top is not None:
+            raise NotImplementedError("token_logprobs has a gradient of logprob and entropy, not of lse and "
+                                      "top_logprob: detach those")
+        if grad_logprob is None and grad_entropy is None:
+            return None, None, None, None
+        logits, tokens, lse, entropy = ctx.saved_tensors
+        # a sum's or a mean's gradient is one number for all rows
+        dense = [g if g is None else g.contiguous() for g in (grad_logprob, grad_entropy)]
+        return token_logprobs_backward(logits, tokens, lse, entropy, *dense,
+                                       inv_temperature=ctx.inv_temperature), None, None, None
+
+
+def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
+    """Log probabilities of one given token per row of [rows, vocabulary] logits (fp32, fp16 or
+    bf16), each row's entropy and log-sum-exp, and its `top` (up to 32) largest alternatives with
+    their log probabilities, ties to the lower index.  tokens: int64 [rows]; a negative one stands
+    for none and scores 0.  Returns TokenLogprobs of fp32 tensors (top_index: int64).
+
+    Where gradients are enabled and the logits require one, logprob and entropy can be
+    differentiated (once; the logits are kept until then); a gradient of lse or top_logprob is refused."""
+    rows, vocab = _logits(logits)
+    if tokens is not None:
+        _vector("tokens", tokens, rows, torch.int64)
+    if not 0 <= top <= 32:
+        raise ValueError(f"token_logprobs: {top} alternatives (0 to 32)")
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_RecordedScore.apply(logits, tokens, top, inv_temperature))
+    return _score(logits, tokens, top, inv_temperature, False)
+
+
 def token_logprobs_backward(logits, tokens, lse, entropy, grad_logprob=None, grad_entropy=None,
                             inv_temperature=1.0, out=None):
     """The gradient of `token_logprobs` by its logits, in their type: of sum(grad_logprob * logprob)
     + sum(grad_entropy * entropy), with the lse and entropy that it returned.  `out` may be the
-    logits themselves."""
+    logits themselves.  Not recorded for autograd: there is no second derivative."""
     rows, vocab = _logits(logits)
     if tokens is not None:
         _vector("tokens", tokens, rows, torch.int64)
@@ -347,6 +404,8 @@ def token_logprobs_backward(logits, tokens, lse, entropy, grad_logprob=None, gra
         out = _fresh(logits, logits.dtype)
     else:
         _written("out", out, (rows, vocab), logits.dtype)
+        if out is not logits:
+            _no_backward("out", out)
     stream = _launch_stream("logits tokens lse entropy grad_logprob grad_entropy out", logits, tokens,
                             lse, entropy, grad_logprob, grad_entropy, out)
     abi.check(abi.load().nb200_token_logprobs_bwd(

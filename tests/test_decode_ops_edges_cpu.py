@@ -4,7 +4,11 @@ index arithmetic compiled for the host, and refusals."""
 import os
 import subprocess
 
+import pytest
+import torch
+
 import newt_b200
+from newt_b200 import ops
 
 CSRC = os.path.join(os.path.dirname(newt_b200.__file__), "csrc")
 
@@ -60,3 +64,30 @@ def test_columns_of_shifted_rows_and_their_groups(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-I", CSRC, str(source), "-o", str(program)], check=True)
     done = subprocess.run([str(program)], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_calls_that_would_lose_a_gradient_are_refused():
+    x, w = torch.zeros(4, 64), torch.zeros(64)
+    cache = ops.new_kv_cache(8, 2, 16, 64, device="cpu")
+    kv = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    table = torch.zeros(2, 4, dtype=torch.int32)
+    lengths, offsets = torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    q = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16)
+
+    def wants(t):
+        return t.clone().requires_grad_()
+
+    calls = {"x": lambda: ops.rmsnorm(wants(x), w), "weight": lambda: ops.rmsnorm(x, torch.nn.Parameter(w)),
+             "residual": lambda: ops.rmsnorm(x, w, residual=wants(x)), "out": lambda: ops.rmsnorm(x, w, out=wants(x)),
+             "k": lambda: ops.kv_append(cache, wants(kv), kv, table, lengths, offsets, 1),
+             "v": lambda: ops.kv_append(cache, kv, wants(kv), table, lengths, offsets, 1),
+             "q": lambda: ops.kv_attention(wants(q), cache, table, lengths),
+             "cache.v_scales": lambda: ops.kv_attention(
+                 q, cache._replace(v_scales=wants(cache.v_scales)), table, lengths)}
+    for name, call in calls.items():
+        with pytest.raises(RuntimeError, match=f"'{name}' requires a gradient.*no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(TypeError, match="must be a CUDA tensor"):   # the next check
+            call()
+        with torch.inference_mode(), pytest.raises(TypeError, match="must be a CUDA tensor"):
+            call()

@@ -113,6 +113,92 @@ def test_token_logprobs_backward_of_large_logits():
     assert torch.isnan(got[0]).all() and torch.isfinite(got[1:]).all()
 
 
+def _scores(x, tokens, inv):
+    """logprob and entropy in 64 bits, for torch to differentiate."""
+    log_p = torch.log_softmax(x * inv, 1)
+    p = log_p.exp()
+    entropy = -torch.where(p > 0, p * log_p, 0.0).sum(1)
+    picked = log_p.gather(1, tokens.clamp(min=0)[:, None])[:, 0]
+    return torch.where(tokens < 0, 0.0, picked), entropy
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("top", [0, 4])
+def test_token_logprobs_is_differentiated(dtype, top):
+    """A training loss through autograd, against the definition differentiated in 64 bits."""
+    gen = _gen(95 + top)
+    wide = _randn(gen, 33, 1200, dtype=dtype, scale=2.0)
+    tokens = torch.randint(0, 1003, (33,), generator=gen, device="cuda")
+    tokens[::5] = -100
+    weight = _randn(gen, 33)
+    losses = {
+        "sum": lambda lp, h: -lp.sum() + 0.1 * h.mean(),              # gradients that are broadcast
+        "weighted": lambda lp, h: (lp * weight).sum() - (0.01 * h * weight).sum(),
+        "logprob": lambda lp, h: lp[::2].mean(), "entropy": lambda lp, h: h.square().sum()}
+    for name, loss in losses.items():
+        leaf = wide.clone().requires_grad_()
+        x = leaf[:, 5:1008]                                           # rows that lie apart, off a boundary
+        s = ops.token_logprobs(x, tokens, top=top, inv_temperature=0.8)
+        with torch.no_grad():
+            plain = ops.token_logprobs(x, tokens, top=top, inv_temperature=0.8)
+        assert not plain.logprob.requires_grad
+        assert all(a is None and b is None or torch.equal(a, b) for a, b in zip(s, plain))
+        loss(s.logprob, s.entropy).backward()
+        exactly = wide[:, 5:1008].double().requires_grad_()
+        loss(*_scores(exactly, tokens, torch.tensor(0.8).double().item())).backward()
+        got, want = leaf.grad[:, 5:1008].double(), exactly.grad
+        # one rounding to the logits' type; before it p is off by 2^-19 of itself, times weights of a
+        # few units and brackets of up to 2^4, and entropies of up to 7 that are differentiated
+        off = (got - want).abs() - (HALF[dtype] * want.abs() + 2.0 ** -14 * want.abs().amax(1, keepdim=True) + 2.0 ** -25)
+        assert off.max() <= 0, (name, off.max())
+        assert (leaf.grad[:, :5] == 0).all() and (leaf.grad[:, 1008:] == 0).all()
+
+
+def test_what_token_logprobs_cannot_differentiate_is_refused():
+    gen = _gen(96)
+    x = _randn(gen, 4, 100).requires_grad_()
+    tokens = torch.tensor([1, 2, 3, -1], device="cuda")
+    for pick in (lambda s: s.lse, lambda s: s.top_logprob):
+        s = ops.token_logprobs(x, tokens, top=3)
+        with pytest.raises(NotImplementedError, match="lse and top_logprob"):
+            (pick(s).sum() + s.logprob.sum()).backward()
+    s = ops.token_logprobs(x, tokens, top=3)
+    assert not s.top_index.requires_grad
+    grad, = torch.autograd.grad(s.logprob.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+    bare = ops.token_logprobs(x)                       # no tokens: the entropy alone
+    assert bare.logprob is None
+    bare.entropy.sum().backward()
+    assert torch.isfinite(x.grad).all()
+
+
+def test_token_logprobs_is_differentiated_in_a_graph_and_on_another_stream():
+    gen = _gen(98)
+    x = _randn(gen, 40, 5001, dtype=BF16).requires_grad_()
+    tokens = torch.randint(0, 5001, (40,), generator=gen, device="cuda")
+
+    def step():
+        s = ops.token_logprobs(x, tokens, inv_temperature=1.25)
+        return torch.autograd.grad((s.logprob + 0.1 * s.entropy).sum(), x)[0]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        x.copy_(_randn(gen, 40, 5001, dtype=BF16))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, step()) and not torch.equal(got, want)
+
+
 # ---- rmsnorm -----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("group", [0, 32, 128])
