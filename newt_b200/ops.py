@@ -18,12 +18,13 @@ nothing.
 
 `token_logprobs` of logits that require a gradient is recorded for autograd; its gradient is also
 there as a function of its own.  The others have no backward pass: where gradients are enabled they
-refuse tensors that require one.
+refuse tensors that require one.  Tensors that a call writes over count as modified in place.
 """
 
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .runtime import abi
 
@@ -160,6 +161,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
     _rows("x", x, shape, dtype)
     _vector("weight", weight, n, dtype)
     _no_backward("x weight residual out scales residual_out", x, weight, residual, out, scales, residual_out)
+    given = [t for t in (out, scales, residual_out) if t is not None]
     if out is None:
         out = _fresh(x, out_dtype)
     else:
@@ -193,6 +195,8 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
         x.data_ptr(), _ptr(residual), weight.data_ptr(), out.data_ptr(), _ptr(residual_out),
         _ptr(scales), rows, n, x.stride(0), residual_stride, out.stride(0), residual_out_stride,
         scale_stride, group, eps, _CODES[dtype], _CODES[out_dtype], stream))
+    if given:
+        increment_version(given)
     return RmsNorm(out, scales, residual_out)
 
 
@@ -267,6 +271,7 @@ def kv_append(cache, k, v, page_table, starts, offsets, max_new):
         packed, k.data_ptr(), v.data_ptr(), shape[0], k.stride(0), k.stride(1), v.stride(0),
         v.stride(1), page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
         starts.data_ptr(), offsets.data_ptr(), batch, max_new, _CODES[dtype], stream))
+    increment_version(cache)
 
 
 def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, out=None):
@@ -291,10 +296,11 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
     _vector("lengths", lengths, batch, torch.int32)
     _page_table(page_table, batch)
     _no_backward("q cache.k_scales cache.v_scales out", q, cache.k_scales, cache.v_scales, out)
-    if out is None:
-        out = _fresh(q, dtype)
-    else:
+    given = out is not None
+    if given:
         _written("out", out, shape, dtype)
+    else:
+        out = _fresh(q, dtype)
     stream = _launch_stream(
         "q page_table lengths out cache.k cache.v cache.k_scales cache.v_scales", q, page_table,
         lengths, out, cache.k, cache.v, cache.k_scales, cache.v_scales)
@@ -308,6 +314,8 @@ def kv_attention(q, cache, page_table, lengths, scale=None, window=0, sinks=0, o
         q.data_ptr(), packed, out.data_ptr(), batch, queries, heads, qb, qt, qh, ob, ot, oh,
         page_table.data_ptr(), page_table.stride(0), pages, lengths.data_ptr(),
         d ** -0.5 if scale is None else scale, window, sinks, code, _ptr(ws), need, stream))
+    if given:
+        increment_version(out)
     return out
 
 
@@ -400,16 +408,19 @@ def token_logprobs_backward(logits, tokens, lse, entropy, grad_logprob=None, gra
         _vector("grad_logprob", grad_logprob, rows, torch.float32)
     if grad_entropy is not None:
         _vector("grad_entropy", grad_entropy, rows, torch.float32)
-    if out is None:
-        out = _fresh(logits, logits.dtype)
-    else:
+    given = out is not None
+    if given:
         _written("out", out, (rows, vocab), logits.dtype)
         if out is not logits:
             _no_backward("out", out)
+    else:
+        out = _fresh(logits, logits.dtype)
     stream = _launch_stream("logits tokens lse entropy grad_logprob grad_entropy out", logits, tokens,
                             lse, entropy, grad_logprob, grad_entropy, out)
     abi.check(abi.load().nb200_token_logprobs_bwd(
         logits.data_ptr(), _ptr(tokens), _ptr(lse), _ptr(entropy), _ptr(grad_logprob),
         _ptr(grad_entropy), out.data_ptr(), rows, vocab, logits.stride(0), out.stride(0),
         inv_temperature, _CODES[logits.dtype], stream))
+    if given:
+        increment_version(out)
     return out

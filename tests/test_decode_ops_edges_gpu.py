@@ -167,10 +167,39 @@ def test_what_token_logprobs_cannot_differentiate_is_refused():
     grad, = torch.autograd.grad(s.logprob.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+    y = x * 1.0
+    s = ops.token_logprobs(y, tokens)
+    ops.token_logprobs_backward(y.detach(), tokens, s.lse.detach(), s.entropy.detach(),
+                                torch.ones(4, device="cuda"), out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        s.logprob.sum().backward()
     bare = ops.token_logprobs(x)                       # no tokens: the entropy alone
     assert bare.logprob is None
     bare.entropy.sum().backward()
     assert torch.isfinite(x.grad).all()
+
+
+def test_writes_count_as_modifications():
+    gen = _gen(97)
+    x, w = _randn(gen, 4, 64, dtype=BF16), _randn(gen, 64, dtype=BF16)
+    out, scales, h = torch.empty_like(x, dtype=ops.E4M3), torch.empty(4, 1, device="cuda"), torch.empty_like(x)
+    before = [t._version for t in (out, scales, h, x)]
+    ops.rmsnorm(x, w, residual=x, out_dtype=ops.E4M3, out=out, scales=scales, residual_out=h)
+    assert [t._version for t in (out, scales, h, x)] == [before[0] + 1, before[1] + 1, before[2] + 1, before[3]]
+    cache = ops.new_kv_cache(4, 1, 16, 64)
+    before = [t._version for t in cache]
+    k = _randn(gen, 3, 1, 64, dtype=BF16)
+    ops.kv_append(cache, k, k, _int32([[0]]), _int32([0]), _int32([0, 3]), 3)
+    assert [t._version for t in cache] == [n + 1 for n in before]
+    q = _randn(gen, 1, 1, 2, 64, dtype=BF16)
+    o = torch.empty_like(q)
+    version = o._version
+    ops.kv_attention(q, cache, _int32([[0]]), _int32([3]), out=o)
+    assert o._version == version + 1
+    with torch.inference_mode():                       # tensors without a version are written too
+        cache = ops.new_kv_cache(4, 1, 16, 64)
+    ops.kv_append(cache, k, k, _int32([[0]]), _int32([0]), _int32([0, 3]), 3)
+    assert torch.equal(ops.kv_attention(q, cache, _int32([[0]]), _int32([3])), o)
 
 
 def test_token_logprobs_is_differentiated_in_a_graph_and_on_another_stream():
