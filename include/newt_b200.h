@@ -291,6 +291,8 @@ int nb200_attention_fwd(const void* q, const void* k, const void* v, void* o,
                         int64_t o_head_stride, int64_t o_row_stride,
                         float scale, int causal, int dtype, void* stream);
 
+/* From here on every tensor starts on a multiple of its element's size; what does not is refused. */
+
 /* ---- root-mean-square norm of rows ------------------------------------------
  *   h = x + residual (fp32; `residual` null: h = x)
  *   y = h * rsqrt(mean(h^2) + eps) * w

@@ -60,6 +60,14 @@ int prepare_kernel(const void* kernel, int smem_bytes);
 int cluster_capacity(const void* kernel, const cudaLaunchConfig_t* config, int* clusters);
 
 static inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Do all of these (null: not given) start on a multiple of `bytes`, a power of two?  What does not is
+// refused: a kernel's access to it would fault the GPU.
+template <class... P>
+static inline bool aligned_to(size_t bytes, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0;
+}
+static inline size_t bytes_of(int dtype) { return dtype == NB200_F32 ? 4 : dtype == NB200_E4M3 ? 1 : 2; }
 #endif  // !__CUDACC_RTC__
 
 // ---- device side -----------------------------------------------------------

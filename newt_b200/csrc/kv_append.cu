@@ -265,6 +265,8 @@ extern "C" int nb200_kv_append(const nb200_kv_cache* cache, const void* k, const
   if (tokens == 0 || batch == 0 || max_new == 0 || max_pages == 0 || cache->pages == 0) return 0;
   if (!k || !v || !page_table || !starts || !offsets)
     return fail(NB200_E_INVALID, "kv append: null tensor pointer");
+  if (!aligned_to(2, k, v) || !aligned_to(4, page_table, starts, offsets))
+    return fail(NB200_E_INVALID, "kv append: a tensor does not start on a multiple of its element");
   if (max_new > tokens) max_new = tokens;
   // a run of max_new tokens touches at most this many pages, of max_pages that there are
   int64_t slots = (max_new + cache->page_size - 2) / cache->page_size + 1;

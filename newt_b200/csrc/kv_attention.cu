@@ -1183,6 +1183,8 @@ extern "C" int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, vo
     return fail(NB200_E_INVALID, "kv attention: scale must be positive and finite");
   if (!q || !out || !lengths || (max_pages > 0 && !page_table))
     return fail(NB200_E_INVALID, "kv attention: null tensor pointer");
+  if (!aligned_to(2, q, out) || !aligned_to(4, page_table, lengths))
+    return fail(NB200_E_INVALID, "kv attention: a tensor does not start on a multiple of its element");
   if (q == out) return fail(NB200_E_INVALID, "kv attention: out must not be q, which other blocks still read");
   if (cache->pages == 0) return fail(NB200_E_INVALID, "kv attention: the cache has no pages");
   const int64_t need = nb200_kv_attention_workspace_bytes(cache, batch, queries, heads, max_pages, dtype);

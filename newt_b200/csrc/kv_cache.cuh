@@ -21,6 +21,8 @@ static inline int check_kv_cache(const char* what, const nb200_kv_cache* c) {
     return fail(NB200_E_INVALID, "%s: null cache pointer", what);
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
     return fail(NB200_E_UNSUPPORTED, "%s: the cache must be 16-byte aligned", what);
+  if (!aligned_to(4, c->k_scales, c->v_scales))
+    return fail(NB200_E_INVALID, "%s: the scales do not start on a multiple of their element", what);
   const int64_t strides[6] = {c->k_page_stride, c->k_head_stride, c->k_token_stride,
                               c->v_page_stride, c->v_head_stride, c->v_token_stride};
   for (int i = 0; i < 6; ++i)

@@ -735,6 +735,9 @@ extern "C" int nb200_token_logprobs(const void* logits, const int64_t* tokens, f
                 (long long)vocab);
   if (!logits || (logprob && !tokens) || (top > 0 && (!top_logprob || !top_index)))
     return fail(NB200_E_INVALID, "token logprobs: null tensor pointer");
+  if (!aligned_to(bytes_of(dtype), logits) || !aligned_to(8, tokens, top_index) ||
+      !aligned_to(4, logprob, entropy, lse, top_logprob))
+    return fail(NB200_E_INVALID, "token logprobs: a tensor does not start on a multiple of its element");
   LogprobParams p{logits, tokens, logprob, entropy, lse, top_logprob, top_index, stride, (int)rows,
                   (int)vocab, (int)top, inv_temperature, fmaxf(kLowest, -1e38f / (inv_temperature * kLog2e))};
   switch (dtype) {
@@ -758,6 +761,9 @@ extern "C" int nb200_token_logprobs_bwd(const void* logits, const int64_t* token
   if (rows == 0 || vocab == 0) return 0;
   if (!logits || !lse || !grad_logits || (grad_logprob && !tokens) || (grad_entropy && !entropy))
     return fail(NB200_E_INVALID, "token logprobs gradient: null tensor pointer");
+  if (!aligned_to(bytes_of(dtype), logits, grad_logits) || !aligned_to(8, tokens) ||
+      !aligned_to(4, lse, entropy, grad_logprob, grad_entropy))
+    return fail(NB200_E_INVALID, "token logprobs gradient: a tensor does not start on a multiple of its element");
   GradParams p{logits, tokens, lse, entropy, grad_logprob, grad_entropy, grad_logits, stride,
                stride_out, (int)rows, (int)vocab, inv_temperature};
   switch (dtype) {

@@ -414,6 +414,8 @@ extern "C" int nb200_rmsnorm(const void* x, const void* residual, const void* w,
   if (rows == 0 || (n == 0 && !(e4m3 && group == 0))) return 0;     // rows without columns still have a scale each
   if ((n > 0 && (!x || !w || !out)) || (e4m3 && !scales))
     return fail(NB200_E_INVALID, "rmsnorm: null tensor pointer");
+  if (!aligned_to(bytes_of(dtype), x, residual, w, residual_out) || !aligned_to(bytes_of(out_dtype), out) || !aligned_to(4, scales))
+    return fail(NB200_E_INVALID, "rmsnorm: a tensor does not start on a multiple of its element");
   RmsParams p;
   p.x = x;
   p.residual = residual;

@@ -9,6 +9,8 @@ import torch
 
 import newt_b200
 from newt_b200 import ops
+from newt_b200.runtime import abi
+from test_decode_ops_cpu import P, _append, _attend, _cache, _grad, _rms, _score
 
 CSRC = os.path.join(os.path.dirname(newt_b200.__file__), "csrc")
 
@@ -91,3 +93,20 @@ def test_calls_that_would_lose_a_gradient_are_refused():
             call()
         with torch.inference_mode(), pytest.raises(TypeError, match="must be a CUDA tensor"):
             call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: _rms(x=P + 1), lambda: _rms(w=P + 1), lambda: _rms(out=P + 1), lambda: _rms(res=P + 1),
+    lambda: _rms(res=P, res_out=P + 1), lambda: _rms(x=P + 2, dtype=abi.F32, out_dtype=abi.F32),
+    lambda: _rms(out_dtype=abi.E4M3, scales=P + 2), lambda: _append(_cache(ks=P + 2)),
+    lambda: _append(k=P + 1), lambda: _append(v=P + 1), lambda: _append(table=P + 2),
+    lambda: _append(starts=P + 1), lambda: _append(offsets=P + 2), lambda: _attend(_cache(vs=P + 1)),
+    lambda: _attend(q=P + 1), lambda: _attend(out=P + 1), lambda: _attend(table=P + 2),
+    lambda: _attend(lengths=P + 2), lambda: _score(logits=P + 2), lambda: _score(logits=P + 1, dtype=abi.F16),
+    lambda: _score(tokens=P + 4), lambda: _score(logprob=P + 2), lambda: _score(top=2, best=P, index=P + 4),
+    lambda: _score(top=2, best=P + 1, index=P), lambda: _grad(logits=P + 2), lambda: _grad(out=P + 3),
+    lambda: _grad(tokens=P + 4), lambda: _grad(lse=P + 1), lambda: _grad(entropy=P + 2), lambda: _grad(g=P + 2),
+    lambda: _grad(ge=P + 1, dtype=abi.BF16)])
+def test_the_library_refuses_what_does_not_start_on_an_element(call):
+    assert call() == abi.E_INVALID
+    assert "multiple of" in abi.last_error()
