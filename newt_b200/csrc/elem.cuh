@@ -99,6 +99,14 @@ __device__ __forceinline__ float2 e4m3x2_values(uint32_t q) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// Exponent of the smallest power of two s with most <= 448 s, 448 = 1.75 * 2^8 being e4m3's largest
+// number: exact, from the bits.  0 and subnormals: -135.
+__device__ __forceinline__ int e4m3_exponent(float most) {
+  const uint32_t b = __float_as_uint(most);
+  return (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 to 127
+
 // E values times `factor` as e4m3; `to` is E-byte aligned.
 template <int E>
 __device__ __forceinline__ void store_e4m3(uint8_t* to, const float* v, float factor) {

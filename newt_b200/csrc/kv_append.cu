@@ -37,13 +37,10 @@ struct AppendParams {
   int aligned[2];                  // 16-byte vectors may be read
 };
 
-// Exponent of the smallest power of two s with most <= 448 s: 448 = 1.75 * 2^8.
-__device__ __forceinline__ int scale_exponent(float most) {
-  const uint32_t b = __float_as_uint(most);
-  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < kMinExponent ? kMinExponent : e > kMaxExponent ? kMaxExponent : e;
+// What a page needs for new tokens of this largest magnitude.
+__device__ __forceinline__ float scale_for(float most) {
+  return power_of_two(min(max(e4m3_exponent(most), kMinExponent), kMaxExponent));
 }
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // Largest magnitude of a vector; skips NaN.
 __device__ __forceinline__ float largest_of(const Vec<__nv_bfloat16>& v) {
@@ -141,7 +138,7 @@ __global__ void __launch_bounds__(256) kv_append_few_kernel(const AppendParams p
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) most = fmaxf(most, largest_of(raw[i]));
   most = sm100::warp_max(most);
-  const float after = fmaxf(power_of_two(scale_exponent(most)), before);
+  const float after = fmaxf(scale_for(most), before);
   const float inv = 1.0f / after;
   __syncwarp();          // everyone has read the old scale
   if (lane == 0) *scale = after;
@@ -206,7 +203,7 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(const AppendParams p)
   __syncthreads();                  // everyone has read the old scale
   most = sm100::warp_max((threadIdx.x & 31) < (blockDim.x >> 5) ? slots[threadIdx.x & 7] : 0.0f);
 
-  const float after = fmaxf(power_of_two(scale_exponent(most)), before);
+  const float after = fmaxf(scale_for(most), before);
   const float inv = 1.0f / after;
   if (threadIdx.x == 0) *scale = after;
   out += token0 * out_token;

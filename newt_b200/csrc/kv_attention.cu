@@ -386,15 +386,12 @@ __device__ __noinline__ void stage_queries(const KvAttnParams& p, Vec<T> raw, in
     bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
   }
   if (r >= RP) return;
-  // most <= 448 * 2^e: 448 = 1.75 * 2^8
-  const uint32_t bits = __float_as_uint(most);
-  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  e = max(e, -100);
-  const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+  const int e = max(e4m3_exponent(most), -100);    // most <= 448 * 2^e
+  const float down = power_of_two(-e);
   if (col8 == 0) {
     const int row = row_tile * RP + r;
     const bool is = row < p.rows;
-    factor[r] = bad ? NAN : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale * kLog2e);
+    factor[r] = bad ? NAN : power_of_two(e) * (p.scale * kLog2e);
     at[r] = is ? first_at + row / p.group : -1;
     out[r] = is ? row / p.group * p.o_token_stride + row % p.group * p.o_head_stride : -1;
   }
