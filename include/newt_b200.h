@@ -382,8 +382,9 @@ int nb200_kv_attention(const void* q, const nb200_kv_cache* cache, void* out, in
  * indices int64.  A negative token stands for none: logprob 0; one beyond the vocabulary gives
  * NaN.  A row of nothing but -inf: logprobs and lse -inf, entropy 0.  A row with NaN or +inf gives NaN.
  * `inv_temperature` is between 1e-20 and 1e20.  tokens / logprob, entropy and lse may be null where
- * they are not wanted.  One pass over the row;
- * results do not depend on the launch's other rows. */
+ * they are not wanted.  One pass over the row.  A row's results are the same in every call of the same
+ * shape, whatever the other rows hold; the number of rows decides how a row is spread over the chip and
+ * may change the last bits. */
 int nb200_token_logprobs(const void* logits, const int64_t* tokens, float* logprob, float* entropy,
                          float* lse, float* top_logprob, int64_t* top_index, int64_t rows,
                          int64_t vocab, int64_t stride, int64_t top, float inv_temperature,

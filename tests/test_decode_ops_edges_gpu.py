@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from newt_b200 import ops
+from newt_b200.examples import kernels
 from newt_b200.runtime import abi
 from test_decode_ops_gpu import (BF16, FP16, FP32, HALF, _attend_exact, _finite_cache, _gen, _int32, _pages, _randn,
                                  _score_exact)
@@ -228,6 +229,45 @@ def test_token_logprobs_is_differentiated_in_a_graph_and_on_another_stream():
     assert torch.equal(got, step()) and not torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("vocab", [1003, 50021])
+def test_a_row_scores_alike_beside_other_rows(vocab, dtype):
+    """The same bits whatever the rows beside it hold, and close ones in calls of other numbers of rows."""
+    gen = _gen(vocab)
+    row = _randn(gen, 1, vocab, dtype=dtype, scale=3.0)
+    one = torch.tensor([17], device="cuda")
+    alone = ops.token_logprobs(row, one, top=5)
+    for rows in (2, 37, 200, 300, 700):
+        results = []
+        for _ in range(2):
+            x = _randn(gen, rows, vocab, dtype=dtype, scale=3.0)
+            x[rows // 2] = row
+            got = ops.token_logprobs(x, one.expand(rows).contiguous(), top=5)
+            results.append([t[rows // 2] for t in got])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+        assert torch.equal(results[0][4], alone.top_index[0])
+        for got, want in zip(results[0][:4], alone[:4]):
+            # twice the sums' error
+            _agree(got, want[0].double(), 2.0 ** -20, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_rows_that_are_not_finite_score_so(bad):
+    """NaN and infinities where the definition has them, whatever path a row takes."""
+    gen = _gen(99)
+    for rows, vocab in ((3, 1003), (300, 1003), (2, 50021), (160, 33)):
+        for dtype in (BF16, FP16, FP32):
+            x = _randn(gen, rows, vocab, dtype=dtype)
+            x[1, vocab // 3] = bad
+            tokens = torch.full((rows,), 3, dtype=torch.int64, device="cuda")
+            got = ops.token_logprobs(x, tokens, top=3)
+            logprob, entropy, lse, _ = _score_exact(x, tokens, 1.0)
+            if bad != -math.inf:
+                logprob[1] = entropy[1] = lse[1] = math.nan       # no probability is defined
+            for mine, want in ((got.logprob, logprob), (got.entropy, entropy), (got.lse, lse)):
+                _agree(mine, want, 2.0 ** -21, 2.0 ** -18)
+
+
 # ---- rmsnorm -----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("group", [0, 32, 128])
@@ -259,6 +299,40 @@ def test_rmsnorm_of_rows_without_columns():
     assert got.out.shape == (3, 0) and (scales == 1).all()          # the scale of nothing
     assert ops.rmsnorm(x, w, out_dtype=ops.E4M3, group=32).scales.shape == (3, 0)
     assert ops.rmsnorm(x, w).out.shape == (3, 0)
+
+
+@pytest.mark.parametrize("rows, n", [(3, 64), (700, 1003), (5, 4096)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_rmsnorm_of_rows_that_are_not_finite(bad, rows, n):
+    """NaN and infinities where the formula has them: every output of a row with NaN, and where a row's
+    infinity is; its other outputs are 0."""
+    gen = _gen(rows + n)
+    for dtype in (BF16, FP16, FP32):
+        x, w = _randn(gen, rows, n, dtype=dtype), _randn(gen, n, dtype=dtype)
+        x[1, n // 2] = bad
+        h = x.double()
+        want = h / (h.square().mean(1, keepdim=True) + 1e-6).sqrt() * w.double()
+        got = ops.rmsnorm(x, w)
+        _agree(got.out, want, HALF[dtype] + 2.0 ** -17, 2.0 ** -24)
+        got = ops.rmsnorm(x, w, residual=torch.zeros_like(x))
+        _agree(got.residual, h, 0.0, 0.0)
+        for group in (0, 32):
+            got = ops.rmsnorm(x, w, out_dtype=ops.E4M3, group=group)
+            keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+            keep[1] = False
+            assert torch.isfinite(got.out.float()[keep]).all() and torch.isfinite(got.scales[keep]).all()
+            nan = torch.isnan(got.out.float()[1])
+            assert nan.all() if math.isnan(bad) else nan.nonzero().tolist() == [[n // 2]]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_rmsnorm_agrees_with_the_generated_kernel(dtype):
+    """The same norm through the block language: fp32 sums on both sides, one rounding each."""
+    gen = _gen(12)
+    for rows, n in ((7, 64), (300, 1000), (64, 4096)):
+        x, w = _randn(gen, rows, n, dtype=dtype), _randn(gen, n, dtype=dtype)
+        mine, other = ops.rmsnorm(x, w, eps=1e-5).out, kernels.rmsnorm(x, w, eps=1e-5)
+        _agree(mine, other, 2 * HALF[dtype] + 2.0 ** -16, 2.0 ** -24)
 
 
 # ---- attention over the cache ------------------------------------------------------------------
