@@ -301,6 +301,35 @@ def test_rmsnorm_of_rows_without_columns():
     assert ops.rmsnorm(x, w).out.shape == (3, 0)
 
 
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows, n", [(1, 1), (3, 64), (700, 100), (5, 1003), (700, 1003), (2, 4096), (300, 8192),
+                                     (2, 32768), (2, 32761)])
+def test_rmsnorm_of_rows_whose_squares_leave_the_range(rows, n, dtype, with_residual):
+    """Values whose squares are infinite or 0 in fp32, beside ordinary rows of the same call."""
+    gen = _gen(rows + n)
+    sizes = [1.0, 1e18, 3e19, 1e30, 1e37, 1e-18, 1e-22, 1e-30, 1e-36, 1.0]
+    x = _randn(gen, rows, n).clamp(-3, 3)
+    x = (x * torch.tensor([sizes[(i + n) % len(sizes)] for i in range(rows)], device="cuda")[:, None]).to(dtype)
+    residual = (x * _randn(gen, rows, 1).clamp(-3, 3)).to(dtype) if with_residual else None
+    w = _randn(gen, n, dtype=dtype)
+    for eps in (0.0, 1e-40, 1e-12, 1e-6):
+        eps = torch.tensor(eps, dtype=FP32).item()
+        h = x.double() + (residual.double() if with_residual else 0.0)
+        want = h / (h.square().mean(1, keepdim=True) + eps).sqrt() * w.double()
+        got = ops.rmsnorm(x, w, residual=residual, eps=eps)
+        # fp32's own sum of x and the residual: 2^-24 of the larger, relative to the row's size
+        slack = 2.0 ** -23 * want.abs().amax(1, keepdim=True) if with_residual else 0.0
+        off = (got.out.double() - want).abs() - ((HALF[dtype] + 2.0 ** -17) * want.abs() + 4 * slack + 1e-38)
+        assert off.max() <= 0, (eps, off.max())
+        if with_residual:
+            _agree(got.residual, h, HALF[dtype] + 2.0 ** -23, 1e-38)
+        got = ops.rmsnorm(x, w, residual=residual, eps=eps, out_dtype=ops.E4M3, group=32)
+        scales = torch.stack([part.abs().amax(1) / 448 for part in want.split(32, 1)], 1)
+        usual = scales > 1.2e-38
+        assert ((got.scales.double() - scales).abs()[usual] <= (2.0 ** -16 * scales + (slack if with_residual else 0.0))[usual]).all()
+
+
 @pytest.mark.parametrize("rows, n", [(3, 64), (700, 1003), (5, 4096)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_rmsnorm_of_rows_that_are_not_finite(bad, rows, n):
