@@ -299,7 +299,8 @@ int nb200_attention_fwd(const void* q, const void* k, const void* v, void* o,
  * `out`: y in `dtype` (out_dtype == dtype), or in e4m3 (out_dtype == NB200_E4M3) as y / s with
  * s = max|y| / 448 over the row (`group` 0) or over each `group` consecutive columns (32, 64 or
  * 128; the last group of a row may be shorter); s = 1 where that quotient is zero or below the
- * normal range.  `scales` is [rows, ceil(n / group)], row stride `stride_scales`; null for
+ * normal range.  The quotients are within 2^-22: a value next to the middle between two e4m3 numbers
+ * may go to either.  `scales` is [rows, ceil(n / group)], row stride `stride_scales`; null for
  * 16/32-bit outputs.  `residual_out` (null: not wanted): h in `dtype`.  One rounding per output.
  * `out` and `residual_out` may be the very tensors x and residual (same base and strides); no
  * other overlap.  Rows of up to 32768 elements, any alignment (16-byte aligned rows of whole vectors

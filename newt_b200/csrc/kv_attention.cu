@@ -16,7 +16,7 @@
 // so that much is true of elements down to 2^-14 of the row's largest (bf16; fp16 2^-15); of smaller
 // ones e4m3's smallest step leaves an error of 2^-22 of the largest (fp16 2^-26).  Probabilities
 // keep 9 bits (two parts) or 14 (three): one more than a bf16 output has, three more than an fp16 one
-// (11 with the first part taken from fp16 too: 31 sequences, 28 rows in fp16, 93.7 us, with 14 94.4).
+// (11 with the first part taken from fp16 too: 32 sequences with a window of 2048 in fp16 26.1 us, with 14 26.4).
 // The sums of a row take them unrounded: a token whose value scale is far below its tile's
 // largest rounds to nothing in the product, but weighs no less.  N = parts * rows, at least 16, was idle
 // anyway.
@@ -42,7 +42,7 @@
 //
 // What bounds it: HBM where there is enough of it to do (64 sequences of 4 to 8 thousand tokens, 8 key
 // heads of 128 in bf16: 132 us, 6.1 TB/s; the sums of 16 rows a key head in fp16 keep the softmax
-// threads busier than HBM: 31 sequences of 11 to 22 thousand tokens, 28 rows, 87 us, a quarter of HBM's
+// threads busier than HBM: 31 sequences of 11 to 22 thousand tokens, 28 rows, 90 us, a quarter of HBM's
 // rate, with issue slots half used and the rest spent on the exchange of the maxima); below some 20 us
 // the chain length -> page -> tile -> scores -> probabilities -> sums, 6.5 us for one sequence of 100 tokens.
 // Some 1.5 of them pass until a block knows its share, 1.5 until its first page is asked for and 1 to 2

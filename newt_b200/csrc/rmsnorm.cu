@@ -6,7 +6,7 @@
 //   residual_out = h
 // One rounding per output; nothing between the loads and the stores is narrower than fp32.  Rows whose
 // squares leave fp32's range (values beyond 1e16 or so, or below 1e-14 with an eps as small) are summed
-// again from scaled values: 0.4 us of 38.5 for having the code there.
+// again from scaled values; that the code is there takes 0.6 of the 39 us below.
 //
 // HBM-bound: 16-bit rows with a residual and an e4m3 output move 7 bytes per element for about
 // ten instructions.  A row lives in registers, ITEMS 16-byte vectors of x and of the residual per
@@ -353,7 +353,8 @@ int launch_rms(const RmsParams& p, Spread spread, cudaStream_t stream) {
     return cuda_check(cudaGetLastError(), "rmsnorm launch");
   };
   // Registers a thread: 64 fit 1024 threads.  Aligned rows do with that (bounds of 256 threads give them 68
-  // and seven CTAs of 128 instead of eight: 39.1 us, not 38.8), shifted ones spill (86: 70 us, 91: 66).
+  // and seven CTAs of 128 instead of eight: 39.1 us, not 38.8), shifted ones spill (rows of 4097 columns with bounds
+  // of 512: 76 us, of 256: 69).
   auto of = [&](auto spread) {
     constexpr int S = decltype(spread)::value;
     constexpr int SMALL = S == ALIGNED ? 512 : 256;
@@ -371,9 +372,9 @@ int dispatch_rms(RmsParams p, cudaStream_t stream) {
   // whether all rows of a tensor start where x's do, modulo the vector; `bytes` per element
   auto with_x = [&](const void* t, int64_t stride, int bytes) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(t), x = reinterpret_cast<uintptr_t>(p.x);
-    return at % bytes == 0 && (at / bytes - x / sizeof(T)) % E == 0 && (stride - p.stride_x) % E == 0;
+    return (at / bytes - x / sizeof(T)) % E == 0 && (stride - p.stride_x) % E == 0;
   };
-  bool together = reinterpret_cast<uintptr_t>(p.x) % sizeof(T) == 0 && at16(p.w);
+  bool together = at16(p.w);
   if (p.residual) together = together && with_x(p.residual, p.stride_residual, sizeof(T));
   if (p.residual_out) together = together && with_x(p.residual_out, p.stride_residual_out, sizeof(T));
   together = together && with_x(p.out, p.stride_out, E4M3 ? 1 : sizeof(T));
@@ -387,7 +388,7 @@ int dispatch_rms(RmsParams p, cudaStream_t stream) {
   int items = 1;
   // Few rows: as many threads as there are vectors, the row's latency counts (8 rows of 4096 bf16:
   // 2.7 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
-  // rows of 4096 fp16: 49.7 us with one, 41.5 with two, 40.2 with four; of 4097: 73 with two, 66).
+  // rows of 4096 fp16: 41.1 us with two, 38.9 with four; of 4097: 70.7 with two, 69.3).
   const int most = p.rows < 2 * device_info().sm_count ? 1 : 4;
   while (32 * items < vectors && items < most) items *= 2;
   while (1024 * items < vectors) items *= 2;
