@@ -383,7 +383,9 @@ def token_logprobs(logits, tokens=None, top=0, inv_temperature=1.0):
     for none and scores 0.  Returns TokenLogprobs of fp32 tensors (top_index: int64).
 
     Where gradients are enabled and the logits require one, logprob and entropy can be
-    differentiated (once; the logits are kept until then); a gradient of lse or top_logprob is refused."""
+    differentiated (once; the logits are kept until then); a gradient of lse or top_logprob is refused.
+    A backward pass can be captured into a graph while no eager graph of the same leaves is alive, as
+    any of torch's."""
     rows, vocab = _logits(logits)
     if tokens is not None:
         _vector("tokens", tokens, rows, torch.int64)
