@@ -100,7 +100,7 @@ __device__ __forceinline__ float2 e4m3x2_values(uint32_t q) {
 }
 
 // Exponent of the smallest power of two s with most <= 448 s, 448 = 1.75 * 2^8 being e4m3's largest
-// number: exact, from the bits.  0 and subnormals: -135.
+// number: exact, from the bits.  0 and subnormals: -135 or -134.
 __device__ __forceinline__ int e4m3_exponent(float most) {
   const uint32_t b = __float_as_uint(most);
   return (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
