@@ -17,7 +17,7 @@
 // ones e4m3's smallest step leaves an error of 2^-22 of the largest (fp16 2^-26).  Probabilities
 // keep 9 bits (two parts) or 14 (three): one more than a bf16 output has, three more than an fp16 one
 // (11 with the first part taken from fp16 too: 32 sequences with a window of 2048 in fp16 26.1 us, with 14 26.4;
-// bf16 with three parts of 14 bits: the same in bf16 25.0 -> 26.3, 28 rows 83.0 -> 89.5, for an output of 8 bits).
+// bf16 with three parts of 14 bits: the same in bf16 25.0 -> 26.3, 28 rows 84.4 -> 89.5, for an output of 8 bits).
 // The sums of a row take them unrounded: a token whose value scale is far below its tile's
 // largest rounds to nothing in the product, but weighs no less.  N = parts * rows, at least 16, was idle
 // anyway.
