@@ -410,11 +410,12 @@ __device__ __noinline__ void stage_queries(const KvAttnParams& p, Vec<T> raw, in
 
 // A token that some rows of the item see and others do not: NaN in its value row, `row` of the tile in
 // shared memory, becomes 0, as zero times NaN would reach the rows that do not see it; `noted` keeps the
-// columns for those that do.  Out of line: it runs at the ends of a window, for several query tokens
-// (32 sequences with a window of 2048 and four of them: 26.1 us, without 25.6).
+// columns for those that do.  The rows' positions are worked out anew: another warp may be staging the
+// item after the next one where this one's stood.  Out of line: it runs at the ends of a window, for
+// several query tokens (32 sequences with a window of 2048 and four of them: 26.1 us, without 25.6).
 template <int D, int RP>
-__device__ __noinline__ void set_nan_aside(const KvAttnParams& p, uint8_t* tile, int row, int token, const int* at,
-                                           uint32_t (*noted)[D / 32]) {
+__device__ __noinline__ void set_nan_aside(const KvAttnParams& p, uint8_t* tile, int row, int token, int first_at,
+                                           int row_tile, uint32_t (*noted)[D / 32]) {
   auto nan_bytes = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };   // 0x7f and 0xff
   uint32_t any = 0;
 #pragma unroll
@@ -439,9 +440,11 @@ __device__ __noinline__ void set_nan_aside(const KvAttnParams& p, uint8_t* tile,
       for (int b = 0; b < 4; ++b) columns |= (nan >> (8 * b + 7) & 1u) << b;
       const int first = i + 4 * k;
 #pragma unroll 1
-      for (int r = 0; r < RP; ++r)
-        if (token <= at[r] && (!p.window || token > at[r] - p.window || token < p.sinks))
+      for (int r = 0; r < RP; ++r) {
+        const int at = first_at + (row_tile * RP + r) / p.group;
+        if (token <= at && (!p.window || token > at - p.window || token < p.sinks))
           atomicOr(&noted[r][first / 32], columns << (first % 32));
+      }
     }
   }
 }
@@ -916,7 +919,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int i = 0; i < D; i += 16)     // neighbours start at different banks
               st_shared_v4(smem_u32(&sh.ring[g % SLOTS][me * D + ((i + me * 16) & (D - 1))]), 0, 0, 0, 0);
           } else if (!plain && ok) {
-            set_nan_aside<D, RP>(p, sh.ring[g % SLOTS], me, token, sh.q_at[item & 1], sh.nan[item & 1]);
+            set_nan_aside<D, RP>(p, sh.ring[g % SLOTS], me, token, c.seq.len - p.nq, c.at.row_tile, sh.nan[item & 1]);
           }
         }
         fence_proxy_async_smem();

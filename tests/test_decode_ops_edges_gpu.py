@@ -428,6 +428,27 @@ def test_attention_keeps_nan_from_one_item_to_the_next():
     _check_some_nan(got, q, cache, table, lengths, 0, 0)
 
 
+@pytest.mark.parametrize("group, nq, dtype", [(16, 20, FP16), (8, 20, BF16), (16, 9, BF16), (5, 33, FP16)])
+def test_attention_keeps_nan_within_its_item_while_the_next_ones_are_staged(group, nq, dtype):
+    """Items of one tile each, whose rows see the NaN of their sequence or see nothing, one after another:
+    some warps are two items further while others still look at the tile."""
+    gen = _gen(group + nq)
+    lengths = [1 + (i * 7) % (nq + 3) for i in range(60)]
+    table, total = _pages(gen, lengths, 16)
+    for d in (64, 128):
+        cache = _finite_cache(gen, total, 1, 16, d)
+        for b, n in enumerate(lengths):
+            for t in range(b % 2, n, 2):
+                codes = cache.v.view(torch.uint8)[table[b, t // 16].item(), 0, t % 16]
+                codes[torch.randint(0, d, (3,), generator=gen, device="cuda")] = 0x7F
+        q = _randn(gen, 60, nq, group, d, dtype=dtype)
+        at = _int32(lengths)
+        calls = [ops.kv_attention(q, cache, table, at) for _ in range(20)]
+        _check_some_nan(calls[0], q, cache, table, at, 0, 0)
+        for got in calls[1:]:
+            assert torch.equal(got.view(torch.int16), calls[0].view(torch.int16))
+
+
 def test_attention_of_more_rows_than_a_tile_keeps_nan_where_it_is_seen():
     """Row tiles of 16 rows, some of which none of a token's queries is in; parts of cut items."""
     gen = _gen(78)
