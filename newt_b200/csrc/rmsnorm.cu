@@ -6,13 +6,13 @@
 //   residual_out = h
 // One rounding per output; nothing between the loads and the stores is narrower than fp32.  Rows whose
 // squares leave fp32's range (values beyond 1e16 or so, or below 1e-14 with an eps as small) are summed
-// again from scaled values; that the code is there takes 0.6 of the 39 us below.
+// again from scaled values; that the code is there takes 0.4 of the 38.5 us below.
 //
 // HBM-bound: 16-bit rows with a residual and an e4m3 output move 7 bytes per element for about
 // ten instructions.  A row lives in registers, ITEMS 16-byte vectors of x and of the residual per
 // thread, so both are read once and all of a row's loads are in flight before its first use.
 // `threads` threads share a row (32: a warp per row, eight rows per CTA; more: one row per CTA): as
-// many warps as the row's vectors fill.  8191 x 4096 fp16 with a residual, e4m3 by 128 columns: 39 us
+// many warps as the row's vectors fill.  8191 x 4096 fp16 with a residual, e4m3 by 128 columns: 38.5 us
 // (6.0 TB/s); 8 x 4096 bf16: 2.7 us, one row's chain of loads and two reductions.
 // Nothing is prefetched across rows: the loads of the other resident CTAs cover a row's
 // reductions.  The weight is read through L1, where it stays: x and the residual do not allocate
@@ -29,7 +29,7 @@ namespace nb200 {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;
-constexpr float kLargestMean = 0x1p+110f, kLeastMean = 0x1p-96f;   // between them no square that counts leaves fp32's range
+constexpr float kLargestSum = 0x1p+120f, kLeastSum = 0x1p-80f;   // between them no square that counts leaves fp32's range
 constexpr int kMaxColumns = 32768;     // 32 values per thread are what 1024 threads have registers for
 constexpr int kMaxShifted = 16384;     // of shifted rows, which take a few registers more
 
@@ -210,10 +210,12 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
   for (int k = 0; k < ITEMS * E; ++k) sum = fmaf(v[k], v[k], sum);
   if (p.residual_out) write(static_cast<T*>(p.residual_out) + row * p.stride_residual_out, v, single);
   sum = reduce_row<Add>(sum, slots[0], warps);
-  float mean = sum / (float)n + p.eps;
-  if (__builtin_expect(!(mean < kLargestMean && mean >= kLeastMean), 0)) {       // the same in all threads of the row
+  float eps = p.eps;
+  // the same in all threads of the row
+  if (__builtin_expect(!(sum < kLargestSum && (sum >= kLeastSum || eps >= kLeastSum)), 0)) {
     // squares that left fp32's range, or a row of zeros, or one that is not finite: once more, scaled
-    const float f = mean < 1.0f ? 0x1p+96f : 0x1p-80f;
+    const float f = sum < 1.0f ? 0x1p+96f : 0x1p-80f;
+    eps = eps * f * f;
     single *= f;
     sum = single * single;
 #pragma unroll
@@ -223,9 +225,8 @@ __global__ void __launch_bounds__(MAX_THREADS) rms_kernel(const RmsParams p) {
     }
     if (warps > 1) __syncthreads();                         // the slots have been read
     sum = reduce_row<Add>(sum, slots[0], warps);
-    mean = sum / (float)n + p.eps * f * f;
   }
-  const float rstd = rsqrtf(mean);
+  const float rstd = rsqrtf(sum / (float)n + eps);
   read_weight(xv);
   if (has_alone) single = single * rstd * Elem<T>::to_f32(w[alone]);
 #pragma unroll
@@ -388,7 +389,7 @@ int dispatch_rms(RmsParams p, cudaStream_t stream) {
   int items = 1;
   // Few rows: as many threads as there are vectors, the row's latency counts (8 rows of 4096 bf16:
   // 2.7 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
-  // rows of 4096 fp16: 41.1 us with two, 38.9 with four; of 4097: 70.7 with two, 69.3).
+  // rows of 4096 fp16: 41.1 us with two, 38.5 with four; of 4097: 70.7 with two, 69.1).
   const int most = p.rows < 2 * device_info().sm_count ? 1 : 4;
   while (32 * items < vectors && items < most) items *= 2;
   while (1024 * items < vectors) items *= 2;
