@@ -13,7 +13,7 @@
 // thread, so both are read once and all of a row's loads are in flight before its first use.
 // `threads` threads share a row (32: a warp per row, eight rows per CTA; more: one row per CTA): as
 // many warps as the row's vectors fill.  8191 x 4096 fp16 with a residual, e4m3 by 128 columns: 38.5 us
-// (6.0 TB/s); 8 x 4096 bf16: 2.7 us, one row's chain of loads and two reductions.
+// (6.0 TB/s); 8 x 4096 bf16: 2.6 us, one row's chain of loads and two reductions.
 // Nothing is prefetched across rows: the loads of the other resident CTAs cover a row's
 // reductions.  The weight is read through L1, where it stays: x and the residual do not allocate
 // there.
@@ -388,7 +388,7 @@ int dispatch_rms(RmsParams p, cudaStream_t stream) {
   const int64_t vectors = spread == SHIFTED ? (p.n >= E ? p.n / E : 1) : cdiv64(p.n > 0 ? p.n : 1, E);
   int items = 1;
   // Few rows: as many threads as there are vectors, the row's latency counts (8 rows of 4096 bf16:
-  // 2.7 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
+  // 2.6 us).  Rows for every SM: four vectors of x and of the residual in flight per thread (8191
   // rows of 4096 fp16: 41.1 us with two, 38.5 with four; of 4097: 70.7 with two, 69.1).
   const int most = p.rows < 2 * device_info().sm_count ? 1 : 4;
   while (32 * items < vectors && items < most) items *= 2;

@@ -123,11 +123,11 @@ def _vector(name, t, length, dtype):
 
 def _no_backward(names, *tensors):
     """Refuses what would lose a gradient without a word."""
-    if torch.is_grad_enabled():
-        for name, t in zip(names.split(), tensors):
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"tensor '{name}' requires a gradient, but this operator has no backward "
-                                   "pass; call it under torch.no_grad() or give it a detached tensor")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            name = next(name for name, other in zip(names.split(), tensors) if other is t)
+            raise RuntimeError(f"tensor '{name}' requires a gradient, but this operator has no backward "
+                               "pass; call it under torch.no_grad() or give it a detached tensor")
 
 
 def _ptr(t):
@@ -161,7 +161,9 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, group=0, out=Non
     _rows("x", x, shape, dtype)
     _vector("weight", weight, n, dtype)
     _no_backward("x weight residual out scales residual_out", x, weight, residual, out, scales, residual_out)
-    given = [t for t in (out, scales, residual_out) if t is not None]
+    given = None
+    if out is not None or scales is not None or residual_out is not None:
+        given = [t for t in (out, scales, residual_out) if t is not None]
     if out is None:
         out = _fresh(x, out_dtype)
     else:
